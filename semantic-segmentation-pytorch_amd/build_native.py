@@ -13,7 +13,10 @@ LIB = os.path.join(OUT_DIR, 'libsemseg_hip.so')
 SOURCES = ['conv_igemm.hip', 'conv_wgrad.hip', 'conv_split.hip', 'weights_prep.hip', 'winograd.hip', 'bn.hip', 'pool_resize.hip', 'head.hip', 'input_pipeline.hip', 'depthwise.hip', 'grouped.hip', 'comm.hip', 'peer.hip', 'probe.hip', 'batch.hip', 'api.hip']
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-I' + os.path.join(ROOT, 'include'), '-I' + CSRC,
-         '-Wno-unused-result']
+         '-Wno-unused-result',
+         # no packed fp32 arithmetic (v_pk_add/mul/fma_f32): some of its forms have given wrong results on this hardware, now and then
+         # and without an error; -O3 makes them by itself from ordinary float code.  The host pass warns that it does not know the feature
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def _newer(a, b):

@@ -14,6 +14,14 @@
 #include "batch.h"
 #include <stdlib.h>
 
+// running statistics: two products and a sum, each rounded by itself.  Written without contraction so that every kernel that finishes
+// a BatchNorm (plain, min/max, fused, peer) leaves the same bits whatever the compiler fuses around it.
+__device__ __forceinline__ float bn_running(float momentum, float old, float value) {
+#pragma clang fp contract(off)
+    const float a = (1.f - momentum) * old, b = momentum * value;
+    return a + b;
+}
+
 // block = 256 threads arranged as cx channel-quads x py row lanes; grid = (quad groups, row chunks)
 struct ColGeom {
     int cx, py, gx, gy, rows_per_block;
@@ -155,10 +163,10 @@ __global__ void bn_finalize_kernel(const double* __restrict__ stats, int C, cons
     const float sc = gamma[c] * is;
     scale[c] = sc;
     shift[c] = beta[c] - muf * sc;
-    if (running_mean) running_mean[c] = (1.f - momentum) * running_mean[c] + momentum * muf;
+    if (running_mean) running_mean[c] = bn_running(momentum, running_mean[c], muf);
     if (running_var) {
         const double unbiased = n > 1.0 ? var * n / (n - 1.0) : var;
-        running_var[c] = (1.f - momentum) * running_var[c] + momentum * (float)unbiased;
+        running_var[c] = bn_running(momentum, running_var[c], (float)unbiased);
     }
 }
 
@@ -604,10 +612,10 @@ __global__ __launch_bounds__(256) void bn_finalize_mm_kernel(const double* __res
         const float sh = beta[c] - muf * sc;
         scale[c] = sc;
         shift[c] = sh;
-        if (running_mean) running_mean[c] = (1.f - momentum) * running_mean[c] + momentum * muf;
+        if (running_mean) running_mean[c] = bn_running(momentum, running_mean[c], muf);
         if (running_var) {
             const double unbiased = n > 1.0 ? var * n / (n - 1.0) : var;
-            running_var[c] = (1.f - momentum) * running_var[c] + momentum * (float)unbiased;
+            running_var[c] = bn_running(momentum, running_var[c], (float)unbiased);
         }
         const float e0 = fmaf(zmm[c], sc, sh), e1 = fmaf(zmm[C + c], sc, sh);
         const float hi = fmaxf(e0, e1) + rmax, lo = fminf(e0, e1) - rmax;
@@ -1328,10 +1336,10 @@ struct bn_fwd_finish_fused_kernel_body {
         const float sh = p_beta - muf * sc;
         scale[c] = sc;
         shift[c] = sh;
-        if (running_mean) running_mean[c] = (1.f - momentum) * p_rmean + momentum * muf;
+        if (running_mean) running_mean[c] = bn_running(momentum, p_rmean, muf);
         if (running_var) {
             const double unbiased = n > 1.0 ? var * n / (n - 1.0) : var;
-            running_var[c] = (1.f - momentum) * p_rvar + momentum * (float)unbiased;
+            running_var[c] = bn_running(momentum, p_rvar, (float)unbiased);
         }
         const float rmax = p_res;
         const float e0 = fmaf(lo, sc, sh), e1 = fmaf(hi, sc, sh);

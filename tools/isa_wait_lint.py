@@ -26,7 +26,7 @@ HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 
 def asm_of(src, out):
     cmd = [HIPCC, '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-I' + os.path.join(ROOT, 'include'), '-I' + CSRC,
-           '-Wno-unused-result', '--cuda-device-only', '-S', src, '-o', out]
+           '-Wno-unused-result', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '--cuda-device-only', '-S', src, '-o', out]
     subprocess.run(cmd, check=True, stderr=subprocess.DEVNULL)
     return out
 
