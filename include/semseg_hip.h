@@ -559,6 +559,87 @@ typedef struct {
 int semseg_sgd_step_fused(const semseg_sgd_tensor2* tensors_host, int n, const float* lr, float momentum,
                           float grad_scale, void* stream);
 
+/* ---------------- AdamW over many tensors (csrc/adamw.hip; beside the SGD step above: the reference's create_optimizers,
+ *                  train.py:115-127, knows SGD alone) -------------------------------------------------------------------------
+ * Element types of gradients and of 16-bit parameter copies. */
+#define SEMSEG_TYPE_F32  0
+#define SEMSEG_TYPE_BF16 1
+#define SEMSEG_TYPE_F16  2
+
+/* one parameter tensor: param, exp_avg, exp_avg_sq are numel floats in the same element order as grad (of grad_type); copy (may be
+ * NULL): numel elements of copy_type (BF16 or F16) that receive the updated parameters rounded to nearest even; step: the tensor's
+ * step count on the device, advanced by the call.  No two tensors of a call may share memory. */
+typedef struct {
+    void* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    void* copy;
+    int* step;
+    int64_t numel;
+    float weight_decay;
+    int grad_type, copy_type;
+} semseg_adamw_tensor;
+/* G = grad * grad_scale * clip[1];  m = b1 m + (1 - b1) G;  v = b2 v + (1 - b2) G^2;  t = ++step;
+ * p -= lr wd p + lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps).
+ * lr: device scalar.  clip (may be NULL): the two floats of semseg_grad_norm; where its norm is not finite the call changes nothing.
+ * workspace: semseg_adamw_workspace_bytes(n), 16-byte aligned, not shared with a call that may run at the same time. */
+size_t semseg_adamw_workspace_bytes(int n);
+int semseg_adamw_step(const semseg_adamw_tensor* tensors_host, int n, const float* lr, double beta1, double beta2, double eps,
+                      float grad_scale, const float* clip, void* workspace, size_t workspace_bytes, void* stream);
+
+/* the same step with states in 8 bits: m_codes, r_codes: numel e4m3 codes of m and of r = sqrt(v); m_scales, r_scales: one float per
+ * 256 elements (ceil(numel / 256)), value = code * scale.  Codes are rounded stochastically from a counter hash of (seed, step, index
+ * of the tensor in the call, element): the same call leaves the same bits.  A block that is not finite gets a NaN scale. */
+typedef struct {
+    void* param;
+    const void* grad;
+    void* copy;
+    void* m_codes;
+    void* m_scales;
+    void* r_codes;
+    void* r_scales;
+    int* step;
+    int64_t numel;
+    float weight_decay;
+    int grad_type, copy_type;
+} semseg_adamw8_tensor;
+int semseg_adamw8_step(const semseg_adamw8_tensor* tensors_host, int n, const float* lr, double beta1, double beta2, double eps,
+                       float grad_scale, const float* clip, uint32_t seed, void* workspace, size_t workspace_bytes, void* stream);
+
+/* global 2-norm of n gradient tensors (types may differ): out[0] = norm of grad * grad_scale, out[1] = min(1, max_norm / (norm + 1e-6))
+ * (1 where max_norm < 0), 0 where the norm is not finite.  Squares are summed in 64 bits in a fixed order. */
+typedef struct {
+    const void* grad;
+    int64_t numel;
+    int grad_type;
+} semseg_grad_tensor;
+size_t semseg_grad_norm_workspace_bytes(const semseg_grad_tensor* tensors_host, int n);
+int semseg_grad_norm(const semseg_grad_tensor* tensors_host, int n, float grad_scale, float max_norm, float* out, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* ---------------- log probability of chosen labels, clipped policy loss with a KL term (csrc/policy.hip; beside log_softmax / NLL,
+ *                  models.py:383,492, train.py:154) -----------------------------------------------------------------------------
+ * z: P rows of C logits of `type` (SEMSEG_TYPE_*), ld >= C elements apart.  A row is valid where its label is not ignore_index and
+ * inside [0, C).  stats: 2 P floats (maximum, logarithm of the sum of exponentials below it) for the backward call; may be NULL in
+ * semseg_label_logp_fwd.
+ * label_logp_fwd: lp[row] = log softmax(z)[label], 0 for rows that are not valid.
+ * policy_loss_fwd: ratio = exp(lp - old_logp); loss = mean over valid rows of -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
+ *   + kl_weight (exp(ref_logp - lp) - (ref_logp - lp) - 1), A = advantage[row / rows_per_advantage]; kl = the mean KL term, clipped =
+ *   the share of rows that are clipped, inv_count = 1 / valid rows (one float each, all 0 without a valid row); coef: P floats for
+ *   the backward call.
+ * label_logp_bwd: dz (P x C dense, z's type) = g[row] * s * (1[c = label] - softmax(z)[c]), s = gloss[0] * inv_count[0] where gloss is
+ *   given (the policy loss: g = coef, inv_count as it left it), else 1; rows that are not valid get zeros. */
+int semseg_label_logp_fwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, int64_t P, int C, float* lp,
+                          float* stats, void* stream);
+size_t semseg_policy_loss_workspace_bytes(void);
+int semseg_policy_loss_fwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, int64_t P, int C,
+                           const float* advantage, int64_t rows_per_advantage, const float* old_logp, const float* ref_logp,
+                           float clip_low, float clip_high, float kl_weight, float* stats, float* coef, float* loss, float* kl, float* clipped,
+                           float* inv_count, void* workspace, size_t workspace_bytes, void* stream);
+int semseg_label_logp_bwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, const float* stats,
+                          const float* g, const float* gloss, const float* inv_count, int64_t P, int C, void* dz, void* stream);
+
 /* ---------------- collectives over RCCL / xGMI ------------------------------------
  * Replace the reference's single-process thread rendezvous: lib/nn/modules/comm.py:46-131 (SyncMaster / SlavePipe queues),
  * lib/nn/modules/batchnorm.py:98-117 (_data_parallel_master: reduce sum / ssum to device 0, broadcast mean / inv_std) and the

@@ -1,0 +1,516 @@
+// AdamW over many tensors at once, states in 32 bits or in 8 (adamw_math.h has the mathematics), and the global norm of many
+// gradients (gfx950).  The framework's other optimiser is sgd_fused_kernel (head.hip).
+//
+// Bound: HBM.  A step with f32 gradients moves 28 bytes an element with states in 32 bits (p, m, v both ways, g once) and 16 with
+// states in 8 bits; the norm moves the gradients once.  Layout of the work: every tensor is cut into chunks, a launch is the chunks of
+// up to ADAM_MAX_TENSORS tensors one after the other, and a block finds its tensor by a binary search in the kernel arguments, so no
+// block is launched for nothing and no tensor needs a launch of its own.  The step count, the learning rate and the clip factor are
+// device memory: a captured graph can be replayed.
+#include "common.h"
+#include "adamw_math.h"
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int ADAM_MAX_TENSORS = 48;
+constexpr int ADAM_CHUNK = 4096;           // elements of a block: 4 quads a thread, all their loads in flight at once
+constexpr int ADAM_QUADS = ADAM_CHUNK / (256 * 4);
+
+static bool type_ok(int t) { return t == SEMSEG_TYPE_F32 || t == SEMSEG_TYPE_BF16 || t == SEMSEG_TYPE_F16; }
+static int type_bytes(int t) { return t == SEMSEG_TYPE_F32 ? 4 : 2; }
+static bool aligned_to(const void* p, int bytes) { return (((uintptr_t)p) & (uintptr_t)(bytes - 1)) == 0; }
+
+// four gradients from element 4 * quad; `type` is the same for the whole block
+__device__ __forceinline__ f32x4 load_quad(const void* g, int type, int64_t quad) {
+    if (type == SEMSEG_TYPE_F32) return reinterpret_cast<const f32x4*>(g)[quad];
+    if (type == SEMSEG_TYPE_BF16) return __builtin_convertvector(reinterpret_cast<const bf16x4*>(g)[quad], f32x4);
+    return __builtin_convertvector(reinterpret_cast<const f16x4*>(g)[quad], f32x4);
+}
+__device__ __forceinline__ float load_one(const void* g, int type, int64_t i) {
+    if (type == SEMSEG_TYPE_F32) return reinterpret_cast<const float*>(g)[i];
+    if (type == SEMSEG_TYPE_BF16) return (float)reinterpret_cast<const __bf16*>(g)[i];
+    return (float)reinterpret_cast<const _Float16*>(g)[i];
+}
+// the 16-bit copy of the updated parameters, rounded to nearest even from the f32 values
+__device__ __forceinline__ void store_quad(void* c, int type, int64_t quad, f32x4 v) {
+    if (type == SEMSEG_TYPE_BF16) reinterpret_cast<bf16x4*>(c)[quad] = __builtin_convertvector(v, bf16x4);
+    else reinterpret_cast<f16x4*>(c)[quad] = __builtin_convertvector(v, f16x4);
+}
+__device__ __forceinline__ void store_one(void* c, int type, int64_t i, float v) {
+    if (type == SEMSEG_TYPE_BF16) reinterpret_cast<__bf16*>(c)[i] = (__bf16)v;
+    else reinterpret_cast<_Float16*>(c)[i] = (_Float16)v;
+}
+
+// the tensor whose chunks hold block `b`: the last one whose first chunk is not behind it
+template <class B>
+__device__ __forceinline__ int tensor_of(const B& batch, uint32_t b) {
+    int lo = 0, hi = batch.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (batch.first[mid] <= b) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// ---------------------------------------------------------------- step counts and coefficients --------------------------------
+constexpr int BEGIN_MAX = 240;
+struct BeginBatch {
+    int* step[BEGIN_MAX];
+    float wd[BEGIN_MAX];
+    int n, base;
+};
+static_assert(sizeof(BeginBatch) <= 4000, "kernel arguments");
+
+__global__ __launch_bounds__(256) void adamw_begin_kernel(const BeginBatch b, const float* __restrict__ lr, double log_b1, double log_b2,
+                                                          float grad_scale, const float* __restrict__ clip, uint32_t seed,
+                                                          AdamCoef* __restrict__ coef) {
+    const int i = threadIdx.x;
+    if (i >= b.n) return;
+    float factor = grad_scale;
+    bool skip = false;
+    if (clip) {                                              // [norm, factor] of semseg_grad_norm
+        skip = !(fabsf(clip[0]) <= 3.402823466e38f);
+        factor *= clip[1];
+    }
+    int t = *b.step[i];
+    if (!skip) {
+        t += 1;
+        *b.step[i] = t;
+    }
+    AdamCoef c = adam_coef((double)lr[0], log_b1, log_b2, (double)b.wd[i], t, factor, seed, (uint32_t)(b.base + i));
+    if (skip) c.root = 0.f;
+    coef[b.base + i] = c;
+}
+
+static size_t coef_bytes(int n) { return (size_t)n * sizeof(AdamCoef); }
+
+template <class TENSOR>
+static int begin_step(const TENSOR* t, int n, const float* lr, double beta1, double beta2, float grad_scale, const float* clip,
+                      uint32_t seed, AdamCoef* coef, hipStream_t st) {
+    const double l1 = log(beta1), l2 = log(beta2);           // beta 0: -infinity, 1 - 0^t = 1
+    for (int base = 0; base < n; base += BEGIN_MAX) {
+        BeginBatch b;
+        b.n = min(BEGIN_MAX, n - base);
+        b.base = base;
+        for (int i = 0; i < b.n; ++i) {
+            b.step[i] = t[base + i].step;
+            b.wd[i] = t[base + i].weight_decay;
+        }
+        hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(256), 0, st, b, lr, l1, l2, grad_scale, clip, seed, coef);
+        SEMSEG_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+static bool hyper_ok(double beta1, double beta2, double eps) {
+    return beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0 && eps <= 3.402823466e38;
+}
+static AdamHyper hyper_of(double beta1, double beta2, double eps) {
+    AdamHyper h;
+    h.b1 = (float)beta1; h.c1 = (float)(1.0 - beta1); h.b2 = (float)beta2; h.c2 = (float)(1.0 - beta2); h.eps = (float)eps;
+    return h;
+}
+
+// ---------------------------------------------------------------- states in 32 bits -------------------------------------------
+struct AdamEntry {
+    float* p; const void* g; float* m; float* v; void* c;
+    int64_t numel;
+    int index;                 // of its AdamCoef
+    uint8_t gtype, ctype, vec, pad;
+};
+struct AdamBatch {
+    AdamEntry t[ADAM_MAX_TENSORS];
+    uint32_t first[ADAM_MAX_TENSORS];
+    int n;
+};
+static_assert(sizeof(AdamBatch) <= 4000, "kernel arguments");
+
+__global__ __launch_bounds__(256) void adamw_kernel(const AdamBatch b, const AdamCoef* __restrict__ coef, AdamHyper h) {
+    const int k = tensor_of(b, blockIdx.x);
+    const AdamEntry t = b.t[k];
+    const AdamCoef c = coef[t.index];
+    if (c.root == 0.f) return;
+    const int64_t start = (int64_t)(blockIdx.x - b.first[k]) * ADAM_CHUNK;
+    const int tid = threadIdx.x;
+    if (t.vec && start + ADAM_CHUNK <= t.numel) {
+        const int64_t q0 = (start >> 2) + tid;
+        f32x4* p4 = reinterpret_cast<f32x4*>(t.p);
+        f32x4* m4 = reinterpret_cast<f32x4*>(t.m);
+        f32x4* v4 = reinterpret_cast<f32x4*>(t.v);
+        f32x4 p[ADAM_QUADS], g[ADAM_QUADS], m[ADAM_QUADS], v[ADAM_QUADS];
+#pragma unroll
+        for (int u = 0; u < ADAM_QUADS; ++u) {
+            g[u] = load_quad(t.g, t.gtype, q0 + u * 256);
+            m[u] = m4[q0 + u * 256];
+            v[u] = v4[q0 + u * 256];
+            p[u] = p4[q0 + u * 256];
+        }
+#pragma unroll
+        for (int u = 0; u < ADAM_QUADS; ++u) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float pj = p[u][j], mj = m[u][j], vj = v[u][j];
+                adam_update32(pj, g[u][j], mj, vj, c, h);
+                p[u][j] = pj; m[u][j] = mj; v[u][j] = vj;
+            }
+            m4[q0 + u * 256] = m[u];
+            v4[q0 + u * 256] = v[u];
+            p4[q0 + u * 256] = p[u];
+            if (t.c) store_quad(t.c, t.ctype, q0 + u * 256, p[u]);
+        }
+        return;
+    }
+    // the last chunk of a tensor, and tensors that start at an odd address
+    const int64_t end = min(t.numel, start + ADAM_CHUNK);
+    for (int64_t i = start + tid; i < end; i += 256) {
+        float p = t.p[i], m = t.m[i], v = t.v[i];
+        adam_update32(p, load_one(t.g, t.gtype, i), m, v, c, h);
+        t.m[i] = m;
+        t.v[i] = v;
+        t.p[i] = p;
+        if (t.c) store_one(t.c, t.ctype, i, p);
+    }
+}
+
+extern "C" size_t semseg_adamw_workspace_bytes(int n) { return n > 0 ? coef_bytes(n) : 0; }
+
+extern "C" int semseg_adamw_step(const semseg_adamw_tensor* tensors_host, int n, const float* lr, double beta1, double beta2, double eps,
+                                 float grad_scale, const float* clip, void* workspace, size_t workspace_bytes, void* stream) {
+    if (n < 0 || (n && (!tensors_host || !lr)) || !hyper_ok(beta1, beta2, eps)) return SEMSEG_EINVAL;
+    for (int i = 0; i < n; ++i) {
+        const semseg_adamw_tensor& t = tensors_host[i];
+        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || !t.step || t.numel <= 0 || !type_ok(t.grad_type) ||
+            (t.copy && (!type_ok(t.copy_type) || t.copy_type == SEMSEG_TYPE_F32)))
+            return SEMSEG_EINVAL;
+        if ((t.numel + ADAM_CHUNK - 1) / ADAM_CHUNK > (int64_t)1 << 30) return SEMSEG_EINVAL;
+    }
+    if (n == 0) return 0;
+    if (!workspace || workspace_bytes < coef_bytes(n) || !aligned16(workspace)) return SEMSEG_EWORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    AdamCoef* coef = (AdamCoef*)workspace;
+    if (int rc = begin_step(tensors_host, n, lr, beta1, beta2, grad_scale, clip, 0u, coef, st)) return rc;
+    const AdamHyper h = hyper_of(beta1, beta2, eps);
+    for (int i = 0; i < n;) {
+        AdamBatch b;
+        b.n = 0;
+        uint32_t chunks = 0;
+        for (; i < n && b.n < ADAM_MAX_TENSORS; ++i) {
+            const semseg_adamw_tensor& t = tensors_host[i];
+            const int64_t c = (t.numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
+            if (chunks + c > (int64_t)1 << 30) break;       // (a launch of its own holds any tensor: checked above)
+            AdamEntry& e = b.t[b.n];
+            e.p = (float*)t.param; e.g = t.grad; e.m = (float*)t.exp_avg; e.v = (float*)t.exp_avg_sq; e.c = t.copy;
+            e.numel = t.numel;
+            e.index = i;
+            e.gtype = (uint8_t)t.grad_type; e.ctype = (uint8_t)t.copy_type;
+            e.vec = aligned16(t.param) && aligned16(t.exp_avg) && aligned16(t.exp_avg_sq) && aligned_to(t.grad, 4 * type_bytes(t.grad_type)) &&
+                    (!t.copy || aligned_to(t.copy, 8));
+            e.pad = 0;
+            b.first[b.n++] = chunks;
+            chunks += (uint32_t)c;
+        }
+        hipLaunchKernelGGL(adamw_kernel, dim3(chunks), dim3(256), 0, st, b, coef, h);
+        SEMSEG_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+// ---------------------------------------------------------------- states in 8 bits --------------------------------------------
+// A wave owns a block of 256 elements (one scale): 4 elements a lane, the block's maxima of |m| and r by shuffles, so the states are
+// read and written once and never leave the registers in between.
+constexpr int ADAM8_MAX_TENSORS = 44;
+constexpr int ADAM8_PER_WAVE = 4;                                     // blocks of a wave, their loads in flight together
+constexpr int ADAM8_CHUNK = 4 * ADAM8_PER_WAVE * ADAM8_BLOCK;         // elements of a thread block
+
+struct Adam8Entry {
+    float* p; const void* g; void* c; uint8_t* m; float* ms; uint8_t* r; float* rs;
+    int64_t numel;
+    int index;
+    uint8_t gtype, ctype, vec, pad;
+};
+struct Adam8Batch {
+    Adam8Entry t[ADAM8_MAX_TENSORS];
+    uint32_t first[ADAM8_MAX_TENSORS];
+    int n;
+};
+static_assert(sizeof(Adam8Batch) <= 4000, "kernel arguments");
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    return v;
+}
+// one e4m3 code of a value that e4m3 holds exactly
+__device__ __forceinline__ uint8_t code_of(float a) { return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(a, 0.f, 0, false) & 0xff); }
+__device__ __forceinline__ float value_of(uint8_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
+__device__ __forceinline__ uint32_t codes_of(const float a[4]) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a[0], a[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a[2], a[3], w, true);
+}
+
+// m and r of one block after the update (4 elements a lane, elements that do not exist are 0) -> scales and rounded values
+__device__ __forceinline__ void adam8_block(float m[4], float r[4], const uint32_t at[4], const AdamCoef& c, float& ms, float& rs) {
+    uint32_t tm = 0, tr = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        tm = max(tm, adam_bits(fabsf(m[j])));
+        tr = max(tr, adam_bits(fabsf(r[j])));
+    }
+    ms = adam8_scale(wave_max_u32(tm));
+    rs = adam8_scale(wave_max_u32(tr));
+    const float im = adam8_inverse(ms), ir = adam8_inverse(rs);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t bits = adam_mix(at[j] + c.base);
+        m[j] = copysignf(adam8_round(m[j], im, bits & 0xffffu, false), m[j]);
+        r[j] = adam8_round(r[j], ir, bits >> 16, true);
+    }
+}
+
+__global__ __launch_bounds__(256) void adamw8_kernel(const Adam8Batch b, const AdamCoef* __restrict__ coef, AdamHyper h) {
+    const int k = tensor_of(b, blockIdx.x);
+    const Adam8Entry t = b.t[k];
+    const AdamCoef c = coef[t.index];
+    if (c.root == 0.f) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t start = (int64_t)(blockIdx.x - b.first[k]) * ADAM8_CHUNK + (threadIdx.x >> 6) * (ADAM8_PER_WAVE * ADAM8_BLOCK);
+    if (t.vec && start + ADAM8_PER_WAVE * ADAM8_BLOCK <= t.numel) {
+        const int64_t q0 = (start >> 2) + lane;
+        f32x4* p4 = reinterpret_cast<f32x4*>(t.p);
+        uint32_t* m4 = reinterpret_cast<uint32_t*>(t.m);
+        uint32_t* r4 = reinterpret_cast<uint32_t*>(t.r);
+        f32x4 p[ADAM8_PER_WAVE], g[ADAM8_PER_WAVE];
+        uint32_t mc[ADAM8_PER_WAVE], rc[ADAM8_PER_WAVE];
+        float ms[ADAM8_PER_WAVE], rs[ADAM8_PER_WAVE];
+#pragma unroll
+        for (int u = 0; u < ADAM8_PER_WAVE; ++u) {
+            g[u] = load_quad(t.g, t.gtype, q0 + u * 64);
+            p[u] = p4[q0 + u * 64];
+            mc[u] = m4[q0 + u * 64];
+            rc[u] = r4[q0 + u * 64];
+            ms[u] = t.ms[(start >> 8) + u];
+            rs[u] = t.rs[(start >> 8) + u];
+        }
+#pragma unroll
+        for (int u = 0; u < ADAM8_PER_WAVE; ++u) {
+            float m[4], r[4];
+            uint32_t at[4];
+            m[0] = __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 0); m[1] = __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 1);
+            m[2] = __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 2); m[3] = __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 3);
+            r[0] = __builtin_amdgcn_cvt_f32_fp8((int)rc[u], 0); r[1] = __builtin_amdgcn_cvt_f32_fp8((int)rc[u], 1);
+            r[2] = __builtin_amdgcn_cvt_f32_fp8((int)rc[u], 2); r[3] = __builtin_amdgcn_cvt_f32_fp8((int)rc[u], 3);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                at[j] = (uint32_t)((q0 + u * 64) * 4 + j);
+                float pj = p[u][j];
+                m[j] *= ms[u];
+                r[j] *= rs[u];
+                adam_update8(pj, g[u][j], m[j], r[j], c, h);
+                p[u][j] = pj;
+            }
+            float msn, rsn;
+            adam8_block(m, r, at, c, msn, rsn);
+            p4[q0 + u * 64] = p[u];
+            m4[q0 + u * 64] = codes_of(m);
+            r4[q0 + u * 64] = codes_of(r);
+            if (lane == 0) {
+                t.ms[(start >> 8) + u] = msn;
+                t.rs[(start >> 8) + u] = rsn;
+            }
+            if (t.c) store_quad(t.c, t.ctype, q0 + u * 64, p[u]);
+        }
+        return;
+    }
+    // the last blocks of a tensor, and tensors that start at an odd address: element lane + 64 j of the block
+    for (int u = 0; u < ADAM8_PER_WAVE; ++u) {
+        const int64_t s = start + u * ADAM8_BLOCK;
+        if (s >= t.numel) return;                            // the same for the whole wave
+        const float ms = t.ms[s >> 8], rs = t.rs[s >> 8];
+        float m[4], r[4], p[4];
+        uint32_t at[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t i = s + lane + 64 * j;
+            at[j] = (uint32_t)i;
+            m[j] = r[j] = p[j] = 0.f;
+            if (i < t.numel) {
+                p[j] = t.p[i];
+                m[j] = value_of(t.m[i]) * ms;
+                r[j] = value_of(t.r[i]) * rs;
+                adam_update8(p[j], load_one(t.g, t.gtype, i), m[j], r[j], c, h);
+            }
+        }
+        float msn, rsn;
+        adam8_block(m, r, at, c, msn, rsn);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t i = s + lane + 64 * j;
+            if (i < t.numel) {
+                t.p[i] = p[j];
+                t.m[i] = code_of(m[j]);
+                t.r[i] = code_of(r[j]);
+                if (t.c) store_one(t.c, t.ctype, i, p[j]);
+            }
+        }
+        if (lane == 0) {
+            t.ms[s >> 8] = msn;
+            t.rs[s >> 8] = rsn;
+        }
+    }
+}
+
+extern "C" int semseg_adamw8_step(const semseg_adamw8_tensor* tensors_host, int n, const float* lr, double beta1, double beta2, double eps,
+                                  float grad_scale, const float* clip, uint32_t seed, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+    if (n < 0 || (n && (!tensors_host || !lr)) || !hyper_ok(beta1, beta2, eps)) return SEMSEG_EINVAL;
+    for (int i = 0; i < n; ++i) {
+        const semseg_adamw8_tensor& t = tensors_host[i];
+        if (!t.param || !t.grad || !t.m_codes || !t.m_scales || !t.r_codes || !t.r_scales || !t.step || t.numel <= 0 ||
+            !type_ok(t.grad_type) || (t.copy && (!type_ok(t.copy_type) || t.copy_type == SEMSEG_TYPE_F32)))
+            return SEMSEG_EINVAL;
+        if ((t.numel + ADAM8_CHUNK - 1) / ADAM8_CHUNK > (int64_t)1 << 30) return SEMSEG_EINVAL;
+    }
+    if (n == 0) return 0;
+    if (!workspace || workspace_bytes < coef_bytes(n) || !aligned16(workspace)) return SEMSEG_EWORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    AdamCoef* coef = (AdamCoef*)workspace;
+    if (int rc = begin_step(tensors_host, n, lr, beta1, beta2, grad_scale, clip, seed, coef, st)) return rc;
+    const AdamHyper h = hyper_of(beta1, beta2, eps);
+    for (int i = 0; i < n;) {
+        Adam8Batch b;
+        b.n = 0;
+        uint32_t chunks = 0;
+        for (; i < n && b.n < ADAM8_MAX_TENSORS; ++i) {
+            const semseg_adamw8_tensor& t = tensors_host[i];
+            const int64_t c = (t.numel + ADAM8_CHUNK - 1) / ADAM8_CHUNK;
+            if (chunks + c > (int64_t)1 << 30) break;
+            Adam8Entry& e = b.t[b.n];
+            e.p = (float*)t.param; e.g = t.grad; e.c = t.copy;
+            e.m = (uint8_t*)t.m_codes; e.ms = (float*)t.m_scales; e.r = (uint8_t*)t.r_codes; e.rs = (float*)t.r_scales;
+            e.numel = t.numel;
+            e.index = i;
+            e.gtype = (uint8_t)t.grad_type; e.ctype = (uint8_t)t.copy_type;
+            e.vec = aligned16(t.param) && aligned_to(t.m_codes, 4) && aligned_to(t.r_codes, 4) &&
+                    aligned_to(t.grad, 4 * type_bytes(t.grad_type)) && (!t.copy || aligned_to(t.copy, 8));
+            e.pad = 0;
+            b.first[b.n++] = chunks;
+            chunks += (uint32_t)c;
+        }
+        hipLaunchKernelGGL(adamw8_kernel, dim3(chunks), dim3(256), 0, st, b, coef, h);
+        SEMSEG_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+// ---------------------------------------------------------------- global norm -------------------------------------------------
+// Squares are summed in 64 bits (an f32 square leaves the range at 2e19 and below 1e-23), one partial sum per chunk in a fixed order,
+// then one block sums the partials: the same bits every time.
+constexpr int NORM_MAX_TENSORS = 140;
+constexpr int NORM_CHUNK = 16384;
+struct NormEntry {
+    const void* g;
+    int64_t numel;
+    uint8_t type, vec, pad[6];
+};
+struct NormBatch {
+    NormEntry t[NORM_MAX_TENSORS];
+    uint32_t first[NORM_MAX_TENSORS];
+    int n;
+};
+static_assert(sizeof(NormBatch) <= 4000, "kernel arguments");
+
+__device__ __forceinline__ void add_square(double& s, float x) { const double d = (double)x; s = fma(d, d, s); }
+
+__global__ __launch_bounds__(256) void grad_norm_kernel(const NormBatch b, double* __restrict__ partial) {
+    __shared__ double sum[4];
+    const int k = tensor_of(b, blockIdx.x);
+    const NormEntry t = b.t[k];
+    const int64_t start = (int64_t)(blockIdx.x - b.first[k]) * NORM_CHUNK;
+    const int64_t end = min(t.numel, start + NORM_CHUNK);
+    double s = 0.0;
+    if (t.vec && start + NORM_CHUNK <= t.numel) {
+        const int64_t q0 = (start >> 2) + threadIdx.x;
+        for (int u = 0; u < NORM_CHUNK / 1024; u += 8) {
+            f32x4 g[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j] = load_quad(t.g, t.type, q0 + (u + j) * 256);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                add_square(s, g[j][0]); add_square(s, g[j][1]); add_square(s, g[j][2]); add_square(s, g[j][3]);
+            }
+        }
+    } else {
+        for (int64_t i = start + threadIdx.x; i < end; i += 256) add_square(s, load_one(t.g, t.type, i));
+    }
+    s = wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[blockIdx.x] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+__global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double* __restrict__ partial, int64_t n, float grad_scale, float max_norm,
+                                                                float* __restrict__ out) {
+    __shared__ double sum[16];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += partial[i];
+    s = wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double total = 0.0;
+        for (int i = 0; i < 16; ++i) total += sum[i];
+        const double norm = sqrt(total) * fabs((double)grad_scale);
+        const float f = (float)norm;
+        float factor = 1.f;
+        if (max_norm >= 0.f) factor = (float)fmin(1.0, (double)max_norm / (norm + 1e-6));
+        out[0] = f;
+        out[1] = fabsf(f) <= 3.402823466e38f ? factor : 0.f;
+    }
+}
+
+static int64_t norm_chunks(int64_t numel) { return (numel + NORM_CHUNK - 1) / NORM_CHUNK; }
+
+extern "C" size_t semseg_grad_norm_workspace_bytes(const semseg_grad_tensor* tensors_host, int n) {
+    int64_t chunks = 0;
+    for (int i = 0; tensors_host && i < n; ++i) chunks += tensors_host[i].numel > 0 ? norm_chunks(tensors_host[i].numel) : 0;
+    return (size_t)(chunks ? chunks : 1) * sizeof(double);
+}
+
+extern "C" int semseg_grad_norm(const semseg_grad_tensor* tensors_host, int n, float grad_scale, float max_norm, float* out, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+    if (n < 0 || (n && !tensors_host) || !out) return SEMSEG_EINVAL;
+    for (int i = 0; i < n; ++i) {
+        const semseg_grad_tensor& t = tensors_host[i];
+        if (!t.grad || t.numel <= 0 || !type_ok(t.grad_type) || norm_chunks(t.numel) > (int64_t)1 << 30) return SEMSEG_EINVAL;
+    }
+    if (!workspace || workspace_bytes < semseg_grad_norm_workspace_bytes(tensors_host, n)) return SEMSEG_EWORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    double* partial = (double*)workspace;
+    int64_t done = 0;
+    for (int i = 0; i < n;) {
+        NormBatch b;
+        b.n = 0;
+        uint32_t chunks = 0;
+        for (; i < n && b.n < NORM_MAX_TENSORS; ++i) {
+            const semseg_grad_tensor& t = tensors_host[i];
+            const int64_t c = norm_chunks(t.numel);
+            if (chunks + c > (int64_t)1 << 30) break;
+            NormEntry& e = b.t[b.n];
+            e.g = t.grad;
+            e.numel = t.numel;
+            e.type = (uint8_t)t.grad_type;
+            e.vec = aligned_to(t.grad, 4 * type_bytes(t.grad_type));
+            for (int j = 0; j < 6; ++j) e.pad[j] = 0;
+            b.first[b.n++] = chunks;
+            chunks += (uint32_t)c;
+        }
+        hipLaunchKernelGGL(grad_norm_kernel, dim3(chunks), dim3(256), 0, st, b, partial + done);
+        SEMSEG_LAUNCH_CHECK();
+        done += chunks;
+    }
+    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(1024), 0, st, (const double*)partial, done, grad_scale, max_norm, out);
+    SEMSEG_LAUNCH_CHECK();
+    return 0;
+}

@@ -1,0 +1,111 @@
+// Per-element arithmetic of the AdamW kernels (adamw.hip) as plain inline functions, so that tests/native/adamw_emulate.cpp runs the
+// SAME code on the host (see depthwise_math.h for the pattern).
+//
+//   m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2      p = p - lr wd p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// States in 8 bits: m and r = sqrt(v) are e4m3 codes (4 exponent bits, 3 mantissa bits, largest value 448) of blocks of 256 elements
+// with one f32 scale each, scale = absmax / 448.  r and not v: v spans the square of r's range, which 8 bits do not.
+// Rounding is stochastic: between two steps r moves by at most (1 - b2) / 2 = 0.05 % of itself towards a new level, a nearest
+// rounding of 3 mantissa bits moves only at 6 %, so r would stay where it is for ever; a rounding that goes up with the probability of
+// the cut-off fraction is right on average.  Its random bits are a counter hash of (seed, step, tensor, element): the same call gives
+// the same bits on every machine.  A positive r never rounds to zero (it divides).
+#pragma once
+#include <stdint.h>
+#include <string.h>
+#include <math.h>
+
+#ifndef SEMSEG_HD
+#ifdef __HIPCC__
+#define SEMSEG_HD __host__ __device__ __forceinline__
+#else
+#define SEMSEG_HD static inline
+#endif
+#endif
+
+constexpr int ADAM8_BLOCK = 256;                 // elements that share one scale
+constexpr float ADAM8_MAX = 448.0f;              // largest e4m3 value
+constexpr float ADAM8_TINY = 7.888609052210118e-31f;      // 2^-100: a block below it is stored as zeros (its scale would lose bits)
+
+// what one step needs per tensor, computed once per call on the device (adamw_begin_kernel): the step count lives there
+struct AdamCoef {
+    float size;        // lr / (1 - b1^t)
+    float root;        // 1 / sqrt(1 - b2^t); 0: leave the tensor alone (the gradients are not finite)
+    float factor;      // what the gradient is multiplied with
+    float decay;       // lr * weight decay
+    uint32_t base;     // counter base of the random bits
+    uint32_t pad[3];
+};
+struct AdamHyper {
+    float b1, c1, b2, c2, eps;      // c = 1 - b, formed in double
+};
+
+SEMSEG_HD uint32_t adam_bits(float x) { uint32_t u; memcpy(&u, &x, 4); return u; }
+SEMSEG_HD float adam_float(uint32_t u) { float x; memcpy(&x, &u, 4); return x; }
+
+// 32 bits scrambled: xor-shifts and odd multipliers (the fractional bits of sqrt 2 and sqrt 3); a bijection
+SEMSEG_HD uint32_t adam_mix(uint32_t x) {
+    x ^= x >> 16;
+    x *= 0x6A09E667u;
+    x ^= x >> 15;
+    x *= 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+
+// the coefficients of step t (t >= 1) of one tensor; double: 1 - b^t cancels for small t
+SEMSEG_HD AdamCoef adam_coef(double lr, double log_b1, double log_b2, double wd, int t, float factor, uint32_t seed, uint32_t ordinal) {
+    AdamCoef c;
+    c.size = (float)(lr / -expm1((double)t * log_b1));
+    c.root = (float)(1.0 / sqrt(-expm1((double)t * log_b2)));
+    c.factor = factor;
+    c.decay = (float)(lr * wd);
+    c.base = adam_mix(seed ^ adam_mix((uint32_t)t ^ adam_mix(ordinal)));
+    c.pad[0] = c.pad[1] = c.pad[2] = 0;
+    return c;
+}
+
+// p, one rounding of the difference: the two small terms are added first
+SEMSEG_HD float adam_moved(float p, float m, float r, const AdamCoef& c, float eps) {
+    const float u = m / fmaf(r, c.root, eps);
+    return p - fmaf(c.size, u, c.decay * p);
+}
+
+// states in 32 bits
+SEMSEG_HD void adam_update32(float& p, float g, float& m, float& v, const AdamCoef& c, const AdamHyper& h) {
+    g *= c.factor;
+    m = fmaf(h.b1, m, h.c1 * g);
+    v = fmaf(h.b2, v, (h.c2 * g) * g);
+    p = adam_moved(p, m, sqrtf(v), c, h.eps);
+}
+
+// states in 8 bits, before they are coded again: m and r in 32 bits.  Every product and sum is rounded by itself (no contraction): the
+// codes depend on the last bit next to a border of the rounding, so the definition fixes it.
+SEMSEG_HD void adam_update8(float& p, float g, float& m, float& r, const AdamCoef& c, const AdamHyper& h) {
+#ifdef __clang__
+#pragma clang fp contract(off)
+#endif
+    g = g * c.factor;
+    const float m0 = h.b1 * m, m1 = h.c1 * g;
+    m = m0 + m1;
+    const float v0 = h.b2 * (r * r), v1 = (h.c2 * g) * g;
+    r = sqrtf(v0 + v1);
+    p = adam_moved(p, m, r, c, h.eps);
+}
+
+// scale of a block from the bit pattern of its largest |value| (patterns order as the values do, NaN above infinity)
+SEMSEG_HD float adam8_scale(uint32_t top) {
+    if (top >= 0x7f800000u) return adam_float(0x7fc00000u);      // a block that is not finite decodes to NaN
+    const float a = adam_float(top);
+    return a < ADAM8_TINY ? 0.0f : a * (1.0f / 448.0f);
+}
+SEMSEG_HD float adam8_inverse(float scale) { return scale > 0.0f ? 1.0f / scale : 0.0f; }      // NaN: 0, codes 0
+
+// |x| / scale, stochastically rounded to an e4m3 value (returned as a float that e4m3 holds exactly).  Below 2^-6 the spacing is
+// constant (2^-9): adding 2^-6 puts the value where a float's own spacing under 3 mantissa bits is 2^-9.
+SEMSEG_HD float adam8_round(float x, float inv, uint32_t random16, bool positive) {
+    float a = fabsf(x) * inv;
+    a = a < ADAM8_MAX ? a : ADAM8_MAX;                           // the largest one may come out a bit above
+    const float low = a < 0.015625f ? 0.015625f : 0.0f;
+    a = adam_float((adam_bits(a + low) + (random16 << 4)) & ~0xFFFFFu) - low;
+    if (positive && a < 0.001953125f && x > 0.0f && inv > 0.0f) a = 0.001953125f;
+    return inv > 0.0f ? a : 0.0f;
+}

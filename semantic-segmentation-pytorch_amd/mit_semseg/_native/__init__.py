@@ -14,6 +14,7 @@ LIB_PATH = os.environ.get('SEMSEG_NATIVE_LIB') or os.path.join(_HERE, 'libsemseg
 _lib = None
 
 c_int, c_f, c_sz, vp = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
+c_d, c_l = ctypes.c_double, ctypes.c_int64
 
 
 class SgdTensor(ctypes.Structure):
@@ -24,6 +25,20 @@ class SgdTensor(ctypes.Structure):
 class SgdTensor2(ctypes.Structure):
     _fields_ = [('param', vp), ('grad', vp), ('momentum_buf', vp), ('numel', ctypes.c_int64), ('weight_decay', c_f),
                 ('first_step', c_int), ('slabs', vp), ('splits', c_int), ('absmax_slots', vp)]
+
+
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [('param', vp), ('grad', vp), ('exp_avg', vp), ('exp_avg_sq', vp), ('copy', vp), ('step', vp),
+                ('numel', ctypes.c_int64), ('weight_decay', c_f), ('grad_type', c_int), ('copy_type', c_int)]
+
+
+class AdamW8Tensor(ctypes.Structure):
+    _fields_ = [('param', vp), ('grad', vp), ('copy', vp), ('m_codes', vp), ('m_scales', vp), ('r_codes', vp), ('r_scales', vp),
+                ('step', vp), ('numel', ctypes.c_int64), ('weight_decay', c_f), ('grad_type', c_int), ('copy_type', c_int)]
+
+
+class GradTensor(ctypes.Structure):
+    _fields_ = [('grad', vp), ('numel', ctypes.c_int64), ('grad_type', c_int)]
 
 
 class SlabTensor(ctypes.Structure):
@@ -164,6 +179,15 @@ SIGNATURES = {
     'semseg_input_label_gather': (c_int, [vp, c_int, vp, vp, c_int, c_int, vp, c_int, vp]),
     'semseg_sgd_step': (c_int, [ctypes.POINTER(SgdTensor), c_int, vp, c_f, c_f, vp]),
     'semseg_sgd_step_fused': (c_int, [ctypes.POINTER(SgdTensor2), c_int, vp, c_f, c_f, vp]),
+    'semseg_adamw_workspace_bytes': (c_sz, [c_int]),
+    'semseg_adamw_step': (c_int, [vp, c_int, vp, c_d, c_d, c_d, c_f, vp, vp, c_sz, vp]),
+    'semseg_adamw8_step': (c_int, [vp, c_int, vp, c_d, c_d, c_d, c_f, vp, ctypes.c_uint32, vp, c_sz, vp]),
+    'semseg_grad_norm_workspace_bytes': (c_sz, [vp, c_int]),
+    'semseg_grad_norm': (c_int, [vp, c_int, c_f, c_f, vp, vp, c_sz, vp]),
+    'semseg_label_logp_fwd': (c_int, [vp, c_int, c_l, vp, c_l, c_l, c_int, vp, vp, vp]),
+    'semseg_policy_loss_workspace_bytes': (c_sz, []),
+    'semseg_policy_loss_fwd': (c_int, [vp, c_int, c_l, vp, c_l, c_l, c_int, vp, c_l, vp, vp, c_f, c_f, c_f] + [vp] * 7 + [c_sz, vp]),
+    'semseg_label_logp_bwd': (c_int, [vp, c_int, c_l, vp, c_l, vp, vp, vp, vp, c_l, c_int, vp, vp]),
     'semseg_weights_absmax_slots': (vp, [vp, c_int, c_int, c_int]),
     'semseg_weights_prepare_h2_after_sgd': (c_int, [ctypes.POINTER(WPrepTensor), c_int, c_int, vp]),
     'semseg_comm_available': (c_int, []),

@@ -9,9 +9,12 @@ train.py:41) is converted once by the nchw_to_nhwc kernel.
 
 There is no CPU / eager fallback: non-CUDA tensors raise.
 """
+import collections
+import contextlib
 import ctypes
 import os
 
+import numpy as np
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
@@ -2300,6 +2303,186 @@ def nll_loss_acc(logp, label, ignore_index=-1):
 
 
 # ------------------------------------------------------------------------------------------------
+# log probability of chosen labels and the clipped policy loss (csrc/policy.hip): tuning a network on a reward
+# ------------------------------------------------------------------------------------------------
+_TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # SEMSEG_TYPE_*
+
+
+def _device_guard(device):
+    """launches go to the current device: make it the tensors' own"""
+    if device.type != 'cuda' or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _row_shape(what, z):
+    """shape of one number per row of logits [N, C, H, W] (rows = pixels) or [P, C]; refuses what is not such logits"""
+    _require_cuda(z)
+    if z.dtype not in _TYPE_CODES:
+        raise TypeError('%s: logits must be float32, bfloat16 or float16, got %s' % (what, z.dtype))
+    if z.dim() not in (2, 4):
+        raise ValueError('%s: logits must be [N, C, H, W] or [P, C], got %s' % (what, tuple(z.shape)))
+    if z.shape[1] < 1 or z.shape[1] > 1 << 30:
+        raise ValueError('%s: %d classes' % (what, z.shape[1]))
+    return (z.shape[0],) if z.dim() == 2 else (z.shape[0], z.shape[2], z.shape[3])
+
+
+def _logit_rows(z):
+    """(detached tensor, elements between rows, rows, classes) of logits that _row_shape has passed"""
+    _refuse_planes_only(z)
+    z = z.detach()
+    if z.dim() == 2:
+        rows, c = z.shape
+        ld = z.stride(0) if rows > 1 else c
+        if (c > 1 and z.stride(1) != 1) or ld < c:
+            z, ld = z.contiguous(), c
+        return z, ld, rows, c
+    n, c, h, w = z.shape
+    if z.numel() == 0:
+        return z, c, 0, c
+    ld = nhwc_ld(z)
+    if ld is None and z.dtype == torch.float32:
+        z, ld = as_nhwc(z)
+    elif ld is None:
+        out = empty_nhwc(n, c, h, w, z.device, z.dtype)
+        z, ld = out.copy_(z), c
+    return z, ld, n * h * w, c
+
+
+def _row_labels(what, z, rows, label):
+    _require_cuda(label)
+    if label.dtype.is_floating_point or label.dtype.is_complex or label.dtype == torch.bool:
+        raise TypeError('%s: labels must be integers, got %s' % (what, label.dtype))
+    if tuple(label.shape) != rows:
+        raise ValueError('%s: expected labels of shape %s, got %s' % (what, rows, tuple(label.shape)))
+    if label.device != z.device:
+        raise ValueError('%s: labels on %s, logits on %s' % (what, label.device, z.device))
+    return label.detach().to(torch.int64).contiguous()
+
+
+def _empty_like_rows(z, shape):
+    """the gradient of logits: dense rows, the logits' logical shape"""
+    if len(shape) == 2:
+        return torch.empty(shape, device=z.device, dtype=z.dtype)
+    return empty_nhwc(*shape, z.device, z.dtype)
+
+
+def _label_logp_bwd(z, ld, shape, label, ignore_index, stats, g, gloss, inv_count):
+    dz = _empty_like_rows(z, shape)
+    P = label.numel()
+    if P:
+        with _device_guard(z.device):
+            _native.check(_native.lib().semseg_label_logp_bwd(_p(z), _TYPE_CODES[z.dtype], ld, _p(label), ignore_index, _p(stats), _p(g),
+                                                              _p(gloss), _p(inv_count), P, shape[1], _p(dz), _st()), 'label_logp_bwd')
+    return dz
+
+
+class LabelLogProbFn(Function):
+    @staticmethod
+    def forward(ctx, z, label, ignore_index):
+        shape, rows = tuple(z.shape), _row_shape('label_log_prob', z)
+        label = _row_labels('label_log_prob', z, rows, label)
+        z, ld, P, c = _logit_rows(z)
+        lp = torch.empty(rows, device=z.device, dtype=torch.float32)
+        stats = torch.empty((P, 2), device=z.device, dtype=torch.float32) if ctx.needs_input_grad[0] else None
+        if P:
+            with _device_guard(z.device):
+                _native.check(_native.lib().semseg_label_logp_fwd(_p(z), _TYPE_CODES[z.dtype], ld, _p(label), ignore_index, P, c, _p(lp),
+                                                                  _p(stats), _st()), 'label_logp_fwd')
+        if stats is not None:
+            ctx.save_for_backward(z, label, stats)
+            ctx.cfg = (ld, shape, ignore_index)
+        return lp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        z, label, stats = ctx.saved_tensors
+        ld, shape, ignore_index = ctx.cfg
+        return _label_logp_bwd(z, ld, shape, label, ignore_index, stats, g.float().contiguous(), None, None), None, None
+
+
+def label_log_prob(z, label, ignore_index=-1):
+    """Log probability of the chosen label under softmax over the classes: z [N, C, H, W] (NHWC memory is read in place, with any
+    pixel stride) or [P, C], float32 / bfloat16 / float16; label [N, H, W] or [P], integers.  Returns float32 of the label's shape;
+    rows whose label is `ignore_index` or outside [0, C) give 0 and a zero gradient.  Log probabilities are logits too, so the
+    output of log_softmax can be handed in.  Differentiable in z."""
+    return LabelLogProbFn.apply(z, label, int(ignore_index))
+
+
+def _row_constants(what, name, t, shapes, device):
+    _require_cuda(t)
+    if t.requires_grad:
+        raise ValueError('%s: %s is a constant of the loss: detach it' % (what, name))
+    if not t.dtype.is_floating_point:
+        raise TypeError('%s: %s must be floating point, got %s' % (what, name, t.dtype))
+    if tuple(t.shape) not in shapes:
+        raise ValueError('%s: expected %s of shape %s, got %s' % (what, name, ' or '.join(map(str, shapes)), tuple(t.shape)))
+    if t.device != device:
+        raise ValueError('%s: %s on %s, logits on %s' % (what, name, t.device, device))
+    return t.float().contiguous()
+
+
+class PolicyLossFn(Function):
+    @staticmethod
+    def forward(ctx, z, label, advantage, old_logp, ref_logp, clip_low, clip_high, kl_weight, ignore_index):
+        what = 'policy_loss'
+        shape, dev, rows = tuple(z.shape), z.device, _row_shape(what, z)
+        label = _row_labels(what, z, rows, label)
+        advantage = _row_constants(what, 'advantage', advantage, ((rows[0],), rows) if z.dim() == 4 else (rows,), dev)
+        old_logp = _row_constants(what, 'old_logp', old_logp, (rows,), dev)
+        ref_logp = None if ref_logp is None else _row_constants(what, 'ref_logp', ref_logp, (rows,), dev)
+        z, ld, P, c = _logit_rows(z)
+        if P == 0:
+            loss, kl, clipped, inv = (torch.zeros((), device=dev) for _ in range(4))
+            stats = coef = torch.empty(0, device=dev)
+        else:
+            loss, kl, clipped, inv = (torch.empty((), device=dev) for _ in range(4))
+            stats, coef = torch.empty((P, 2), device=dev), torch.empty(P, device=dev)
+            L = _native.lib()
+            # scratch of its own: the caching allocator orders its reuse by stream and by captured graph
+            ws = torch.empty(L.semseg_policy_loss_workspace_bytes(), device=dev, dtype=torch.uint8)
+            with _device_guard(dev):
+                _native.check(L.semseg_policy_loss_fwd(_p(z), _TYPE_CODES[z.dtype], ld, _p(label), ignore_index, P, c, _p(advantage),
+                                                       P // advantage.numel(), _p(old_logp), _p(ref_logp), clip_low, clip_high, kl_weight,
+                                                       _p(stats), _p(coef), _p(loss), _p(kl), _p(clipped), _p(inv), _p(ws), ws.numel(),
+                                                       _st()), 'policy_loss_fwd')
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(z, label, stats, coef, inv)
+            ctx.cfg = (ld, shape, ignore_index)
+        ctx.mark_non_differentiable(kl, clipped)
+        return loss, kl, clipped
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gloss, gkl, gclipped):
+        z, label, stats, coef, inv = ctx.saved_tensors
+        ld, shape, ignore_index = ctx.cfg
+        dz = _label_logp_bwd(z, ld, shape, label, ignore_index, stats, coef, gloss.float().contiguous(), inv)
+        return (dz,) + (None,) * 8
+
+
+def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip_high=0.2, kl_weight=0.0, ignore_index=-1):
+    """Clipped policy loss with a KL term over per-row categoricals (logits z as in label_log_prob): with lp the log probability of
+    the chosen label under z and ratio = exp(lp - old_logp), the mean over the rows that count of
+
+        -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_weight (exp(ref_logp - lp) - (ref_logp - lp) - 1)
+
+    advantage: one number per image [N] or one per row (the label's shape); old_logp, ref_logp: the label's shape, constants
+    (label_log_prob under no_grad gives them).  Rows whose label is `ignore_index` or outside [0, C) do not count.
+    Returns three scalars: the loss (differentiable in z), the mean KL term (0 without ref_logp) and the share of rows whose clipped
+    term is the smaller one; all 0 where no row counts."""
+    clip_low, clip_high, kl_weight = float(clip_low), float(clip_high), float(kl_weight)
+    if not 0.0 <= clip_low <= 1.0 or not 0.0 <= clip_high < float('inf'):
+        raise ValueError('policy_loss: clip_low must lie in [0, 1] and clip_high must not be negative, got %r, %r' % (clip_low, clip_high))
+    if not 0.0 <= kl_weight < float('inf'):
+        raise ValueError('policy_loss: kl_weight must not be negative, got %r' % kl_weight)
+    if kl_weight > 0.0 and ref_logp is None:
+        raise ValueError('policy_loss: a KL term needs ref_logp')
+    return PolicyLossFn.apply(z, label, advantage, old_logp, ref_logp, clip_low, clip_high, kl_weight, int(ignore_index))
+
+
+# ------------------------------------------------------------------------------------------------
 # optimiser
 # ------------------------------------------------------------------------------------------------
 def sgd_step(params, grads, bufs, first_step, weight_decays, lr_tensor, momentum=0.9, grad_scale=1.0):
@@ -2360,3 +2543,209 @@ def finish_leftover_slabs():
     for i, (slabs, out, numel, splits, _) in enumerate(items):
         arr[i].slabs, arr[i].out, arr[i].numel, arr[i].splits = slabs.data_ptr(), out.data_ptr(), numel, splits
     _native.check(_native.lib().semseg_reduce_slabs_multi(arr, len(items), _st()), 'reduce_slabs_multi')
+
+
+# ---- AdamW (csrc/adamw.hip) ------------------------------------------------------------------------------------------------------
+_ADAMW = np.dtype(_native.AdamWTensor)
+_ADAMW8 = np.dtype(_native.AdamW8Tensor)
+_GRADS = np.dtype(_native.GradTensor)
+ADAMW8_BLOCK = 256          # elements that share one scale of the 8-bit states
+
+# 8-bit states of one parameter, in the order of its memory: e4m3 codes of the first moment and of the square root of the second, one
+# float32 scale per ADAMW8_BLOCK elements
+AdamW8State = collections.namedtuple('AdamW8State', 'm m_scale r r_scale')
+
+
+def _is_dense(t):
+    """every element of the tensor's span of memory belongs to it, once"""
+    if t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)):
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _same_order(a, b):
+    """two tensors whose elements follow each other in memory in the same order (strides of axes of one element say nothing)"""
+    if a.stride() == b.stride():
+        return a.numel() == b.numel()
+    return a.shape == b.shape and all(x == y or n == 1 for x, y, n in zip(a.stride(), b.stride(), a.shape))
+
+
+def _optimiser_lists(what, params, grads, steps, weight_decays, lr_tensor, betas, eps, clip, copies, states):
+    """the checks of arguments that the AdamW steps share; returns (device, live indices)"""
+    n = len(params)
+    if not (len(grads) == len(steps) == len(weight_decays) == n and all(len(s) == n for s in states) and
+            (copies is None or len(copies) == n)):
+        raise ValueError('%s: the lists differ in length' % what)
+    b1, b2 = betas
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0) or not 0.0 <= eps < float('inf'):
+        raise ValueError('%s: betas must lie in [0, 1) and eps must not be negative, got %r, %r' % (what, betas, eps))
+    if n == 0:
+        return None, []
+    dev = params[0].device
+    _require_cuda(params[0])
+    index = params[0].get_device()
+    for p, g, s in zip(params, grads, steps):
+        if p.dtype is not torch.float32:
+            raise TypeError('%s: parameters must be float32 (a 16-bit copy goes into `copies`), got %s' % (what, p.dtype))
+        if g.dtype not in _TYPE_CODES:
+            raise TypeError('%s: gradients must be float32, bfloat16 or float16, got %s' % (what, g.dtype))
+        if s.dtype is not torch.int32 or s.numel() != 1:
+            raise TypeError('%s: a step count is one int32 on the device, got %s %s' % (what, s.dtype, tuple(s.shape)))
+        if p.get_device() != index or g.get_device() != index or s.get_device() != index:
+            raise ValueError('%s: all tensors of a call must be on one HIP device' % what)
+        if not _same_order(p, g) or not _is_dense(p):
+            raise RuntimeError('%s: a %s parameter and its gradient differ in layout or are not dense (strides %s, %s)'
+                               % (what, tuple(p.shape), p.stride(), g.stride()))
+    for more, c in zip(params, copies or ()):
+        if c is not None and (c.dtype not in (torch.bfloat16, torch.float16) or c.get_device() != index or not _same_order(more, c)):
+            raise RuntimeError('%s: a copy must be bfloat16 or float16 in its parameter\'s layout on its device' % what)
+    for name, t, count in (('lr_tensor', lr_tensor, 1), ('clip', clip, 2)):
+        if t is not None and (t.dtype is not torch.float32 or t.numel() != count or not t.is_contiguous() or t.get_device() != index):
+            raise ValueError('%s: %s must hold %d float32 on the parameters\' device' % (what, name, count))
+    live = [i for i in range(n) if params[i].numel()]
+    if len({params[i].data_ptr() for i in live}) != len(live) or len({steps[i].data_ptr() for i in live}) != len(live):
+        raise ValueError('%s: the same parameter or step count twice in one call' % what)
+    return dev, live
+
+
+def _fill_common(rec, params, grads, steps, weight_decays, copies, live):
+    rec['param'] = [params[i].data_ptr() for i in live]
+    rec['grad'] = [grads[i].data_ptr() for i in live]
+    rec['step'] = [steps[i].data_ptr() for i in live]
+    rec['numel'] = [params[i].numel() for i in live]
+    rec['weight_decay'] = [weight_decays[i] for i in live]
+    rec['grad_type'] = [_TYPE_CODES[grads[i].dtype] for i in live]
+    if copies is not None:
+        rec['copy'] = [0 if copies[i] is None else copies[i].data_ptr() for i in live]
+        rec['copy_type'] = [0 if copies[i] is None else _TYPE_CODES[copies[i].dtype] for i in live]
+
+
+def _weights_changed(params):
+    """prepared weight planes are stale until prepare_conv_weights runs again (the kernels write behind torch's version counters)"""
+    if not _WPLANES:
+        return
+    for p in params:
+        rec = _WPLANES.get(id(p))
+        if rec is not None:
+            _WPLANES[id(p)] = (rec[0], -1, rec[2], rec[3], rec[4], rec[5], rec[6])
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, weight_decays, lr_tensor, betas=(0.9, 0.999), eps=1e-8, grad_scale=1.0,
+               clip=None, copies=None):
+    """One AdamW step over many tensors, states in 32 bits.  All lists are parallel.  params, exp_avgs, exp_avg_sqs: float32 in one
+    layout; grads: the same layout, float32 / bfloat16 / float16; steps: one int32 device scalar per tensor (views of one tensor
+    will do), advanced by the call; lr_tensor: one float32 on the device; grad_scale multiplies the gradients; clip: what grad_norm
+    returned -- its factor multiplies them too, and where its norm is not finite the call changes nothing; copies: optional list of
+    bfloat16 / float16 tensors (or None) that receive the updated parameters.  Everything the step reads that changes from step to
+    step is device memory, so a captured call can be replayed."""
+    dev, live = _optimiser_lists('adamw_step', params, grads, steps, weight_decays, lr_tensor, betas, eps, clip, copies,
+                                 (exp_avgs, exp_avg_sqs))
+    if not live:
+        return
+    index = params[0].get_device()
+    for p, m, v in zip(params, exp_avgs, exp_avg_sqs):
+        if m.dtype is not torch.float32 or v.dtype is not torch.float32 or m.get_device() != index or v.get_device() != index or \
+                not _same_order(p, m) or not _same_order(p, v):
+            raise RuntimeError('adamw_step: the states of a %s parameter must be float32 in its layout on its device' % (tuple(p.shape),))
+    rec = np.zeros(len(live), dtype=_ADAMW)
+    _fill_common(rec, params, grads, steps, weight_decays, copies, live)
+    rec['exp_avg'] = [exp_avgs[i].data_ptr() for i in live]
+    rec['exp_avg_sq'] = [exp_avg_sqs[i].data_ptr() for i in live]
+    L = _native.lib()
+    with _device_guard(dev):
+        ws = torch.empty(L.semseg_adamw_workspace_bytes(len(live)), device=dev, dtype=torch.uint8)
+        _native.check(L.semseg_adamw_step(vp(rec.ctypes.data), len(live), _p(lr_tensor), betas[0], betas[1], eps, float(grad_scale),
+                                          _p(clip), _p(ws), ws.numel(), _st()), 'adamw_step')
+    _weights_changed(params)
+
+
+def adamw8_state(param):
+    """fresh 8-bit AdamW states of a parameter: an AdamW8State of zeros"""
+    n = param.numel()
+    blocks = -(-n // ADAMW8_BLOCK)
+
+    def codes():
+        return torch.zeros(n, device=param.device, dtype=torch.uint8).view(torch.float8_e4m3fn)
+
+    def scales():
+        return torch.zeros(blocks, device=param.device, dtype=torch.float32)
+
+    return AdamW8State(codes(), scales(), codes(), scales())
+
+
+def adamw8_values(state, param):
+    """(exp_avg, exp_avg_sq) that an AdamW8State stands for, float32 in the parameter's layout"""
+    m, ms, r, rs = state
+    out = []
+    for codes, scale in ((m, ms), (r, rs)):
+        x = codes.view(torch.float8_e4m3fn).float() * scale.repeat_interleave(ADAMW8_BLOCK)[:codes.numel()]
+        out.append(x.as_strided(param.shape, param.stride()))
+    return out[0], out[1].square()
+
+
+def adamw8_step(params, grads, states, steps, weight_decays, lr_tensor, betas=(0.9, 0.999), eps=1e-8, grad_scale=1.0, clip=None,
+                copies=None, seed=0):
+    """adamw_step with states in 8 bits: `states` holds one AdamW8State (adamw8_state) per parameter, blocks of ADAMW8_BLOCK
+    elements share a scale.  The update itself is computed in 32 bits from the decoded states; they are coded again with stochastic
+    rounding whose random bits come from (seed, step count, index in the list, element): the same call gives the same states."""
+    what = 'adamw8_step'
+    dev, live = _optimiser_lists(what, params, grads, steps, weight_decays, lr_tensor, betas, eps, clip, copies, (states,))
+    if not live:
+        return
+    index = params[0].get_device()
+    for p, (m, ms, r, rs) in zip(params, states):
+        n = p.numel()
+        blocks = -(-n // ADAMW8_BLOCK)
+        for codes, scale in ((m, ms), (r, rs)):
+            if codes.dtype not in (torch.uint8, torch.float8_e4m3fn) or scale.dtype is not torch.float32 or codes.numel() != n or \
+                    scale.numel() != blocks or not codes.is_contiguous() or not scale.is_contiguous() or \
+                    codes.get_device() != index or scale.get_device() != index:
+                raise RuntimeError('%s: the state of a %s parameter must be %d codes and %d float32 scales on its device (adamw8_state)'
+                                   % (what, tuple(p.shape), n, blocks))
+    rec = np.zeros(len(live), dtype=_ADAMW8)
+    _fill_common(rec, params, grads, steps, weight_decays, copies, live)
+    for k, name in enumerate(('m_codes', 'm_scales', 'r_codes', 'r_scales')):
+        rec[name] = [states[i][k].data_ptr() for i in live]
+    L = _native.lib()
+    with _device_guard(dev):
+        ws = torch.empty(L.semseg_adamw_workspace_bytes(len(live)), device=dev, dtype=torch.uint8)
+        _native.check(L.semseg_adamw8_step(vp(rec.ctypes.data), len(live), _p(lr_tensor), betas[0], betas[1], eps, float(grad_scale),
+                                           _p(clip), int(seed) & 0xFFFFFFFF, _p(ws), ws.numel(), _st()), what)
+    _weights_changed(params)
+
+
+def grad_norm(grads, max_norm=None, grad_scale=1.0):
+    """Global 2-norm of gradients (float32 / bfloat16 / float16, any mix, dense): float32 [2] on the device -- the norm of
+    grad * grad_scale and the factor min(1, max_norm / (norm + 1e-6)) that brings it to max_norm (1 without max_norm, 0 where the norm
+    is not finite).  Nothing is scaled: adamw_step / adamw8_step take the result as `clip`.  Sums run in 64 bits in a fixed order."""
+    if max_norm is not None and not 0.0 <= max_norm:
+        raise ValueError('grad_norm: max_norm must not be negative, got %r' % max_norm)
+    if not grads:
+        raise ValueError('grad_norm: no gradients')
+    _require_cuda(grads[0])
+    dev = grads[0].device
+    for g in grads:
+        if g.dtype not in _TYPE_CODES:
+            raise TypeError('grad_norm: gradients must be float32, bfloat16 or float16, got %s' % g.dtype)
+        if g.get_device() != grads[0].get_device():
+            raise ValueError('grad_norm: all gradients must be on one HIP device')
+        if not _is_dense(g):
+            raise RuntimeError('grad_norm: a %s gradient is not dense (strides %s)' % (tuple(g.shape), g.stride()))
+    live = [g for g in grads if g.numel()]
+    rec = np.zeros(len(live), dtype=_GRADS)
+    rec['grad'] = [g.data_ptr() for g in live]
+    rec['numel'] = [g.numel() for g in live]
+    rec['grad_type'] = [_TYPE_CODES[g.dtype] for g in live]
+    L = _native.lib()
+    table = vp(rec.ctypes.data)
+    with _device_guard(dev):
+        out = torch.empty(2, device=dev, dtype=torch.float32)
+        ws = torch.empty(L.semseg_grad_norm_workspace_bytes(table, len(live)), device=dev, dtype=torch.uint8)
+        _native.check(L.semseg_grad_norm(table, len(live), float(grad_scale), -1.0 if max_norm is None else float(max_norm), _p(out),
+                                         _p(ws), ws.numel(), _st()), 'grad_norm')
+    return out
