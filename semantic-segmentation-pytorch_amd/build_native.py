@@ -11,6 +11,8 @@ CSRC = os.path.join(HERE, 'csrc')
 OUT_DIR = os.path.join(HERE, 'mit_semseg', '_native')
 LIB = os.path.join(OUT_DIR, 'libsemseg_hip.so')
 SOURCES = ['conv_igemm.hip', 'conv_wgrad.hip', 'conv_split.hip', 'weights_prep.hip', 'winograd.hip', 'bn.hip', 'pool_resize.hip', 'head.hip', 'adamw.hip', 'policy.hip', 'input_pipeline.hip', 'depthwise.hip', 'grouped.hip', 'comm.hip', 'peer.hip', 'probe.hip', 'batch.hip', 'api.hip']
+HOST_SRC = os.path.join(CSRC, 'host_table.cpp')      # CPython extension (host code only): tensor lists -> descriptor tables
+HOST_LIB = os.path.join(OUT_DIR, '_host.so')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-I' + os.path.join(ROOT, 'include'), '-I' + CSRC,
          '-Wno-unused-result',
@@ -21,6 +23,17 @@ FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-I' + os.path.j
 
 def _newer(a, b):
     return (not os.path.exists(b)) or os.path.getmtime(a) > os.path.getmtime(b)
+
+
+def _host_command(out, depfile):
+    import sysconfig
+    import torch
+    base = os.path.join(os.path.dirname(torch.__file__), 'include')
+    return ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-D_GLIBCXX_USE_CXX11_ABI=%d' % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+            '-I' + os.path.join(ROOT, 'include'), '-isystem', base, '-isystem', os.path.join(base, 'torch', 'csrc', 'api', 'include'),
+            '-isystem', sysconfig.get_paths()['include'], '-MMD', '-MF', depfile, HOST_SRC, '-o', out,
+            # torch is imported first and has these loaded; named here so that the loader takes their symbols
+            '-L' + os.path.join(os.path.dirname(torch.__file__), 'lib'), '-ltorch_python', '-ltorch_cpu', '-lc10']
 
 
 def _depfile_deps(depfile):
@@ -81,6 +94,9 @@ def _build_locked(force, verbose):
         if force or _stale(src, obj):
             # -MMD: the compiler lists every user header it read (csrc/*.h, include/semseg_hip.h) in obj.d; no hand-kept list
             jobs.append((obj, [HIPCC] + FLAGS + ['-MMD', '-MF', obj + '.d' + tag, '-c', src, '-o', obj + tag]))
+    objects = len(jobs)
+    if force or _stale(HOST_SRC, HOST_LIB):
+        jobs.append((HOST_LIB, _host_command(HOST_LIB + tag, HOST_LIB + '.d' + tag)))
     if jobs:
         def run(job):
             obj, cmd = job
@@ -89,7 +105,7 @@ def _build_locked(force, verbose):
             os.replace(obj + tag, obj)
         with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as ex:
             list(ex.map(run, jobs))
-    if jobs or not os.path.exists(LIB):
+    if objects or not os.path.exists(LIB):
         _run([HIPCC, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', LIB + tag] + objs + ['-ldl'], verbose)
         os.replace(LIB + tag, LIB)
     return LIB

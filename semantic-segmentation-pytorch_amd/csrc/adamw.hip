@@ -162,15 +162,59 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamBatch b, const Ada
         }
         return;
     }
-    // the last chunk of a tensor, and tensors that start at an odd address
-    const int64_t end = min(t.numel, start + ADAM_CHUNK);
-    for (int64_t i = start + tid; i < end; i += 256) {
-        float p = t.p[i], m = t.m[i], v = t.v[i];
-        adam_update32(p, load_one(t.g, t.gtype, i), m, v, c, h);
-        t.m[i] = m;
-        t.v[i] = v;
-        t.p[i] = p;
-        if (t.c) store_one(t.c, t.ctype, i, p);
+    // the last chunk of a tensor, and tensors that start at an odd address: loads that would pass the end read the last place again, so
+    // that all of a thread's loads still leave together, and are not stored (one load at a time took 38 us for the 115 small tensors of a
+    // ResNet50)
+    const int left = (int)min(t.numel - start, (int64_t)ADAM_CHUNK);
+    const int quads = t.vec ? left >> 2 : 0;
+    if (quads) {
+        f32x4* p4 = reinterpret_cast<f32x4*>(t.p) + (start >> 2);
+        f32x4* m4 = reinterpret_cast<f32x4*>(t.m) + (start >> 2);
+        f32x4* v4 = reinterpret_cast<f32x4*>(t.v) + (start >> 2);
+        f32x4 p[ADAM_QUADS], g[ADAM_QUADS], m[ADAM_QUADS], v[ADAM_QUADS];
+#pragma unroll
+        for (int u = 0; u < ADAM_QUADS; ++u) {
+            const int q = min(tid + u * 256, quads - 1);
+            g[u] = load_quad(t.g, t.gtype, (start >> 2) + q);
+            m[u] = m4[q];
+            v[u] = v4[q];
+            p[u] = p4[q];
+        }
+#pragma unroll
+        for (int u = 0; u < ADAM_QUADS; ++u) {
+            const int q = tid + u * 256;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float pj = p[u][j], mj = m[u][j], vj = v[u][j];
+                adam_update32(pj, g[u][j], mj, vj, c, h);
+                p[u][j] = pj; m[u][j] = mj; v[u][j] = vj;
+            }
+            if (q < quads) {
+                m4[q] = m[u];
+                v4[q] = v[u];
+                p4[q] = p[u];
+                if (t.c) store_quad(t.c, t.ctype, (start >> 2) + q, p[u]);
+            }
+        }
+    }
+    for (int base = quads * 4; base < left; base += 4 * 256) {
+        float p[4], g[4], m[4], v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t i = start + min(base + tid + u * 256, left - 1);
+            p[u] = t.p[i]; m[u] = t.m[i]; v[u] = t.v[i]; g[u] = load_one(t.g, t.gtype, i);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t i = start + base + tid + u * 256;
+            adam_update32(p[u], g[u], m[u], v[u], c, h);
+            if (base + tid + u * 256 < left) {
+                t.m[i] = m[u];
+                t.v[i] = v[u];
+                t.p[i] = p[u];
+                if (t.c) store_one(t.c, t.ctype, i, p[u]);
+            }
+        }
     }
 }
 
@@ -237,36 +281,49 @@ struct Adam8Batch {
 };
 static_assert(sizeof(Adam8Batch) <= 4000, "kernel arguments");
 
+// maximum over the wave, as a scalar.  Within a row of 16 lanes by lane permutations of the instruction itself, then across the rows:
+// 6 instructions and a read of lane 63 (shuffles through LDS take 18 and their waits).  All lanes must be active.
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-    return v;
+#define SEMSEG_DPP_MAX(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, ctrl, rows, 0xf, false))
+    SEMSEG_DPP_MAX(0xB1, 0xf);        // neighbours
+    SEMSEG_DPP_MAX(0x4E, 0xf);        // pairs
+    SEMSEG_DPP_MAX(0x141, 0xf);       // mirrored halves of a row
+    SEMSEG_DPP_MAX(0x140, 0xf);       // mirrored rows
+    SEMSEG_DPP_MAX(0x142, 0xa);       // lane 15 of a row to the next: rows 1 and 3
+    SEMSEG_DPP_MAX(0x143, 0xc);       // lane 31 to rows 2 and 3
+#undef SEMSEG_DPP_MAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-// one e4m3 code of a value that e4m3 holds exactly
-__device__ __forceinline__ uint8_t code_of(float a) { return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(a, 0.f, 0, false) & 0xff); }
-__device__ __forceinline__ float value_of(uint8_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
-__device__ __forceinline__ uint32_t codes_of(const float a[4]) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a[0], a[1], 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a[2], a[3], w, true);
-}
+// the e4m3 code of byte J in a word of four
+template <int J>
+__device__ __forceinline__ float value_of(uint32_t w) { return __builtin_amdgcn_cvt_f32_fp8((int)w, J); }
 
-// m and r of one block after the update (4 elements a lane, elements that do not exist are 0) -> scales and rounded values
-__device__ __forceinline__ void adam8_block(float m[4], float r[4], const uint32_t at[4], const AdamCoef& c, float& ms, float& rs) {
+// m and r of one block after the update (4 elements a lane, elements that do not exist are 0) -> scales and words of codes
+__device__ __forceinline__ void adam8_block(const float m[4], const float r[4], const uint32_t at[4], const AdamCoef& c, float& ms, float& rs,
+                                            uint32_t& mc, uint32_t& rc) {
     uint32_t tm = 0, tr = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        tm = max(tm, adam_bits(fabsf(m[j])));
-        tr = max(tr, adam_bits(fabsf(r[j])));
+        tm = max(tm, adam_bits(m[j]) & 0x7fffffffu);
+        tr = max(tr, adam_bits(r[j]) & 0x7fffffffu);
     }
     ms = adam8_scale(wave_max_u32(tm));
     rs = adam8_scale(wave_max_u32(tr));
     const float im = adam8_inverse(ms), ir = adam8_inverse(rs);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t bits = adam_mix(at[j] + c.base);
-        m[j] = copysignf(adam8_round(m[j], im, bits & 0xffffu, false), m[j]);
-        r[j] = adam8_round(r[j], ir, bits >> 16, true);
+    int wm = 0, wr = 0;
+#define SEMSEG_ADAM8_CODE(j)                                                                                     \
+    {                                                                                                            \
+        const uint32_t bits = adam_mix(at[j] + c.base);                                                          \
+        wm = __builtin_amdgcn_cvt_sr_fp8_f32(adam8_scaled_m(m[j], im), bits << 16, wm, j);                       \
+        wr = __builtin_amdgcn_cvt_sr_fp8_f32(adam8_scaled_r(r[j], ir), bits & 0xffff0000u, wr, j);               \
     }
+    SEMSEG_ADAM8_CODE(0)
+    SEMSEG_ADAM8_CODE(1)
+    SEMSEG_ADAM8_CODE(2)
+    SEMSEG_ADAM8_CODE(3)
+#undef SEMSEG_ADAM8_CODE
+    mc = (uint32_t)wm;
+    rc = (uint32_t)wr;
 }
 
 __global__ __launch_bounds__(256) void adamw8_kernel(const Adam8Batch b, const AdamCoef* __restrict__ coef, AdamHyper h) {
@@ -276,8 +333,10 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Adam8Batch b, const A
     if (c.root == 0.f) return;
     const int lane = threadIdx.x & 63;
     const int64_t start = (int64_t)(blockIdx.x - b.first[k]) * ADAM8_CHUNK + (threadIdx.x >> 6) * (ADAM8_PER_WAVE * ADAM8_BLOCK);
-    if (t.vec && start + ADAM8_PER_WAVE * ADAM8_BLOCK <= t.numel) {
-        const int64_t q0 = (start >> 2) + lane;
+    if (start >= t.numel) return;                            // the same for the whole wave, as everything about blocks here
+    const int full = t.vec ? (int)min((t.numel - start) >> 8, (int64_t)ADAM8_PER_WAVE) : 0;
+    if (full) {
+        const int64_t q0 = (start >> 2) + lane, s0 = start >> 8;
         f32x4* p4 = reinterpret_cast<f32x4*>(t.p);
         uint32_t* m4 = reinterpret_cast<uint32_t*>(t.m);
         uint32_t* r4 = reinterpret_cast<uint32_t*>(t.r);
@@ -286,21 +345,21 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Adam8Batch b, const A
         float ms[ADAM8_PER_WAVE], rs[ADAM8_PER_WAVE];
 #pragma unroll
         for (int u = 0; u < ADAM8_PER_WAVE; ++u) {
-            g[u] = load_quad(t.g, t.gtype, q0 + u * 64);
-            p[u] = p4[q0 + u * 64];
-            mc[u] = m4[q0 + u * 64];
-            rc[u] = r4[q0 + u * 64];
-            ms[u] = t.ms[(start >> 8) + u];
-            rs[u] = t.rs[(start >> 8) + u];
+            const int b = min(u, full - 1);                  // a block behind the last whole one is the last one again, not stored
+            g[u] = load_quad(t.g, t.gtype, q0 + b * 64);
+            p[u] = p4[q0 + b * 64];
+            mc[u] = m4[q0 + b * 64];
+            rc[u] = r4[q0 + b * 64];
+            ms[u] = t.ms[s0 + b];
+            rs[u] = t.rs[s0 + b];
         }
 #pragma unroll
         for (int u = 0; u < ADAM8_PER_WAVE; ++u) {
+            if (u >= full) break;
             float m[4], r[4];
             uint32_t at[4];
-            m[0] = __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 0); m[1] = __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 1);
-            m[2] = __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 2); m[3] = __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 3);
-            r[0] = __builtin_amdgcn_cvt_f32_fp8((int)rc[u], 0); r[1] = __builtin_amdgcn_cvt_f32_fp8((int)rc[u], 1);
-            r[2] = __builtin_amdgcn_cvt_f32_fp8((int)rc[u], 2); r[3] = __builtin_amdgcn_cvt_f32_fp8((int)rc[u], 3);
+            m[0] = value_of<0>(mc[u]); m[1] = value_of<1>(mc[u]); m[2] = value_of<2>(mc[u]); m[3] = value_of<3>(mc[u]);
+            r[0] = value_of<0>(rc[u]); r[1] = value_of<1>(rc[u]); r[2] = value_of<2>(rc[u]); r[3] = value_of<3>(rc[u]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 at[j] = (uint32_t)((q0 + u * 64) * 4 + j);
@@ -311,20 +370,20 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Adam8Batch b, const A
                 p[u][j] = pj;
             }
             float msn, rsn;
-            adam8_block(m, r, at, c, msn, rsn);
+            uint32_t mn, rn;
+            adam8_block(m, r, at, c, msn, rsn, mn, rn);
             p4[q0 + u * 64] = p[u];
-            m4[q0 + u * 64] = codes_of(m);
-            r4[q0 + u * 64] = codes_of(r);
+            m4[q0 + u * 64] = mn;
+            r4[q0 + u * 64] = rn;
             if (lane == 0) {
-                t.ms[(start >> 8) + u] = msn;
-                t.rs[(start >> 8) + u] = rsn;
+                t.ms[s0 + u] = msn;
+                t.rs[s0 + u] = rsn;
             }
             if (t.c) store_quad(t.c, t.ctype, q0 + u * 64, p[u]);
         }
-        return;
     }
-    // the last blocks of a tensor, and tensors that start at an odd address: element lane + 64 j of the block
-    for (int u = 0; u < ADAM8_PER_WAVE; ++u) {
+    // the last block of a tensor, and tensors that start at an odd address: element lane + 64 j of the block
+    for (int u = full; u < ADAM8_PER_WAVE; ++u) {
         const int64_t s = start + u * ADAM8_BLOCK;
         if (s >= t.numel) return;                            // the same for the whole wave
         const float ms = t.ms[s >> 8], rs = t.rs[s >> 8];
@@ -337,20 +396,21 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Adam8Batch b, const A
             m[j] = r[j] = p[j] = 0.f;
             if (i < t.numel) {
                 p[j] = t.p[i];
-                m[j] = value_of(t.m[i]) * ms;
-                r[j] = value_of(t.r[i]) * rs;
+                m[j] = value_of<0>(t.m[i]) * ms;
+                r[j] = value_of<0>(t.r[i]) * rs;
                 adam_update8(p[j], load_one(t.g, t.gtype, i), m[j], r[j], c, h);
             }
         }
         float msn, rsn;
-        adam8_block(m, r, at, c, msn, rsn);
+        uint32_t mn, rn;
+        adam8_block(m, r, at, c, msn, rsn, mn, rn);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int64_t i = s + lane + 64 * j;
             if (i < t.numel) {
                 t.p[i] = p[j];
-                t.m[i] = code_of(m[j]);
-                t.r[i] = code_of(r[j]);
+                t.m[i] = (uint8_t)(mn >> (8 * j));
+                t.r[i] = (uint8_t)(rn >> (8 * j));
                 if (t.c) store_one(t.c, t.ctype, i, p[j]);
             }
         }
@@ -423,6 +483,23 @@ static_assert(sizeof(NormBatch) <= 4000, "kernel arguments");
 
 __device__ __forceinline__ void add_square(double& s, float x) { const double d = (double)x; s = fma(d, d, s); }
 
+__device__ __forceinline__ void add_squares(double& s, u32x4 v, int type) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (type == SEMSEG_TYPE_F32) {
+            add_square(s, adam_float(v[j]));
+        } else if (type == SEMSEG_TYPE_BF16) {
+            add_square(s, adam_float(v[j] << 16));
+            add_square(s, adam_float(v[j] & 0xffff0000u));
+        } else {
+            typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+            const f16x2 x = __builtin_bit_cast(f16x2, v[j]);
+            add_square(s, (float)x[0]);
+            add_square(s, (float)x[1]);
+        }
+    }
+}
+
 __global__ __launch_bounds__(256) void grad_norm_kernel(const NormBatch b, double* __restrict__ partial) {
     __shared__ double sum[4];
     const int k = tensor_of(b, blockIdx.x);
@@ -430,17 +507,24 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const NormBatch b, doubl
     const int64_t start = (int64_t)(blockIdx.x - b.first[k]) * NORM_CHUNK;
     const int64_t end = min(t.numel, start + NORM_CHUNK);
     double s = 0.0;
-    if (t.vec && start + NORM_CHUNK <= t.numel) {
-        const int64_t q0 = (start >> 2) + threadIdx.x;
-        for (int u = 0; u < NORM_CHUNK / 1024; u += 8) {
-            f32x4 g[8];
+    if (t.vec) {
+        // 16-byte loads, 8 of a thread in flight (f32: 4 elements each, 16 bits: 8); past the end the last place again, not added
+        const int per = t.type == SEMSEG_TYPE_F32 ? 4 : 8;
+        const int vecs = (int)(end - start) / per;
+        const u32x4* g4 = reinterpret_cast<const u32x4*>(t.g) + start / per;
+        for (int base = 0; base < vecs; base += 8 * 256) {
+            u32x4 g[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = load_quad(t.g, t.type, q0 + (u + j) * 256);
+            for (int j = 0; j < 8; ++j) g[j] = g4[min(base + j * 256 + (int)threadIdx.x, vecs - 1)];
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                add_square(s, g[j][0]); add_square(s, g[j][1]); add_square(s, g[j][2]); add_square(s, g[j][3]);
+                if (base + j * 256 + (int)threadIdx.x >= vecs) g[j] = u32x4{0u, 0u, 0u, 0u};
+                add_squares(s, g[j], t.type);
             }
         }
+        const int64_t i = start + (int64_t)vecs * per + threadIdx.x;
+        if (i < end) add_square(s, load_one(t.g, t.type, i));           // fewer than 8 are left
     } else {
         for (int64_t i = start + threadIdx.x; i < end; i += 256) add_square(s, load_one(t.g, t.type, i));
     }
@@ -501,7 +585,7 @@ extern "C" int semseg_grad_norm(const semseg_grad_tensor* tensors_host, int n, f
             e.g = t.grad;
             e.numel = t.numel;
             e.type = (uint8_t)t.grad_type;
-            e.vec = aligned_to(t.grad, 4 * type_bytes(t.grad_type));
+            e.vec = aligned16(t.grad);
             for (int j = 0; j < 6; ++j) e.pad[j] = 0;
             b.first[b.n++] = chunks;
             chunks += (uint32_t)c;

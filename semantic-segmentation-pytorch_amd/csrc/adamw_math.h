@@ -77,18 +77,24 @@ SEMSEG_HD void adam_update32(float& p, float g, float& m, float& v, const AdamCo
     p = adam_moved(p, m, sqrtf(v), c, h.eps);
 }
 
-// states in 8 bits, before they are coded again: m and r in 32 bits.  Every product and sum is rounded by itself (no contraction): the
-// codes depend on the last bit next to a border of the rounding, so the definition fixes it.
-SEMSEG_HD void adam_update8(float& p, float g, float& m, float& r, const AdamCoef& c, const AdamHyper& h) {
-#ifdef __clang__
-#pragma clang fp contract(off)
+// Root and reciprocal of the 8-bit step: the hardware's, off by at most one unit of the last place (the correctly rounded ones take
+// about 12 instructions each, and the 8-bit step has so few bytes an element that instructions bound it).  The root takes denormals as
+// zero: a second moment below 1e-38, a gradient below 1e-17.
+#if defined(__HIP_DEVICE_COMPILE__)
+SEMSEG_HD float adam_root(float x) { return __builtin_amdgcn_sqrtf(x); }
+SEMSEG_HD float adam_reciprocal(float x) { return __builtin_amdgcn_rcpf(x); }
+#else
+SEMSEG_HD float adam_root(float x) { return sqrtf(x); }
+SEMSEG_HD float adam_reciprocal(float x) { return 1.0f / x; }
 #endif
-    g = g * c.factor;
-    const float m0 = h.b1 * m, m1 = h.c1 * g;
-    m = m0 + m1;
-    const float v0 = h.b2 * (r * r), v1 = (h.c2 * g) * g;
-    r = sqrtf(v0 + v1);
-    p = adam_moved(p, m, r, c, h.eps);
+
+// states in 8 bits, before they are coded again: m and r in 32 bits
+SEMSEG_HD void adam_update8(float& p, float g, float& m, float& r, const AdamCoef& c, const AdamHyper& h) {
+    g *= c.factor;
+    m = fmaf(h.b1, m, h.c1 * g);
+    r = adam_root(fmaf(h.b2, r * r, (h.c2 * g) * g));
+    const float u = m * adam_reciprocal(fmaf(r, c.root, h.eps));
+    p = p - fmaf(c.size, u, c.decay * p);
 }
 
 // scale of a block from the bit pattern of its largest |value| (patterns order as the values do, NaN above infinity)
@@ -97,15 +103,19 @@ SEMSEG_HD float adam8_scale(uint32_t top) {
     const float a = adam_float(top);
     return a < ADAM8_TINY ? 0.0f : a * (1.0f / 448.0f);
 }
-SEMSEG_HD float adam8_inverse(float scale) { return scale > 0.0f ? 1.0f / scale : 0.0f; }      // NaN: 0, codes 0
+SEMSEG_HD float adam8_inverse(float scale) { return scale > 0.0f ? adam_reciprocal(scale) : 0.0f; }
 
-// |x| / scale, stochastically rounded to an e4m3 value (returned as a float that e4m3 holds exactly).  Below 2^-6 the spacing is
-// constant (2^-9): adding 2^-6 puts the value where a float's own spacing under 3 mantissa bits is 2^-9.
-SEMSEG_HD float adam8_round(float x, float inv, uint32_t random16, bool positive) {
-    float a = fabsf(x) * inv;
-    a = a < ADAM8_MAX ? a : ADAM8_MAX;                           // the largest one may come out a bit above
+// what is coded: value / scale, limited to the range (the largest may come out a bit above); a positive r is at least the smallest code
+SEMSEG_HD float adam8_limited(float a, float low) { return fminf(fmaxf(a, low), ADAM8_MAX); }
+SEMSEG_HD float adam8_scaled_m(float m, float inv) { return adam8_limited(m * inv, -ADAM8_MAX); }
+SEMSEG_HD float adam8_scaled_r(float r, float inv) { return adam8_limited(r * inv, r > 0.0f ? 0.001953125f : 0.0f); }
+
+// stochastic rounding of |a| <= 448 to the e4m3 grid: 16 random bits are added below the last kept bit of the mantissa, then all below is
+// cut off.  Below 2^-6 the grid is even (2^-9): adding 2^-6 puts the value where a float's own bits line up with it.  The hardware's
+// conversion (v_cvt_sr_fp8_f32 with the bits on top of its seed) gives the same codes; this form is the host's.
+SEMSEG_HD float adam8_round(float x, uint32_t random16) {
+    float a = fabsf(x);
     const float low = a < 0.015625f ? 0.015625f : 0.0f;
     a = adam_float((adam_bits(a + low) + (random16 << 4)) & ~0xFFFFFu) - low;
-    if (positive && a < 0.001953125f && x > 0.0f && inv > 0.0f) a = 0.001953125f;
-    return inv > 0.0f ? a : 0.0f;
+    return copysignf(a, x);
 }

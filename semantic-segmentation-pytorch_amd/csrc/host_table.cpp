@@ -1,0 +1,239 @@
+// Host side of the multi-tensor entry points: reads lists of torch tensors, checks them and writes the descriptor tables of
+// include/semseg_hip.h.  An optimiser step over a few hundred tensors asks each of them for its address, type, device, size and
+// layout; from Python that costs about 2 us a tensor (0.48 ms for the 168 tensors of ResNet50dilated + PPM with 8-bit states, twice the
+// time of the kernels), here about 20 ns.  A CPython extension, no kernels and no GPU calls in it: the library that holds those stays a
+// plain C ABI.
+#include <Python.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <exception>
+#include <vector>
+
+#include "semseg_hip.h"
+
+namespace {
+
+struct Refused {};                      // a Python error has been set
+
+struct Seq {                            // a list or tuple, held
+    PyObject* fast;
+    explicit Seq(PyObject* o, const char* what) : fast(PySequence_Fast(o, what)) {
+        if (!fast) throw Refused();
+    }
+    ~Seq() { Py_DECREF(fast); }
+    Seq(const Seq&) = delete;
+    Seq& operator=(const Seq&) = delete;
+    Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(fast); }
+    PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(fast, i); }
+};
+
+[[noreturn]] void refuse(PyObject* type, const char* format, ...) {
+    va_list args;
+    va_start(args, format);
+    PyErr_FormatV(type, format, args);
+    va_end(args);
+    throw Refused();
+}
+
+const at::Tensor& tensor(PyObject* o, const char* what) {
+    if (!THPVariable_Check(o)) refuse(PyExc_TypeError, "%s: expected a tensor, got %s", what, Py_TYPE(o)->tp_name);
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.defined() || t.layout() != at::kStrided) refuse(PyExc_TypeError, "%s: tensors must be strided", what);
+    return t;
+}
+
+int type_code(const at::Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return SEMSEG_TYPE_F32;
+        case at::kBFloat16: return SEMSEG_TYPE_BF16;
+        case at::kHalf: return SEMSEG_TYPE_F16;
+        default: return -1;
+    }
+}
+
+// elements of two tensors follow each other in memory in the same order; strides of axes of one element say nothing
+bool same_order(const at::Tensor& a, const at::Tensor& b) {
+    if (a.numel() != b.numel()) return false;
+    const auto sa = a.strides(), sb = b.strides();
+    if (sa == sb) return true;
+    if (a.sizes() != b.sizes()) return false;
+    for (size_t i = 0; i < sa.size(); ++i)
+        if (a.size(i) != 1 && sa[i] != sb[i]) return false;
+    return true;
+}
+
+void* address(const at::Tensor& t) { return const_cast<void*>(t.const_data_ptr()); }
+
+typedef std::vector<std::pair<uintptr_t, uintptr_t>> Ranges;
+void disjoint(Ranges& r, const char* what, const char* name) {
+    std::sort(r.begin(), r.end());
+    for (size_t i = 1; i < r.size(); ++i)
+        if (r[i].first < r[i - 1].second) refuse(PyExc_ValueError, "%s: the same %s twice in one call (or overlapping ones)", what, name);
+}
+
+// the part that both AdamW tables share; returns false for a tensor without elements
+template <class ENTRY>
+bool common(ENTRY& e, const char* what, const at::Tensor& p, PyObject* grad, PyObject* step, PyObject* wd, PyObject* copy,
+            const at::Device& dev, Ranges& params, Ranges& steps) {
+    const at::Tensor& g = tensor(grad, what);
+    const at::Tensor& s = tensor(step, what);
+    if (p.scalar_type() != at::kFloat)
+        refuse(PyExc_TypeError, "%s: parameters must be float32 (a 16-bit copy goes into `copies`)", what);
+    if (type_code(g) < 0) refuse(PyExc_TypeError, "%s: gradients must be float32, bfloat16 or float16", what);
+    if (s.scalar_type() != at::kInt || s.numel() != 1) refuse(PyExc_TypeError, "%s: a step count is one int32 on the device", what);
+    if (p.device() != dev || g.device() != dev || s.device() != dev)
+        refuse(PyExc_ValueError, "%s: all tensors of a call must be on one HIP device", what);
+    if (!p.is_non_overlapping_and_dense() || !same_order(p, g))
+        refuse(PyExc_RuntimeError, "%s: a parameter of %zd elements and its gradient differ in layout or are not dense", what,
+               (Py_ssize_t)p.numel());
+    e.copy = nullptr;
+    e.copy_type = 0;
+    if (copy && copy != Py_None) {
+        const at::Tensor& c = tensor(copy, what);
+        if (type_code(c) <= SEMSEG_TYPE_F32 || c.device() != dev || !same_order(p, c))
+            refuse(PyExc_RuntimeError, "%s: a copy must be bfloat16 or float16 in its parameter's layout on its device", what);
+        e.copy = address(c);
+        e.copy_type = type_code(c);
+    }
+    const double decay = PyFloat_AsDouble(wd);
+    if (decay == -1.0 && PyErr_Occurred()) throw Refused();
+    e.param = address(p);
+    e.grad = address(g);
+    e.step = (int*)address(s);
+    e.numel = p.numel();
+    e.weight_decay = (float)decay;
+    e.grad_type = type_code(g);
+    if (e.numel == 0) return false;
+    params.emplace_back((uintptr_t)e.param, (uintptr_t)e.param + 4 * (uintptr_t)e.numel);
+    steps.emplace_back((uintptr_t)e.step, (uintptr_t)e.step + 4);
+    return true;
+}
+
+template <class ENTRY, class FILL>
+PyObject* adam_table(PyObject* const* args, Py_ssize_t n_states, FILL fill) {
+    const char* what = PyUnicode_AsUTF8(args[0]);
+    if (!what) throw Refused();
+    const char* lists = "expected a list of tensors";
+    Seq params(args[1], lists), grads(args[2], lists), steps(args[3], lists), wds(args[4], "expected a list of numbers");
+    const bool copying = args[5] != Py_None;
+    Seq copies(copying ? args[5] : args[1], lists);
+    const Py_ssize_t n = params.size();
+    bool even = grads.size() == n && steps.size() == n && wds.size() == n && copies.size() == n;
+    std::vector<std::unique_ptr<Seq>> states;
+    for (Py_ssize_t k = 0; k < n_states; ++k) {
+        states.emplace_back(new Seq(args[6 + k], lists));
+        even = even && states.back()->size() == n;
+    }
+    if (!even) refuse(PyExc_ValueError, "%s: the lists differ in length", what);
+    std::vector<ENTRY> table;
+    table.reserve(n);
+    Ranges param_at, step_at;
+    param_at.reserve(n);
+    step_at.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const at::Tensor& p = tensor(params[i], what);
+        const at::Device dev = THPVariable_Unpack(params[0]).device();
+        ENTRY e{};
+        const bool live = common(e, what, p, grads[i], steps[i], wds[i], copying ? copies[i] : nullptr, dev, param_at, step_at);
+        fill(e, what, p, dev, states, i);
+        if (live) table.push_back(e);
+    }
+    disjoint(param_at, what, "parameter");
+    disjoint(step_at, what, "step count");
+    PyObject* bytes = PyBytes_FromStringAndSize((const char*)table.data(), (Py_ssize_t)(table.size() * sizeof(ENTRY)));
+    if (!bytes) throw Refused();
+    return Py_BuildValue("Nn", bytes, (Py_ssize_t)table.size());
+}
+
+void fill32(semseg_adamw_tensor& e, const char* what, const at::Tensor& p, const at::Device& dev,
+            const std::vector<std::unique_ptr<Seq>>& states, Py_ssize_t i) {
+    const at::Tensor& m = tensor((*states[0])[i], what);
+    const at::Tensor& v = tensor((*states[1])[i], what);
+    if (m.scalar_type() != at::kFloat || v.scalar_type() != at::kFloat || m.device() != dev || v.device() != dev || !same_order(p, m) ||
+        !same_order(p, v))
+        refuse(PyExc_RuntimeError, "%s: the states of a parameter of %zd elements must be float32 in its layout on its device", what,
+               (Py_ssize_t)p.numel());
+    e.exp_avg = address(m);
+    e.exp_avg_sq = address(v);
+}
+
+void fill8(semseg_adamw8_tensor& e, const char* what, const at::Tensor& p, const at::Device& dev,
+           const std::vector<std::unique_ptr<Seq>>& states, Py_ssize_t i) {
+    Seq state((*states[0])[i], "expected an AdamW8State");
+    const int64_t n = p.numel(), blocks = (n + 255) / 256;
+    bool ok = state.size() == 4;
+    void* at_[4] = {};
+    for (int k = 0; ok && k < 4; ++k) {
+        const at::Tensor& t = tensor(state[k], what);
+        const bool codes = k % 2 == 0;
+        const auto type = t.scalar_type();
+        ok = (codes ? type == at::kByte || type == at::kFloat8_e4m3fn : type == at::kFloat) && t.numel() == (codes ? n : blocks) &&
+             t.is_contiguous() && t.device() == dev;
+        at_[k] = address(t);
+    }
+    if (!ok)
+        refuse(PyExc_RuntimeError, "%s: the state of a parameter of %zd elements must be as many codes and %zd float32 scales, twice, on its "
+               "device (adamw8_state)", what, (Py_ssize_t)n, (Py_ssize_t)blocks);
+    e.m_codes = at_[0];
+    e.m_scales = at_[1];
+    e.r_codes = at_[2];
+    e.r_scales = at_[3];
+}
+
+template <class F>
+PyObject* guarded(F f) {
+    try {
+        return f();
+    } catch (const Refused&) {
+        return nullptr;
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
+// (what, params, grads, steps, weight_decays, copies or None, exp_avgs, exp_avg_sqs) -> (table, entries)
+PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 8) return PyErr_Format(PyExc_TypeError, "adamw_table: 8 arguments");
+    return guarded([&] { return adam_table<semseg_adamw_tensor>(args, 2, fill32); });
+}
+// (what, params, grads, steps, weight_decays, copies or None, states) -> (table, entries)
+PyObject* adamw8_table(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 7) return PyErr_Format(PyExc_TypeError, "adamw8_table: 7 arguments");
+    return guarded([&] { return adam_table<semseg_adamw8_tensor>(args, 1, fill8); });
+}
+// (grads,) -> (table, entries)
+PyObject* grad_table(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 1) return PyErr_Format(PyExc_TypeError, "grad_table: 1 argument");
+    return guarded([&]() -> PyObject* {
+        const char* what = "grad_norm";
+        Seq grads(args[0], "expected a list of tensors");
+        std::vector<semseg_grad_tensor> table;
+        table.reserve(grads.size());
+        for (Py_ssize_t i = 0; i < grads.size(); ++i) {
+            const at::Tensor& g = tensor(grads[i], what);
+            if (type_code(g) < 0) refuse(PyExc_TypeError, "%s: gradients must be float32, bfloat16 or float16", what);
+            if (g.device() != THPVariable_Unpack(grads[0]).device()) refuse(PyExc_ValueError, "%s: all gradients must be on one HIP device", what);
+            if (!g.is_non_overlapping_and_dense()) refuse(PyExc_RuntimeError, "%s: a gradient of %zd elements is not dense", what, (Py_ssize_t)g.numel());
+            semseg_grad_tensor e{};
+            e.grad = address(g);
+            e.numel = g.numel();
+            e.grad_type = type_code(g);
+            if (e.numel) table.push_back(e);
+        }
+        PyObject* bytes = PyBytes_FromStringAndSize((const char*)table.data(), (Py_ssize_t)(table.size() * sizeof(table[0])));
+        if (!bytes) throw Refused();
+        return Py_BuildValue("Nn", bytes, (Py_ssize_t)table.size());
+    });
+}
+
+PyMethodDef methods[] = {{"adamw_table", (PyCFunction)(void*)adamw_table, METH_FASTCALL, nullptr},
+                         {"adamw8_table", (PyCFunction)(void*)adamw8_table, METH_FASTCALL, nullptr},
+                         {"grad_table", (PyCFunction)(void*)grad_table, METH_FASTCALL, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__host(void) { return PyModule_Create(&module); }

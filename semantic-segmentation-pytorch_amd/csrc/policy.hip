@@ -15,6 +15,7 @@
 
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 template <class T, int V>
 struct Vec {
@@ -25,13 +26,32 @@ struct Vec<T, 1> {
     typedef T type;
 };
 template <class T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&x)[V]) {
-    const typename Vec<T, V>::type v = *reinterpret_cast<const typename Vec<T, V>::type*>(p);
+__device__ __forceinline__ void unpack(const typename Vec<T, V>::type& v, float (&x)[V]) {
     if constexpr (V == 1) {
         x[0] = (float)v;
     } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) x[j] = (float)v[j];
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ void load_vec(const T* p, float (&x)[V]) {
+    unpack<T, V>(*reinterpret_cast<const typename Vec<T, V>::type*>(p), x);
+}
+// H vectors of a row, a group of G lanes' apart; what lies behind the row is -infinity
+template <class T, int G, int V, int H>
+__device__ __forceinline__ void load_part(const T* __restrict__ zr, int c0, int C, typename Vec<T, V>::type (&raw)[H]) {
+#pragma unroll
+    for (int u = 0; u < H; ++u) {
+        const int c = c0 + u * (G * V);
+        if (c + V <= C) {
+            raw[u] = *reinterpret_cast<const typename Vec<T, V>::type*>(zr + c);
+        } else if constexpr (V == 1) {
+            raw[u] = (T)-INFINITY;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) raw[u][j] = c + j < C ? zr[c + j] : (T)-INFINITY;
+        }
     }
 }
 template <class T, int V>
@@ -54,6 +74,7 @@ struct PolicyArgs {
     const float* old_logp;              // [P]
     const float* ref_logp;              // [P] or NULL
     int64_t rows_per_advantage;
+    int small_rows;                     // row numbers fit 32 bits (a 64-bit division costs more than a row of 150 classes)
     float clip_low, clip_high, kl_weight;
     float* coef;                        // [P] d(loss * valid rows) / d lp
     double* partial;                    // [blocks][4]: loss, kl, clipped, valid
@@ -88,6 +109,66 @@ __device__ __forceinline__ float group_sum(float v, float* lds) {
     return v;
 }
 
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+struct RowSums {
+    double loss = 0.0, kl = 0.0;
+    int clipped = 0, count = 0;
+};
+// one row's answer, by one lane
+template <bool POLICY>
+__device__ __forceinline__ void finish_row(int64_t row, float za, bool valid, float top, float logs, float* __restrict__ lp_out,
+                                           float2* __restrict__ stats, const PolicyArgs& pa, RowSums& acc) {
+    const float lp = valid ? (za - top) - logs : 0.f;
+    if (stats) stats[row] = make_float2(top, logs);
+    if constexpr (!POLICY) {
+        lp_out[row] = lp;
+    } else {
+        float coef = 0.f;
+        if (valid) {
+            const float A = pa.advantage[pa.small_rows ? (int64_t)((uint32_t)row / (uint32_t)pa.rows_per_advantage) : row / pa.rows_per_advantage];
+            const float ratio = expf(lp - pa.old_logp[row]);
+            const float whole = ratio * A;
+            const float cut = fminf(fmaxf(ratio, 1.f - pa.clip_low), 1.f + pa.clip_high) * A;
+            const bool clip = cut < whole;
+            float l = clip ? -cut : -whole;
+            coef = clip ? 0.f : -whole;
+            if (pa.ref_logp) {
+                const float d = pa.ref_logp[row] - lp;
+                const float e = expm1f(d);                           // exp(d) - 1 - d cancels for small d
+                const float k = e - d;
+                l = fmaf(pa.kl_weight, k, l);
+                coef = fmaf(-pa.kl_weight, e, coef);
+                acc.kl += (double)k;
+            }
+            acc.loss += (double)l;
+            acc.clipped += clip ? 1 : 0;
+            acc.count += 1;
+        }
+        pa.coef[row] = coef;
+    }
+}
+__device__ __forceinline__ void block_partial(const RowSums& acc, double* __restrict__ partial) {
+    __shared__ double sum[4][4];
+    const double loss = wave_sum_d(acc.loss), kl = wave_sum_d(acc.kl);
+    const double clipped = wave_sum_d((double)acc.clipped), count = wave_sum_d((double)acc.count);
+    const int w = threadIdx.x >> 6, j = threadIdx.x;
+    if ((threadIdx.x & 63) == 0) { sum[w][0] = loss; sum[w][1] = kl; sum[w][2] = clipped; sum[w][3] = count; }
+    __syncthreads();
+    if (j < 4) partial[(int64_t)blockIdx.x * 4 + j] = (sum[0][j] + sum[1][j]) + (sum[2][j] + sum[3][j]);
+}
+
 // POLICY: the loss (lp is not written); otherwise lp of every row.  stats[row] = {max, log sum} (may be NULL)
 template <class T, int G, int V, bool POLICY>
 __global__ __launch_bounds__(256) void label_logp_kernel(const T* __restrict__ z, int64_t ld, const int64_t* __restrict__ label,
@@ -96,7 +177,7 @@ __global__ __launch_bounds__(256) void label_logp_kernel(const T* __restrict__ z
     __shared__ float lds[8];
     constexpr int ROWS = 256 / G;
     const int sub = threadIdx.x % G;
-    double loss = 0.0, kl = 0.0, clipped = 0.0, count = 0.0;
+    RowSums acc;
     for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < P; row0 += (int64_t)gridDim.x * ROWS) {
         const int64_t row = row0 + threadIdx.x / G;
         const bool live = row < P;
@@ -106,79 +187,103 @@ __global__ __launch_bounds__(256) void label_logp_kernel(const T* __restrict__ z
         const float za = valid ? (float)zr[a] : 0.f;
         float m = -INFINITY, s = 0.f;
         if (live) {
-            for (int c0 = sub * V; c0 < C; c0 += G * V * LP_HELD) {
-                float x[LP_HELD][V];
+            // a long row (a block's) has the next part on its way while one is summed
+            constexpr int HELD = G == 256 ? LP_HELD / 2 : LP_HELD;
+            typename Vec<T, V>::type raw[HELD], next[HELD];
+            load_part<T, G, V, HELD>(zr, sub * V, C, raw);
+            for (int c0 = sub * V; c0 < C; c0 += G * V * HELD) {
+                if (G == 256 && c0 + G * V * HELD < C) load_part<T, G, V, HELD>(zr, c0 + G * V * HELD, C, next);
+                __builtin_amdgcn_sched_barrier(0);
+                float x[HELD][V];
                 float top = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < LP_HELD; ++u) {
-                    const int c = c0 + u * (G * V);
-                    if (c + V <= C) {
-                        load_vec<T, V>(zr + c, x[u]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < V; ++j) x[u][j] = c + j < C ? (float)zr[c + j] : -INFINITY;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < LP_HELD; ++u)
+                for (int u = 0; u < HELD; ++u) {
+                    unpack<T, V>(raw[u], x[u]);
 #pragma unroll
                     for (int j = 0; j < V; ++j) top = fmaxf(top, x[u][j]);
+                }
                 const float mn = fmaxf(m, top);
                 const float ref = mn == -INFINITY ? 0.f : mn;            // nothing but -infinity so far: exp(-inf) = 0, not NaN
                 s *= m == -INFINITY ? 0.f : __expf(m - ref);
 #pragma unroll
-                for (int u = 0; u < LP_HELD; ++u)
+                for (int u = 0; u < HELD; ++u)
 #pragma unroll
                     for (int j = 0; j < V; ++j) s += __expf(x[u][j] - ref);
                 m = mn;
+                if (G < 256) break;                                      // rows of a group fit its lanes' registers (group_of)
+#pragma unroll
+                for (int u = 0; u < HELD; ++u) raw[u] = next[u];
             }
         }
         const float top = group_max<G>(m, lds);
         const float ref = top == -INFINITY ? 0.f : top;
         s = group_sum<G>(m == -INFINITY && s == 0.f ? 0.f : s * __expf(m - ref), lds);
         const float logs = logf(s);
-        if (sub == 0 && live) {
-            const float lp = valid ? (za - ref) - logs : 0.f;
-            if (stats) stats[row] = make_float2(ref, logs);
-            if constexpr (!POLICY) {
-                lp_out[row] = lp;
+        if (sub == 0 && live) finish_row<POLICY>(row, za, valid, ref, logs, lp_out, stats, pa, acc);
+    }
+    if constexpr (POLICY) block_partial(acc, pa.partial);
+}
+
+// Dense rows of few classes: a block takes 256 / L rows, one stretch of memory, in 16-byte loads that no row's start or end interrupts,
+// through LDS; then L lanes read a row each.  A row alone is 300 to 600 bytes at 150 classes: loads of its own are 4 or 8 bytes wide.
+constexpr int TILE_BYTES = 20480;       // 8 blocks of a compute unit at once
+template <class T, int L, int W, bool POLICY>
+__global__ __launch_bounds__(256) void label_logp_tile_kernel(const T* __restrict__ z, const int64_t* __restrict__ label, int64_t ignore,
+                                                              int64_t P, int C, float* __restrict__ lp_out, float2* __restrict__ stats,
+                                                              const PolicyArgs pa) {
+    constexpr int ROWS = 256 / L, PER = 16 / (int)sizeof(T);
+    constexpr int HELD = TILE_BYTES / 256 / ((int)sizeof(T) * W);      // W: elements of a read from LDS (2 where C is even)
+    __shared__ u32x4 tile[TILE_BYTES / 16];
+    const int sub = threadIdx.x % L;
+    const int64_t tiles = (P + ROWS - 1) / ROWS;
+    RowSums acc;
+    for (int64_t b = blockIdx.x; b < tiles; b += gridDim.x) {
+        const int64_t row0 = b * ROWS, row = row0 + threadIdx.x / L;
+        const int count = (int)min(P - row0, (int64_t)ROWS) * C;       // elements of this tile
+        const T* src = z + row0 * C;                                   // ROWS * C elements are whole 16-byte pieces: L <= 16
+        const int vecs = count / PER;
+        const bool live = row < P;
+        const int64_t a = live ? label[row] : -1;
+        u32x4 v[TILE_BYTES / 4096];
+#pragma unroll
+        for (int u = 0; u < TILE_BYTES / 4096; ++u)
+            v[u] = vecs ? reinterpret_cast<const u32x4*>(src)[min((int)threadIdx.x + u * 256, vecs - 1)] : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int u = 0; u < TILE_BYTES / 4096; ++u)
+            if ((int)threadIdx.x + u * 256 < vecs) tile[threadIdx.x + u * 256] = v[u];
+        T* t = reinterpret_cast<T*>(tile);
+        for (int i = vecs * PER + threadIdx.x; i < count; i += 256) t[i] = src[i];         // the end of the last tile
+        __syncthreads();
+        const bool valid = live && a != ignore && a >= 0 && a < C;
+        const T* tr = t + (live ? threadIdx.x / L : 0) * C;
+        float x[HELD][W];
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) {
+            const int c = (sub + k * L) * W;
+            if (c < C) {
+                load_vec<T, W>(tr + c, x[k]);
             } else {
-                float coef = 0.f;
-                if (valid) {
-                    const float A = pa.advantage[row / pa.rows_per_advantage];
-                    const float ratio = expf(lp - pa.old_logp[row]);
-                    const float whole = ratio * A;
-                    const float cut = fminf(fmaxf(ratio, 1.f - pa.clip_low), 1.f + pa.clip_high) * A;
-                    const bool clip = cut < whole;
-                    float l = clip ? -cut : -whole;
-                    coef = clip ? 0.f : -whole;
-                    float k = 0.f;
-                    if (pa.ref_logp) {
-                        const float d = pa.ref_logp[row] - lp;
-                        const float e = expm1f(d);                       // exp(d) - 1 - d cancels for small d
-                        k = e - d;
-                        l = fmaf(pa.kl_weight, k, l);
-                        coef = fmaf(-pa.kl_weight, e, coef);
-                    }
-                    loss += (double)l;
-                    kl += (double)k;
-                    clipped += clip ? 1.0 : 0.0;
-                    count += 1.0;
-                }
-                pa.coef[row] = coef;
+#pragma unroll
+                for (int j = 0; j < W; ++j) x[k][j] = -INFINITY;
             }
         }
-    }
-    if constexpr (POLICY) {
-        __shared__ double sum[4][4];
-        loss = wave_sum_d(loss); kl = wave_sum_d(kl); clipped = wave_sum_d(clipped); count = wave_sum_d(count);
-        const int w = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) { sum[w][0] = loss; sum[w][1] = kl; sum[w][2] = clipped; sum[w][3] = count; }
+#pragma unroll
+        for (int k = 0; k < HELD; ++k)
+#pragma unroll
+            for (int j = 0; j < W; ++j) m = fmaxf(m, x[k][j]);
+        m = lanes_max<L>(m);
+        const float top = m == -INFINITY ? 0.f : m;
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < HELD; ++k)
+#pragma unroll
+            for (int j = 0; j < W; ++j) s += __expf(x[k][j] - top);
+        s = lanes_sum<L>(s);
+        if (sub == 0 && live) finish_row<POLICY>(row, valid ? (float)tr[a] : 0.f, valid, top, logf(s), lp_out, stats, pa, acc);
         __syncthreads();
-        if (threadIdx.x < 4)
-            pa.partial[(int64_t)blockIdx.x * 4 + threadIdx.x] =
-                (sum[0][threadIdx.x] + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x]);
     }
+    if constexpr (POLICY) block_partial(acc, pa.partial);
 }
 
 struct PolicyOut {
@@ -308,8 +413,39 @@ static int lp_group(const LpCall& c, int G) {
         default: return lp_launch<T, 256, V>(c);
     }
 }
+// lanes of a row in the tile kernel: the fewest whose rows fit the tile; 0: rows too long, not dense or not aligned
+static int tile_lanes(int bytes, const void* z, int64_t ld, int64_t P, int C) {
+    if ((ld != C && P > 1) || !aligned16(z)) return 0;
+    for (int l = 1; l <= 16; l *= 2)
+        if ((int64_t)(256 / l) * C * bytes <= TILE_BYTES) return l;
+    return 0;
+}
+template <class T, int L, int W>
+static int tile_launch(const LpCall& c) {
+    const int64_t tiles = (c.P + 256 / L - 1) / (256 / L);
+    const int grid = (int)(tiles < LP_MAX_BLOCKS ? tiles : LP_MAX_BLOCKS);
+    if (c.pa) {
+        auto k = label_logp_tile_kernel<T, L, W, true>;
+        hipLaunchKernelGGL(k, dim3(grid), dim3(256), 0, c.st, (const T*)c.z, c.label, c.ignore, c.P, c.C, (float*)nullptr, c.stats, *c.pa);
+    } else {
+        auto k = label_logp_tile_kernel<T, L, W, false>;
+        hipLaunchKernelGGL(k, dim3(grid), dim3(256), 0, c.st, (const T*)c.z, c.label, c.ignore, c.P, c.C, c.lp, c.stats, PolicyArgs{});
+    }
+    SEMSEG_LAUNCH_CHECK();
+    return 0;
+}
 template <class T>
 static int lp_typed(const LpCall& c) {
+    if (!c.dz) {
+        switch (tile_lanes((int)sizeof(T), c.z, c.ld, c.P, c.C)) {
+            case 1: return c.C % 2 ? tile_launch<T, 1, 1>(c) : tile_launch<T, 1, 2>(c);
+            case 2: return c.C % 2 ? tile_launch<T, 2, 1>(c) : tile_launch<T, 2, 2>(c);
+            case 4: return c.C % 2 ? tile_launch<T, 4, 1>(c) : tile_launch<T, 4, 2>(c);
+            case 8: return c.C % 2 ? tile_launch<T, 8, 1>(c) : tile_launch<T, 8, 2>(c);
+            case 16: return c.C % 2 ? tile_launch<T, 16, 1>(c) : tile_launch<T, 16, 2>(c);
+            default: break;
+        }
+    }
     const int V = vec_of((int)sizeof(T), c.z, c.ld, c.dz, c.C);
     const int G = group_of(c.C, V);
     if constexpr (sizeof(T) == 4) {
@@ -349,13 +485,15 @@ extern "C" int semseg_policy_loss_fwd(const void* z, int type, int64_t ld, const
     if (!workspace || workspace_bytes < semseg_policy_loss_workspace_bytes()) return SEMSEG_EWORKSPACE;
     PolicyArgs pa{};
     pa.advantage = advantage; pa.old_logp = old_logp; pa.ref_logp = ref_logp; pa.rows_per_advantage = rows_per_advantage;
+    pa.small_rows = P <= (int64_t)1 << 31 && rows_per_advantage <= (int64_t)1 << 31;
     pa.clip_low = clip_low; pa.clip_high = clip_high; pa.kl_weight = kl_weight; pa.coef = coef; pa.partial = (double*)workspace;
     LpCall c{};
     c.z = z; c.ld = ld; c.label = label; c.ignore = ignore_index; c.P = P; c.C = C; c.stats = (float2*)stats; c.st = (hipStream_t)stream;
     c.pa = &pa;
     if (int rc = lp_dispatch(c, type)) return rc;
     const int bytes = type == SEMSEG_TYPE_F32 ? 4 : 2;
-    const int blocks = lp_blocks(P, group_of(C, vec_of(bytes, z, ld, nullptr, C)), LP_MAX_BLOCKS);
+    const int l = tile_lanes(bytes, z, ld, P, C);
+    const int blocks = lp_blocks(P, l ? l : group_of(C, vec_of(bytes, z, ld, nullptr, C)), LP_MAX_BLOCKS);
     hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(256), 0, c.st, (const double*)workspace, blocks,
                        PolicyOut{{loss, kl, clipped, inv_count}});
     SEMSEG_LAUNCH_CHECK();

@@ -27,20 +27,6 @@ class SgdTensor2(ctypes.Structure):
                 ('first_step', c_int), ('slabs', vp), ('splits', c_int), ('absmax_slots', vp)]
 
 
-class AdamWTensor(ctypes.Structure):
-    _fields_ = [('param', vp), ('grad', vp), ('exp_avg', vp), ('exp_avg_sq', vp), ('copy', vp), ('step', vp),
-                ('numel', ctypes.c_int64), ('weight_decay', c_f), ('grad_type', c_int), ('copy_type', c_int)]
-
-
-class AdamW8Tensor(ctypes.Structure):
-    _fields_ = [('param', vp), ('grad', vp), ('copy', vp), ('m_codes', vp), ('m_scales', vp), ('r_codes', vp), ('r_scales', vp),
-                ('step', vp), ('numel', ctypes.c_int64), ('weight_decay', c_f), ('grad_type', c_int), ('copy_type', c_int)]
-
-
-class GradTensor(ctypes.Structure):
-    _fields_ = [('grad', vp), ('numel', ctypes.c_int64), ('grad_type', c_int)]
-
-
 class SlabTensor(ctypes.Structure):
     _fields_ = [('slabs', vp), ('out', vp), ('numel', ctypes.c_int64), ('splits', c_int)]
 
@@ -246,6 +232,16 @@ def lib():
             fn.argtypes = args
         _lib = h
     return _lib
+
+
+def host():
+    """the CPython extension that turns lists of tensors into descriptor tables (csrc/host_table.cpp); raises if it is not built"""
+    try:
+        from . import _host
+    except ImportError as e:
+        raise NativeLibraryMissing('%s/_host.so not built or not loadable (%s): run `python '
+                                   'semantic-segmentation-pytorch_amd/build_native.py`' % (_HERE, e))
+    return _host
 
 
 class NativeError(RuntimeError):

@@ -14,7 +14,6 @@ import contextlib
 import ctypes
 import os
 
-import numpy as np
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
@@ -2357,7 +2356,9 @@ def _row_labels(what, z, rows, label):
         raise ValueError('%s: expected labels of shape %s, got %s' % (what, rows, tuple(label.shape)))
     if label.device != z.device:
         raise ValueError('%s: labels on %s, logits on %s' % (what, label.device, z.device))
-    return label.detach().to(torch.int64).contiguous()
+    if label.dtype is not torch.int64:
+        label = label.to(torch.int64)
+    return label if label.is_contiguous() else label.contiguous()
 
 
 def _empty_like_rows(z, shape):
@@ -2368,13 +2369,21 @@ def _empty_like_rows(z, shape):
 
 
 def _label_logp_bwd(z, ld, shape, label, ignore_index, stats, g, gloss, inv_count):
+    """gradient of the logits; stats, g, gloss, inv_count: device addresses"""
     dz = _empty_like_rows(z, shape)
     P = label.numel()
     if P:
         with _device_guard(z.device):
-            _native.check(_native.lib().semseg_label_logp_bwd(_p(z), _TYPE_CODES[z.dtype], ld, _p(label), ignore_index, _p(stats), _p(g),
-                                                              _p(gloss), _p(inv_count), P, shape[1], _p(dz), _st()), 'label_logp_bwd')
+            _native.check(_native.lib().semseg_label_logp_bwd(z.data_ptr(), _TYPE_CODES[z.dtype], ld, label.data_ptr(), ignore_index, stats,
+                                                              g, gloss, inv_count, P, shape[1], dz.data_ptr(), _st()), 'label_logp_bwd')
     return dz
+
+
+def _upstream(g):
+    """an upstream gradient as dense float32"""
+    if g.dtype is not torch.float32:
+        g = g.float()
+    return g if g.is_contiguous() else g.contiguous()
 
 
 class LabelLogProbFn(Function):
@@ -2384,11 +2393,11 @@ class LabelLogProbFn(Function):
         label = _row_labels('label_log_prob', z, rows, label)
         z, ld, P, c = _logit_rows(z)
         lp = torch.empty(rows, device=z.device, dtype=torch.float32)
-        stats = torch.empty((P, 2), device=z.device, dtype=torch.float32) if ctx.needs_input_grad[0] else None
+        stats = torch.empty(2 * P, device=z.device, dtype=torch.float32) if ctx.needs_input_grad[0] else None
         if P:
             with _device_guard(z.device):
-                _native.check(_native.lib().semseg_label_logp_fwd(_p(z), _TYPE_CODES[z.dtype], ld, _p(label), ignore_index, P, c, _p(lp),
-                                                                  _p(stats), _st()), 'label_logp_fwd')
+                _native.check(_native.lib().semseg_label_logp_fwd(z.data_ptr(), _TYPE_CODES[z.dtype], ld, label.data_ptr(), ignore_index, P,
+                                                                  c, lp.data_ptr(), _p(stats), _st()), 'label_logp_fwd')
         if stats is not None:
             ctx.save_for_backward(z, label, stats)
             ctx.cfg = (ld, shape, ignore_index)
@@ -2399,7 +2408,8 @@ class LabelLogProbFn(Function):
     def backward(ctx, g):
         z, label, stats = ctx.saved_tensors
         ld, shape, ignore_index = ctx.cfg
-        return _label_logp_bwd(z, ld, shape, label, ignore_index, stats, g.float().contiguous(), None, None), None, None
+        g = _upstream(g)
+        return _label_logp_bwd(z, ld, shape, label, ignore_index, stats.data_ptr(), g.data_ptr(), 0, 0), None, None
 
 
 def label_log_prob(z, label, ignore_index=-1):
@@ -2420,7 +2430,9 @@ def _row_constants(what, name, t, shapes, device):
         raise ValueError('%s: expected %s of shape %s, got %s' % (what, name, ' or '.join(map(str, shapes)), tuple(t.shape)))
     if t.device != device:
         raise ValueError('%s: %s on %s, logits on %s' % (what, name, t.device, device))
-    return t.float().contiguous()
+    if t.dtype is not torch.float32:
+        t = t.float()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 class PolicyLossFn(Function):
@@ -2429,26 +2441,32 @@ class PolicyLossFn(Function):
         what = 'policy_loss'
         shape, dev, rows = tuple(z.shape), z.device, _row_shape(what, z)
         label = _row_labels(what, z, rows, label)
-        advantage = _row_constants(what, 'advantage', advantage, ((rows[0],), rows) if z.dim() == 4 else (rows,), dev)
+        advantage = _row_constants(what, 'advantage', advantage, ((rows[0],), rows) if len(rows) == 3 else (rows,), dev)
         old_logp = _row_constants(what, 'old_logp', old_logp, (rows,), dev)
-        ref_logp = None if ref_logp is None else _row_constants(what, 'ref_logp', ref_logp, (rows,), dev)
+        if ref_logp is not None:
+            ref_logp = _row_constants(what, 'ref_logp', ref_logp, (rows,), dev)
         z, ld, P, c = _logit_rows(z)
+        ctx.set_materialize_grads(False)
         if P == 0:
-            loss, kl, clipped, inv = (torch.zeros((), device=dev) for _ in range(4))
-            stats = coef = torch.empty(0, device=dev)
+            loss, kl, clipped = (torch.zeros((), device=dev) for _ in range(3))
+            kept = torch.zeros(1, device=dev)
         else:
-            loss, kl, clipped, inv = (torch.empty((), device=dev) for _ in range(4))
-            stats, coef = torch.empty((P, 2), device=dev), torch.empty(P, device=dev)
+            loss, kl, clipped = (torch.empty((), device=dev) for _ in range(3))
             L = _native.lib()
-            # scratch of its own: the caching allocator orders its reuse by stream and by captured graph
-            ws = torch.empty(L.semseg_policy_loss_workspace_bytes(), device=dev, dtype=torch.uint8)
+            # one buffer of its own (the caching allocator orders its reuse by stream and by captured graph): what the backward pass
+            # reads -- maximum and logarithm of the sum per row, gradient per row, 1 / rows that count -- and the partial sums
+            scratch = L.semseg_policy_loss_workspace_bytes()
+            kept = torch.empty(scratch // 4 + 3 * P + 1, device=dev, dtype=torch.float32)
+            ws = kept.data_ptr()
+            stats = ws + scratch
+            coef = stats + 8 * P
             with _device_guard(dev):
-                _native.check(L.semseg_policy_loss_fwd(_p(z), _TYPE_CODES[z.dtype], ld, _p(label), ignore_index, P, c, _p(advantage),
-                                                       P // advantage.numel(), _p(old_logp), _p(ref_logp), clip_low, clip_high, kl_weight,
-                                                       _p(stats), _p(coef), _p(loss), _p(kl), _p(clipped), _p(inv), _p(ws), ws.numel(),
-                                                       _st()), 'policy_loss_fwd')
+                _native.check(L.semseg_policy_loss_fwd(z.data_ptr(), _TYPE_CODES[z.dtype], ld, label.data_ptr(), ignore_index, P, c,
+                                                       advantage.data_ptr(), P // advantage.numel(), old_logp.data_ptr(), _p(ref_logp),
+                                                       clip_low, clip_high, kl_weight, stats, coef, loss.data_ptr(), kl.data_ptr(),
+                                                       clipped.data_ptr(), coef + 4 * P, ws, scratch, _st()), 'policy_loss_fwd')
         if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(z, label, stats, coef, inv)
+            ctx.save_for_backward(z, label, kept)
             ctx.cfg = (ld, shape, ignore_index)
         ctx.mark_non_differentiable(kl, clipped)
         return loss, kl, clipped
@@ -2456,10 +2474,15 @@ class PolicyLossFn(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gloss, gkl, gclipped):
-        z, label, stats, coef, inv = ctx.saved_tensors
+        if gloss is None:
+            return (None,) * 9
+        z, label, kept = ctx.saved_tensors
         ld, shape, ignore_index = ctx.cfg
-        dz = _label_logp_bwd(z, ld, shape, label, ignore_index, stats, coef, gloss.float().contiguous(), inv)
-        return (dz,) + (None,) * 8
+        gloss = _upstream(gloss)
+        P = label.numel()
+        inv = kept.data_ptr() + 4 * (kept.numel() - 1)
+        coef = inv - 4 * P
+        return (_label_logp_bwd(z, ld, shape, label, ignore_index, coef - 8 * P, coef, gloss.data_ptr(), inv),) + (None,) * 8
 
 
 def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip_high=0.2, kl_weight=0.0, ignore_index=-1):
@@ -2546,9 +2569,6 @@ def finish_leftover_slabs():
 
 
 # ---- AdamW (csrc/adamw.hip) ------------------------------------------------------------------------------------------------------
-_ADAMW = np.dtype(_native.AdamWTensor)
-_ADAMW8 = np.dtype(_native.AdamW8Tensor)
-_GRADS = np.dtype(_native.GradTensor)
 ADAMW8_BLOCK = 256          # elements that share one scale of the 8-bit states
 
 # 8-bit states of one parameter, in the order of its memory: e4m3 codes of the first moment and of the square root of the second, one
@@ -2556,73 +2576,17 @@ ADAMW8_BLOCK = 256          # elements that share one scale of the 8-bit states
 AdamW8State = collections.namedtuple('AdamW8State', 'm m_scale r r_scale')
 
 
-def _is_dense(t):
-    """every element of the tensor's span of memory belongs to it, once"""
-    if t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)):
-        return True
-    want = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
-
-
-def _same_order(a, b):
-    """two tensors whose elements follow each other in memory in the same order (strides of axes of one element say nothing)"""
-    if a.stride() == b.stride():
-        return a.numel() == b.numel()
-    return a.shape == b.shape and all(x == y or n == 1 for x, y, n in zip(a.stride(), b.stride(), a.shape))
-
-
-def _optimiser_lists(what, params, grads, steps, weight_decays, lr_tensor, betas, eps, clip, copies, states):
-    """the checks of arguments that the AdamW steps share; returns (device, live indices)"""
-    n = len(params)
-    if not (len(grads) == len(steps) == len(weight_decays) == n and all(len(s) == n for s in states) and
-            (copies is None or len(copies) == n)):
-        raise ValueError('%s: the lists differ in length' % what)
+def _check_step(what, params, lr_tensor, betas, eps, clip):
+    """the arguments of an AdamW step that are not lists (the lists: csrc/host_table.cpp)"""
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0) or not 0.0 <= eps < float('inf'):
         raise ValueError('%s: betas must lie in [0, 1) and eps must not be negative, got %r, %r' % (what, betas, eps))
-    if n == 0:
-        return None, []
-    dev = params[0].device
-    _require_cuda(params[0])
-    index = params[0].get_device()
-    for p, g, s in zip(params, grads, steps):
-        if p.dtype is not torch.float32:
-            raise TypeError('%s: parameters must be float32 (a 16-bit copy goes into `copies`), got %s' % (what, p.dtype))
-        if g.dtype not in _TYPE_CODES:
-            raise TypeError('%s: gradients must be float32, bfloat16 or float16, got %s' % (what, g.dtype))
-        if s.dtype is not torch.int32 or s.numel() != 1:
-            raise TypeError('%s: a step count is one int32 on the device, got %s %s' % (what, s.dtype, tuple(s.shape)))
-        if p.get_device() != index or g.get_device() != index or s.get_device() != index:
-            raise ValueError('%s: all tensors of a call must be on one HIP device' % what)
-        if not _same_order(p, g) or not _is_dense(p):
-            raise RuntimeError('%s: a %s parameter and its gradient differ in layout or are not dense (strides %s, %s)'
-                               % (what, tuple(p.shape), p.stride(), g.stride()))
-    for more, c in zip(params, copies or ()):
-        if c is not None and (c.dtype not in (torch.bfloat16, torch.float16) or c.get_device() != index or not _same_order(more, c)):
-            raise RuntimeError('%s: a copy must be bfloat16 or float16 in its parameter\'s layout on its device' % what)
-    for name, t, count in (('lr_tensor', lr_tensor, 1), ('clip', clip, 2)):
-        if t is not None and (t.dtype is not torch.float32 or t.numel() != count or not t.is_contiguous() or t.get_device() != index):
-            raise ValueError('%s: %s must hold %d float32 on the parameters\' device' % (what, name, count))
-    live = [i for i in range(n) if params[i].numel()]
-    if len({params[i].data_ptr() for i in live}) != len(live) or len({steps[i].data_ptr() for i in live}) != len(live):
-        raise ValueError('%s: the same parameter or step count twice in one call' % what)
-    return dev, live
-
-
-def _fill_common(rec, params, grads, steps, weight_decays, copies, live):
-    rec['param'] = [params[i].data_ptr() for i in live]
-    rec['grad'] = [grads[i].data_ptr() for i in live]
-    rec['step'] = [steps[i].data_ptr() for i in live]
-    rec['numel'] = [params[i].numel() for i in live]
-    rec['weight_decay'] = [weight_decays[i] for i in live]
-    rec['grad_type'] = [_TYPE_CODES[grads[i].dtype] for i in live]
-    if copies is not None:
-        rec['copy'] = [0 if copies[i] is None else copies[i].data_ptr() for i in live]
-        rec['copy_type'] = [0 if copies[i] is None else _TYPE_CODES[copies[i].dtype] for i in live]
+    if params:
+        _require_cuda(params[0])
+        index = params[0].get_device()
+        for name, t, count in (('lr_tensor', lr_tensor, 1), ('clip', clip, 2)):
+            if t is not None and (t.dtype is not torch.float32 or t.numel() != count or not t.is_contiguous() or t.get_device() != index):
+                raise ValueError("%s: %s must hold %d float32 on the parameters' device" % (what, name, count))
 
 
 def _weights_changed(params):
@@ -2643,24 +2607,16 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, weight_decays, lr_te
     returned -- its factor multiplies them too, and where its norm is not finite the call changes nothing; copies: optional list of
     bfloat16 / float16 tensors (or None) that receive the updated parameters.  Everything the step reads that changes from step to
     step is device memory, so a captured call can be replayed."""
-    dev, live = _optimiser_lists('adamw_step', params, grads, steps, weight_decays, lr_tensor, betas, eps, clip, copies,
-                                 (exp_avgs, exp_avg_sqs))
-    if not live:
+    _check_step('adamw_step', params, lr_tensor, betas, eps, clip)
+    table, n = _native.host().adamw_table('adamw_step', params, grads, steps, weight_decays, copies, exp_avgs, exp_avg_sqs)
+    if n == 0:
         return
-    index = params[0].get_device()
-    for p, m, v in zip(params, exp_avgs, exp_avg_sqs):
-        if m.dtype is not torch.float32 or v.dtype is not torch.float32 or m.get_device() != index or v.get_device() != index or \
-                not _same_order(p, m) or not _same_order(p, v):
-            raise RuntimeError('adamw_step: the states of a %s parameter must be float32 in its layout on its device' % (tuple(p.shape),))
-    rec = np.zeros(len(live), dtype=_ADAMW)
-    _fill_common(rec, params, grads, steps, weight_decays, copies, live)
-    rec['exp_avg'] = [exp_avgs[i].data_ptr() for i in live]
-    rec['exp_avg_sq'] = [exp_avg_sqs[i].data_ptr() for i in live]
-    L = _native.lib()
+    L, dev = _native.lib(), params[0].device
     with _device_guard(dev):
-        ws = torch.empty(L.semseg_adamw_workspace_bytes(len(live)), device=dev, dtype=torch.uint8)
-        _native.check(L.semseg_adamw_step(vp(rec.ctypes.data), len(live), _p(lr_tensor), betas[0], betas[1], eps, float(grad_scale),
-                                          _p(clip), _p(ws), ws.numel(), _st()), 'adamw_step')
+        # scratch of its own: the caching allocator orders its reuse by stream and by captured graph
+        ws = torch.empty(L.semseg_adamw_workspace_bytes(n), device=dev, dtype=torch.uint8)
+        _native.check(L.semseg_adamw_step(table, n, _p(lr_tensor), betas[0], betas[1], eps, grad_scale, _p(clip), _p(ws), ws.numel(),
+                                          _st()), 'adamw_step')
     _weights_changed(params)
 
 
@@ -2693,29 +2649,15 @@ def adamw8_step(params, grads, states, steps, weight_decays, lr_tensor, betas=(0
     """adamw_step with states in 8 bits: `states` holds one AdamW8State (adamw8_state) per parameter, blocks of ADAMW8_BLOCK
     elements share a scale.  The update itself is computed in 32 bits from the decoded states; they are coded again with stochastic
     rounding whose random bits come from (seed, step count, index in the list, element): the same call gives the same states."""
-    what = 'adamw8_step'
-    dev, live = _optimiser_lists(what, params, grads, steps, weight_decays, lr_tensor, betas, eps, clip, copies, (states,))
-    if not live:
+    _check_step('adamw8_step', params, lr_tensor, betas, eps, clip)
+    table, n = _native.host().adamw8_table('adamw8_step', params, grads, steps, weight_decays, copies, states)
+    if n == 0:
         return
-    index = params[0].get_device()
-    for p, (m, ms, r, rs) in zip(params, states):
-        n = p.numel()
-        blocks = -(-n // ADAMW8_BLOCK)
-        for codes, scale in ((m, ms), (r, rs)):
-            if codes.dtype not in (torch.uint8, torch.float8_e4m3fn) or scale.dtype is not torch.float32 or codes.numel() != n or \
-                    scale.numel() != blocks or not codes.is_contiguous() or not scale.is_contiguous() or \
-                    codes.get_device() != index or scale.get_device() != index:
-                raise RuntimeError('%s: the state of a %s parameter must be %d codes and %d float32 scales on its device (adamw8_state)'
-                                   % (what, tuple(p.shape), n, blocks))
-    rec = np.zeros(len(live), dtype=_ADAMW8)
-    _fill_common(rec, params, grads, steps, weight_decays, copies, live)
-    for k, name in enumerate(('m_codes', 'm_scales', 'r_codes', 'r_scales')):
-        rec[name] = [states[i][k].data_ptr() for i in live]
-    L = _native.lib()
+    L, dev = _native.lib(), params[0].device
     with _device_guard(dev):
-        ws = torch.empty(L.semseg_adamw_workspace_bytes(len(live)), device=dev, dtype=torch.uint8)
-        _native.check(L.semseg_adamw8_step(vp(rec.ctypes.data), len(live), _p(lr_tensor), betas[0], betas[1], eps, float(grad_scale),
-                                           _p(clip), int(seed) & 0xFFFFFFFF, _p(ws), ws.numel(), _st()), what)
+        ws = torch.empty(L.semseg_adamw_workspace_bytes(n), device=dev, dtype=torch.uint8)
+        _native.check(L.semseg_adamw8_step(table, n, _p(lr_tensor), betas[0], betas[1], eps, grad_scale, _p(clip), int(seed) & 0xFFFFFFFF,
+                                           _p(ws), ws.numel(), _st()), 'adamw8_step')
     _weights_changed(params)
 
 
@@ -2728,24 +2670,11 @@ def grad_norm(grads, max_norm=None, grad_scale=1.0):
     if not grads:
         raise ValueError('grad_norm: no gradients')
     _require_cuda(grads[0])
-    dev = grads[0].device
-    for g in grads:
-        if g.dtype not in _TYPE_CODES:
-            raise TypeError('grad_norm: gradients must be float32, bfloat16 or float16, got %s' % g.dtype)
-        if g.get_device() != grads[0].get_device():
-            raise ValueError('grad_norm: all gradients must be on one HIP device')
-        if not _is_dense(g):
-            raise RuntimeError('grad_norm: a %s gradient is not dense (strides %s)' % (tuple(g.shape), g.stride()))
-    live = [g for g in grads if g.numel()]
-    rec = np.zeros(len(live), dtype=_GRADS)
-    rec['grad'] = [g.data_ptr() for g in live]
-    rec['numel'] = [g.numel() for g in live]
-    rec['grad_type'] = [_TYPE_CODES[g.dtype] for g in live]
-    L = _native.lib()
-    table = vp(rec.ctypes.data)
+    table, n = _native.host().grad_table(grads)
+    L, dev = _native.lib(), grads[0].device
     with _device_guard(dev):
         out = torch.empty(2, device=dev, dtype=torch.float32)
-        ws = torch.empty(L.semseg_grad_norm_workspace_bytes(table, len(live)), device=dev, dtype=torch.uint8)
-        _native.check(L.semseg_grad_norm(table, len(live), float(grad_scale), -1.0 if max_norm is None else float(max_norm), _p(out),
-                                         _p(ws), ws.numel(), _st()), 'grad_norm')
+        ws = torch.empty(L.semseg_grad_norm_workspace_bytes(table, n), device=dev, dtype=torch.uint8)
+        _native.check(L.semseg_grad_norm(table, n, grad_scale, -1.0 if max_norm is None else max_norm, _p(out), _p(ws), ws.numel(),
+                                         _st()), 'grad_norm')
     return out

@@ -1,6 +1,6 @@
 // TEST INFRASTRUCTURE: host build of the per-element code of csrc/adamw.hip (adamw_math.h) behind the same C ABI, with the same blocks
-// of the 8-bit states, so that the AdamW steps and the Python entry points above them can be checked against float64 without a GPU, and
-// the GPU's results bit for bit against these (tests/test_finetune_cpu.py, tests/test_gpu_finetune.py).  Never shipped.
+// of the 8-bit states, so that the AdamW steps and the Python entry points above them can be checked against float64 without a GPU
+// (tests/test_finetune_cpu.py; the GPU's results are held to the same bounds, tests/test_gpu_finetune.py).  Never shipped.
 #include <stddef.h>
 #include "semseg_hip.h"
 #include "adamw_math.h"
@@ -113,8 +113,8 @@ extern "C" int semseg_adamw8_step(const semseg_adamw8_tensor* t, int n, const fl
             const float im = adam8_inverse(ms), ir = adam8_inverse(rs);
             for (int64_t j = s; j < end; ++j) {
                 const uint32_t bits = adam_mix((uint32_t)j + c.base);
-                mc[j] = encode(copysignf(adam8_round(m[j - s], im, bits & 0xffffu, false), m[j - s]));
-                rc[j] = encode(adam8_round(r[j - s], ir, bits >> 16, true));
+                mc[j] = encode(adam8_round(adam8_scaled_m(m[j - s], im), bits & 0xffffu));
+                rc[j] = encode(adam8_round(adam8_scaled_r(r[j - s], ir), bits >> 16));
             }
         }
     }

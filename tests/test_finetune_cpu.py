@@ -273,30 +273,55 @@ def mix(x):
     return x ^ (x >> 16)
 
 
-def check_codes(x, codes, scales, random16, positive):
-    """codes and scales against the definition applied to the exact states `x` (float64): the scale within 4 roundings, a code equal to
-    the stochastic rounding unless the value is within its own error of the border"""
+def check_codes(x, err, codes, scales, random16, positive):
+    """codes and scales against the definition applied to the exact states `x` (float64), of which the float32 ones are off by `err`: a
+    scale is its largest value's error and 2 roundings off, a code equals the stochastic rounding unless the value is within its error
+    (its own, and 8 roundings of scale, reciprocal and product) of a border"""
     n = x.numel()
     pad = torch.nn.functional.pad(x, (0, -n % 256)).view(-1, 256)
     top = pad.abs().amax(1)
     want = torch.where(top < 2.0 ** -100, torch.zeros_like(top), top / 448)
-    assert torch.all((scales.double() - want).abs() <= 12 * U32 * want)
+    off = torch.nn.functional.pad(err, (0, -n % 256)).view(-1, 256).amax(1) / 448 + 2 * U32 * want
+    assert torch.all((scales.double() - want).abs() <= off)
     s = want.repeat_interleave(256)[:n]
     live = s > 0
-    a = torch.where(live, x.abs() / torch.where(live, s, torch.ones_like(s)), torch.zeros_like(s)).clamp(max=448)
+    safe = torch.where(live, s, torch.ones_like(s))
+    a = torch.where(live, x.abs() / safe, torch.zeros_like(s)).clamp(max=448)
+    if positive:
+        a = torch.where((x > 0) & live, a.clamp(min=2.0 ** -9), a)
     q = spacing(a)
     exact = a / q + random16.double() / 65536
-    got = codes.view(torch.float8_e4m3fn).double()
     low = torch.floor(exact) * q
-    if positive:
-        low = torch.where((x > 0) & (low == 0) & live, torch.full_like(low, 2.0 ** -9), low)
-    differ = got.abs() != torch.where(live, low, torch.zeros_like(low))
-    # a border is an integer of `exact`, or a power of two where the spacing changes; errors of the value: 16 roundings of up to 448 / 2^-9
-    near = (exact - exact.round()).abs() < 40 * U32 * (a / q + 1)
+    got = codes.view(torch.float8_e4m3fn).double()
+    differ = (got.abs() != low) & live
+    border = (err / safe + a * (8 * U32 + off.repeat_interleave(256)[:n] / safe)) / q + 2.0 ** -20
+    near = (exact - exact.round()).abs() <= border
     assert not torch.any(differ & ~near)
     assert torch.all((got.abs() - low).abs()[differ] <= q[differ] * 1.001)
-    nonzero = got != 0
+    nonzero = (got != 0) & live
     assert torch.equal(torch.sign(got)[nonzero], torch.sign(x)[nonzero])
+
+
+def check_step8(p0, g, m0, r0, p, state, t, lr, wd, betas, eps, seed, ordinal, factor=1.0):
+    """one 8-bit step from the decoded states m0, r0 (float64).  m, r^2: as check_step, each with one rounding more (the decoding), a
+    product of codes and scales; root and reciprocal are up to one unit (2 roundings) off."""
+    n = p.numel()
+    flat = [x.reshape(-1) if x.is_contiguous() else x.as_strided((n,), (1,)) for x in (p0, g, p)]
+    p0, g, p = flat
+    rp, rm, rv, move = reference_step(p0, g, m0, r0 * r0, t, lr, wd, betas, eps, factor)
+    terms = betas[0] * m0.abs() + (1 - betas[0]) * (g.double() * factor).abs()
+    spread = terms / (1 - betas[0] ** t) * lr / ((rv / (1 - betas[1] ** t)).sqrt() + eps)
+    assert torch.all((p.double() - rp).abs() <= U32 * rp.abs() + 20 * U32 * (spread + lr * wd * p0.double().abs()) + 2.0 ** -148)
+    bits = mix((torch.arange(n) + mix(seed ^ mix(t ^ mix(ordinal)))) & 0xFFFFFFFF)
+    check_codes(rm, 6 * U32 * terms, state[0], state[1], bits & 0xFFFF, False)
+    r = rv.sqrt()
+    check_codes(r, 7 * U32 * r + 1.1e-19, state[2], state[3], bits >> 16, True)
+
+
+def decoded(state):
+    """(m, r) of a state in float64"""
+    n = state[0].numel()
+    return [c.view(torch.float8_e4m3fn).double() * s.double().repeat_interleave(256)[:n] for c, s in ((state[0], state[1]), (state[2], state[3]))]
 
 
 @pytest.mark.parametrize('n', [1, 3, 255, 256, 257, 1000, 4099])
@@ -309,25 +334,17 @@ def test_adamw8_arithmetic(emulated, n, grad):
     step, lr, betas, eps, wd, seed = torch.zeros(1, dtype=torch.int32), torch.tensor([1e-2]), (0.9, 0.999), 1e-8, 0.01, 77
     for t in range(1, 5):
         g = (torch.randn(n, generator=gen) * 10 ** (torch.rand(n, generator=gen) * 3 - 3)).to(grad)
-        m0, v0 = ops.adamw8_values(state, p)
-        m0 = state.m.double() * state.m_scale.double().repeat_interleave(256)[:n]
-        r0 = state.r.double() * state.r_scale.double().repeat_interleave(256)[:n]
+        m0, r0 = decoded(state)
         p0 = p.clone()
         copy = torch.empty(n, dtype=torch.bfloat16)
         ops.adamw8_step([p], [g], [state], [step], [wd], lr, betas, eps, copies=[copy], seed=seed)
         assert int(step) == t
-        rp, rm, rv, move = reference_step(p0, g, m0, r0 * r0, t, float(lr), wd, betas, eps)
-        spread = (betas[0] * m0.abs() + 0.1 * g.double().abs()) / (1 - betas[0] ** t) * float(lr) / ((rv / (1 - betas[1] ** t)).sqrt() + eps)
-        assert torch.all((p.double() - rp).abs() <= U32 * rp.abs() + 18 * U32 * (spread + float(lr) * wd * p0.double().abs()))
         assert torch.equal(copy, p.bfloat16())
-        bits = mix((torch.arange(n) + mix(seed ^ mix(t ^ mix(0)))) & 0xFFFFFFFF)
-        check_codes(rm, state.m, state.m_scale, bits & 0xFFFF, False)
-        check_codes(rv.sqrt(), state.r, state.r_scale, bits >> 16, True)
+        check_step8(p0, g, m0, r0, p, state, t, float(lr), wd, betas, eps, seed, 0)
         m1, v1 = ops.adamw8_values(state, p)
-        # a code is within one spacing (1/8 of the value, or 2^-9 of the largest / 448) of what it stands for
-        top = torch.nn.functional.pad(rm.abs(), (0, -n % 256)).view(-1, 256).amax(1).repeat_interleave(256)[:n]
-        assert torch.all((m1.double() - rm).abs() <= (rm.abs() / 8).clamp(min=2.0 ** -9 / 448) + top * 2.0 ** -9 / 448 * 1.001)
-        assert torch.all(v1 >= 0) and torch.all(v1[rv > 0] > 0)
+        m, r = decoded(state)
+        assert torch.all((m1.double() - m).abs() <= 2 * U32 * m.abs()) and torch.all((v1.double() - r * r).abs() <= 6 * U32 * r * r)
+        assert torch.all(v1 >= 0) and torch.all(v1[g != 0] > 0)
 
 
 def test_adamw8_rounding_is_right_on_average(emulated):
