@@ -18,6 +18,7 @@ _C = CN({
               'fc_dim': 2048},
     'TRAIN': {
         'batch_size_per_gpu': 2, 'num_epoch': 20, 'start_epoch': 0, 'epoch_iters': 5000, 'optim': 'SGD',
+        'beta2': 0.999, 'eps': 1e-8, 'clip_grad_norm': 0.0,      # optim AdamW, AdamW8bit; 0: gradients are not clipped
         'lr_encoder': 0.02, 'lr_decoder': 0.02, 'lr_pow': 0.9, 'beta1': 0.9, 'weight_decay': 1e-4, 'deep_sup_scale': 0.4,
         'fix_bn': False, 'workers': 16, 'disp_iter': 20, 'seed': 304,
     },

@@ -165,7 +165,8 @@ def train_worker(rank, world, cfg, gpus, port):
         print('1 Epoch = {} iters'.format(cfg.TRAIN.epoch_iters))
     max_iters = cfg.TRAIN.epoch_iters * cfg.TRAIN.num_epoch
     step = TrainStep(sm, lr_encoder=cfg.TRAIN.lr_encoder, lr_decoder=cfg.TRAIN.lr_decoder, momentum=cfg.TRAIN.beta1,
-                     weight_decay=cfg.TRAIN.weight_decay, lr_pow=cfg.TRAIN.lr_pow, max_iters=max_iters, graph=True)
+                     weight_decay=cfg.TRAIN.weight_decay, lr_pow=cfg.TRAIN.lr_pow, max_iters=max_iters, graph=True, optim=cfg.TRAIN.optim,
+                     beta2=cfg.TRAIN.beta2, eps=cfg.TRAIN.eps, clip_grad_norm=cfg.TRAIN.clip_grad_norm or None)
     step.iter = cfg.TRAIN.start_epoch * cfg.TRAIN.epoch_iters          # cur_iter of train.py:35
     history = {'train': {'epoch': [], 'loss': [], 'acc': []}}
     for epoch in range(cfg.TRAIN.start_epoch, cfg.TRAIN.num_epoch):

@@ -74,6 +74,72 @@ class FusedSGD:
         self.steps += 1
 
 
+class FusedAdamW:
+    """AdamW (decoupled weight decay) for groups like FusedSGD's, one multi-tensor HIP kernel per group (csrc/adamw.hip), with its
+    states in 32 bits or, `bits=8`, in blocks of 8-bit codes (parameters of fewer than `min_8bit` elements -- biases, BN affine -- keep
+    32 bits: they are a thousandth of the memory and the noisiest to code).  `max_norm`: the gradients of all groups are scaled to at
+    most this global norm, and a step whose gradients are not finite changes nothing (`float('inf')`: only that).
+
+    lr, step counts and the clip factor are device memory, the states exist from the start: a captured step can be replayed.  A
+    parameter without a gradient is left alone, its step count too.  `clip` is the [norm, factor] of the last step
+    (of a captured step: until the next one)."""
+
+    def __init__(self, groups, betas=(0.9, 0.999), eps=1e-8, bits=32, max_norm=None, min_8bit=4096, seed=0):
+        """groups: list of dict(params=[...], lr=float, weight_decay=float)."""
+        if bits not in (8, 32):
+            raise ValueError('AdamW states have 8 or 32 bits, not %r' % (bits,))
+        if max_norm is not None and not max_norm >= 0.0:
+            raise ValueError('max_norm must not be negative, got %r' % (max_norm,))
+        self.groups, self.betas, self.eps, self.max_norm, self.seed = groups, betas, eps, max_norm, seed
+        self.state = {}                               # parameter -> (its step count, its state: two tensors or an ops.AdamW8State)
+        self.steps = 0
+        self.clip = None
+        for g in groups:
+            dev = g['params'][0].device
+            g['lr_t'] = torch.full((1,), float(g['lr']), device=dev, dtype=torch.float32)
+            counts = torch.zeros(len(g['params']), device=dev, dtype=torch.int32).unbind()
+            for p, count in zip(g['params'], counts):
+                if bits == 8 and p.numel() >= min_8bit:
+                    self.state[p] = (count, ops.adamw8_state(p))
+                else:
+                    self.state[p] = (count, (torch.zeros_like(p), torch.zeros_like(p)))
+
+    set_lr = FusedSGD.set_lr
+    zero_grad = FusedSGD.zero_grad
+
+    def step(self, grad_scale=1.0):
+        live = [[p for p in g['params'] if p.grad is not None] for g in self.groups]
+        grads = [p.grad for ps in live for p in ps]
+        self.clip = ops.grad_norm(grads, self.max_norm, grad_scale) if self.max_norm is not None and grads else None
+        for i, (g, ps) in enumerate(zip(self.groups, live)):
+            wide = [p for p in ps if not isinstance(self.state[p][1], ops.AdamW8State)]
+            coded = [p for p in ps if isinstance(self.state[p][1], ops.AdamW8State)]
+            if wide:
+                st = [self.state[p] for p in wide]
+                ops.adamw_step(wide, [p.grad for p in wide], [s[1][0] for s in st], [s[1][1] for s in st], [s[0] for s in st],
+                               [g['weight_decay']] * len(wide), g['lr_t'], self.betas, self.eps, grad_scale, self.clip)
+            if coded:
+                st = [self.state[p] for p in coded]
+                ops.adamw8_step(coded, [p.grad for p in coded], [s[1] for s in st], [s[0] for s in st], [g['weight_decay']] * len(coded),
+                                g['lr_t'], self.betas, self.eps, grad_scale, self.clip, seed=self.seed + i)
+        self.steps += 1
+
+
+OPTIMISERS = ('sgd', 'adamw', 'adamw8bit')          # TRAIN.optim, whatever the case
+
+
+def build_optimiser(name, groups, momentum=0.9, beta2=0.999, eps=1e-8, clip_grad_norm=None):
+    """the optimiser of TRAIN.optim: 'SGD' (train.py:115-127), 'AdamW' or 'AdamW8bit' (momentum is AdamW's beta1)"""
+    key = str(name).lower()
+    if key not in OPTIMISERS:
+        raise ValueError('TRAIN.optim must be SGD, AdamW or AdamW8bit, got %r' % (name,))
+    if key == 'sgd':
+        if clip_grad_norm is not None:
+            raise ValueError('clip_grad_norm goes with AdamW: the SGD step of the reference (train.py:115-127) has no clipping')
+        return FusedSGD(groups, momentum)
+    return FusedAdamW(groups, (momentum, beta2), eps, 8 if key == 'adamw8bit' else 32, clip_grad_norm)
+
+
 class SegmentedStep:
     """The data-parallel training step as a CHAIN of hipGraphs with the collectives between them.
 
@@ -204,7 +270,9 @@ class TrainStep:
     (a few MB), against 288 GB of HBM."""
 
     def __init__(self, segmentation_module, lr_encoder=0.02, lr_decoder=0.02, momentum=0.9, weight_decay=1e-4,
-                 lr_pow=0.9, max_iters=100000, graph=False, group=None, bucket_bytes=64 << 20, max_graphs=None):
+                 lr_pow=0.9, max_iters=100000, graph=False, group=None, bucket_bytes=64 << 20, max_graphs=None, optim='SGD', beta2=0.999,
+                 eps=1e-8, clip_grad_norm=None):
+        """optim: 'SGD', 'AdamW' or 'AdamW8bit'; momentum is AdamW's beta1; clip_grad_norm (AdamW): bound on the global gradient norm"""
         self.sm = segmentation_module
         enc, dec = segmentation_module.encoder, segmentation_module.decoder
         groups = []
@@ -212,7 +280,7 @@ class TrainStep:
             decay, no_decay = group_weight(net)
             groups.append(dict(params=decay, lr=lr, weight_decay=weight_decay, base_lr=lr))
             groups.append(dict(params=no_decay, lr=lr, weight_decay=0.0, base_lr=lr))
-        self.opt = FusedSGD(groups, momentum)
+        self.opt = build_optimiser(optim, groups, momentum, beta2, eps, clip_grad_norm)
         self.lr_pow, self.max_iters = lr_pow, max_iters
         self.iter = 0
         self.group = group
@@ -290,7 +358,7 @@ class TrainStep:
         # backward on a single rank, one per gradient bucket (from the hook that completes it, before its all-reduce) on a rank of
         # a data-parallel job (ops.defer_wgrad_reduces)
         with ops.defer_wgrad_reduces(flush_at_buckets=self.buckets is not None and self.buckets.flushes_deferred,
-                                     into_sgd=self.buckets is None), \
+                                     into_sgd=self.buckets is None and isinstance(self.opt, FusedSGD)), \
                 ops.defer_fork_sums():        # ... and the gradient sums at the forks are formed by the BN kernels that consume them
             loss.backward()
         if tl is not None:

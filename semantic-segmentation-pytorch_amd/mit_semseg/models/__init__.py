@@ -1,1 +1,1 @@
-from .models import ModelBuilder, SegmentationModule
+from .models import ModelBuilder, PolicyLoss, SegmentationModule

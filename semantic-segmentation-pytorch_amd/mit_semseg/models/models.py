@@ -25,8 +25,27 @@ class SegmentationModuleBase(nn.Module):
         return acc
 
 
+class PolicyLoss(nn.Module):
+    """Criterion of SegmentationModule for tuning a trained network on a reward (a metric of whole label maps, say) instead of labels:
+    the label map is one that was sampled from the network, `advantage` what it earned (per image or per pixel), and the loss is the
+    clipped policy loss with a KL term of ops.policy_loss.  forward(scores, label, advantage, old_logp, ref_logp) -> loss; `kl` and
+    `clipped` hold the mean KL term and the share of clipped pixels of the last forward."""
+
+    def __init__(self, clip_low=0.2, clip_high=0.2, kl_weight=0.0, ignore_index=-1):
+        super(PolicyLoss, self).__init__()
+        self.clip_low, self.clip_high, self.kl_weight, self.ignore_index = clip_low, clip_high, kl_weight, ignore_index
+        self.kl = self.clipped = None
+
+    def forward(self, scores, label, advantage, old_logp, ref_logp=None):
+        loss, self.kl, self.clipped = ops.policy_loss(scores, label, advantage, old_logp, ref_logp, self.clip_low, self.clip_high,
+                                                      self.kl_weight, self.ignore_index)
+        return loss
+
+
 class SegmentationModule(SegmentationModuleBase):
-    """models.py:21-47.  forward(feed_dict) -> (loss, acc); forward(feed_dict, segSize=(H,W)) -> softmax probs."""
+    """models.py:21-47.  forward(feed_dict) -> (loss, acc); forward(feed_dict, segSize=(H,W)) -> softmax probs.
+    With a PolicyLoss as criterion the feed carries 'advantage', 'old_logp' and (for its KL term) 'ref_logp' beside the sampled
+    'seg_label'; label_log_prob gives both kinds of log probabilities."""
 
     def __init__(self, net_enc, net_dec, crit, deep_sup_scale=None):
         super(SegmentationModule, self).__init__()
@@ -47,6 +66,16 @@ class SegmentationModule(SegmentationModuleBase):
         loss = crit(pred, label)
         return loss, (self.pixel_acc(pred, label) if want_acc else None)
 
+    def _main_scores(self, feats):
+        pred = self.decoder(feats)
+        return pred[0] if isinstance(pred, tuple) else pred
+
+    def label_log_prob(self, feed_dict):
+        """[N, H, W] log probability of every pixel of feed_dict['seg_label'] under the network (its scores are at the labels' size);
+        pixels that the criterion ignores give 0"""
+        feats = self.encoder(feed_dict['img_data'], return_feature_maps=True)
+        return ops.label_log_prob(self._main_scores(feats), feed_dict['seg_label'], getattr(self.crit, 'ignore_index', -1))
+
     def forward(self, feed_dict, *, segSize=None):
         if isinstance(feed_dict, (list, tuple)):      # UserScatteredDataParallel passes a 1-element list per GPU
             feed_dict = feed_dict[0]
@@ -54,6 +83,10 @@ class SegmentationModule(SegmentationModuleBase):
         if segSize is not None:                       # inference
             return self.decoder(feats, segSize=segSize)
         label = feed_dict['seg_label']
+        if isinstance(self.crit, PolicyLoss):         # the label map was drawn from the main head: an auxiliary one takes no part
+            pred = self._main_scores(feats)
+            loss = self.crit(pred, label, feed_dict['advantage'], feed_dict['old_logp'], feed_dict.get('ref_logp'))
+            return loss, self.pixel_acc(pred.detach(), label)
         if self.deep_sup_scale is not None:           # deep supervision
             pred, pred_deepsup = self.decoder(feats)
         else:

@@ -2594,6 +2594,7 @@ def _weights_changed(params):
     if not _WPLANES:
         return
     for p in params:
+        _ABSMAX_FRESH.pop(id(p), None)
         rec = _WPLANES.get(id(p))
         if rec is not None:
             _WPLANES[id(p)] = (rec[0], -1, rec[2], rec[3], rec[4], rec[5], rec[6])
