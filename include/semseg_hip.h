@@ -636,7 +636,11 @@ size_t semseg_policy_loss_workspace_bytes(void);
 int semseg_policy_loss_fwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, int64_t P, int C,
                            const float* advantage, int64_t rows_per_advantage, const float* old_logp, const float* ref_logp,
                            float clip_low, float clip_high, float kl_weight, float* stats, float* coef, float* loss, float* kl, float* clipped,
-                           float* inv_count, void* workspace, size_t workspace_bytes, void* stream);
+                           float* inv_count, void* dz, void* workspace, size_t workspace_bytes, void* stream);
+/* dz (may be NULL): the gradient of the logits for an upstream gradient of 1, written by the forward call where policy_loss_one_pass says
+ * so (dense float32 rows of few classes, enough of them); scale_by multiplies n floats (16-byte aligned) by a device scalar. */
+int semseg_policy_loss_one_pass(const void* z, int type, int64_t ld, int64_t P, int C);
+int semseg_scale_by(float* x, int64_t n, const float* g, void* stream);
 int semseg_label_logp_bwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, const float* stats,
                           const float* g, const float* gloss, const float* inv_count, int64_t P, int C, void* dz, void* stream);
 

@@ -2,10 +2,12 @@
 // gradients (gfx950).  The framework's other optimiser is sgd_fused_kernel (head.hip).
 //
 // Bound: HBM.  A step with f32 gradients moves 28 bytes an element with states in 32 bits (p, m, v both ways, g once) and 16 with
-// states in 8 bits; the norm moves the gradients once.  Layout of the work: every tensor is cut into chunks, a launch is the chunks of
-// up to ADAM_MAX_TENSORS tensors one after the other, and a block finds its tensor by a binary search in the kernel arguments, so no
-// block is launched for nothing and no tensor needs a launch of its own.  The step count, the learning rate and the clip factor are
-// device memory: a captured graph can be replayed.
+// states in 8 bits; the norm moves the gradients once.  Layout of the work: every tensor is cut into chunks, a launch is the chunks of all
+// tensors one after the other, and a block finds its tensor by comparing its number with the tensors' first chunks, 64 at a time, so no
+// block is launched for nothing and no tensor needs a launch of its own.  The table of tensors of an AdamW step lies in the workspace: a
+// small kernel before the step, which advances the step counts and forms the coefficients, copies it there from its arguments (a launch
+// of the step per 48 tensors, with the table in its arguments, took 10 % longer for 168 tensors).  Step counts, learning rate and clip
+// factor are device memory: a captured graph can be replayed.
 #include "common.h"
 #include "adamw_math.h"
 
@@ -14,7 +16,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int ADAM_MAX_TENSORS = 48;
+constexpr int ADAM_MAX_TENSORS = 1024;     // of one launch of a step
 constexpr int ADAM_CHUNK = 4096;           // elements of a block: 4 quads a thread, all their loads in flight at once
 constexpr int ADAM_QUADS = ADAM_CHUNK / (256 * 4);
 
@@ -43,65 +45,81 @@ __device__ __forceinline__ void store_one(void* c, int type, int64_t i, float v)
     else reinterpret_cast<_Float16*>(c)[i] = (_Float16)v;
 }
 
-// the tensor whose chunks hold block `b`: the last one whose first chunk is not behind it
-template <class B>
-__device__ __forceinline__ int tensor_of(const B& batch, uint32_t b) {
-    int lo = 0, hi = batch.n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (batch.first[mid] <= b) lo = mid; else hi = mid - 1;
-    }
-    return lo;
+// the tensor whose chunks hold block `b`: as many first chunks are not behind it, less one.  One comparison a lane.
+__device__ __forceinline__ int tensor_of(const uint32_t* first, int n, uint32_t b) {
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+    for (int base = 0; base < n; base += 64) count += __popcll(__ballot(base + lane < n && first[min(base + lane, n - 1)] <= b));
+    return __builtin_amdgcn_readfirstlane(count) - 1;
 }
 
-// ---------------------------------------------------------------- step counts and coefficients --------------------------------
-constexpr int BEGIN_MAX = 240;
-struct BeginBatch {
-    int* step[BEGIN_MAX];
-    float wd[BEGIN_MAX];
-    int n, base;
+// ---------------------------------------------------------------- step counts, coefficients, table ----------------------------
+struct AdamEntry {                  // one tensor, states in 32 bits
+    float* p; const void* g; void* c; float* m; float* v;
+    int64_t numel;
+    AdamCoef coef;
+    uint8_t gtype, ctype, vec, pad;
 };
-static_assert(sizeof(BeginBatch) <= 4000, "kernel arguments");
+struct Adam8Entry {                 // one tensor, states in 8 bits
+    float* p; const void* g; void* c; uint8_t* m; float* ms; uint8_t* r; float* rs;
+    int64_t numel;
+    AdamCoef coef;
+    uint8_t gtype, ctype, vec, pad;
+};
+// what the small kernel gets of a tensor in its arguments
+struct AdamItem {
+    float* p; const void* g; void* c; float* m; float* v; int* step;
+    int64_t numel;
+    float wd;
+    uint32_t first;
+    uint8_t gtype, ctype, vec, pad;
+};
+struct Adam8Item {
+    float* p; const void* g; void* c; uint8_t* m; float* ms; uint8_t* r; float* rs; int* step;
+    int64_t numel;
+    float wd;
+    uint32_t first;
+    uint8_t gtype, ctype, vec, pad;
+};
+__device__ __forceinline__ void put_states(AdamEntry& e, const AdamItem& i) { e.m = i.m; e.v = i.v; }
+__device__ __forceinline__ void put_states(Adam8Entry& e, const Adam8Item& i) { e.m = i.m; e.ms = i.ms; e.r = i.r; e.rs = i.rs; }
 
-__global__ __launch_bounds__(256) void adamw_begin_kernel(const BeginBatch b, const float* __restrict__ lr, double log_b1, double log_b2,
-                                                          float grad_scale, const float* __restrict__ clip, uint32_t seed,
-                                                          AdamCoef* __restrict__ coef) {
-    const int i = threadIdx.x;
-    if (i >= b.n) return;
-    float factor = grad_scale;
+template <class ITEM>
+struct BeginBatch {
+    static constexpr int MAX = 3800 / (int)sizeof(ITEM);
+    ITEM item[MAX];
+    int n, base;                    // tensors of this batch, and the index of the first one in the call
+};
+struct BeginArgs {
+    const float* lr; const float* clip;
+    double log_b1, log_b2;
+    float grad_scale;
+    uint32_t seed;
+};
+
+template <class ITEM, class ENTRY>
+__global__ __launch_bounds__(64) void adamw_begin_kernel(const BeginBatch<ITEM> b, const BeginArgs a, ENTRY* __restrict__ table,
+                                                         uint32_t* __restrict__ first) {
+    const int k = threadIdx.x;
+    if (k >= b.n) return;
+    const ITEM i = b.item[k];
+    int t = *i.step;
+    float factor = a.grad_scale;
     bool skip = false;
-    if (clip) {                                              // [norm, factor] of semseg_grad_norm
-        skip = !(fabsf(clip[0]) <= 3.402823466e38f);
-        factor *= clip[1];
+    if (a.clip) {                                            // [norm, factor] of semseg_grad_norm
+        skip = !(fabsf(a.clip[0]) <= 3.402823466e38f);
+        factor *= a.clip[1];
     }
-    int t = *b.step[i];
-    if (!skip) {
-        t += 1;
-        *b.step[i] = t;
-    }
-    AdamCoef c = adam_coef((double)lr[0], log_b1, log_b2, (double)b.wd[i], t, factor, seed, (uint32_t)(b.base + i));
-    if (skip) c.root = 0.f;
-    coef[b.base + i] = c;
-}
-
-static size_t coef_bytes(int n) { return (size_t)n * sizeof(AdamCoef); }
-
-template <class TENSOR>
-static int begin_step(const TENSOR* t, int n, const float* lr, double beta1, double beta2, float grad_scale, const float* clip,
-                      uint32_t seed, AdamCoef* coef, hipStream_t st) {
-    const double l1 = log(beta1), l2 = log(beta2);           // beta 0: -infinity, 1 - 0^t = 1
-    for (int base = 0; base < n; base += BEGIN_MAX) {
-        BeginBatch b;
-        b.n = min(BEGIN_MAX, n - base);
-        b.base = base;
-        for (int i = 0; i < b.n; ++i) {
-            b.step[i] = t[base + i].step;
-            b.wd[i] = t[base + i].weight_decay;
-        }
-        hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(256), 0, st, b, lr, l1, l2, grad_scale, clip, seed, coef);
-        SEMSEG_LAUNCH_CHECK();
-    }
-    return 0;
+    if (!skip) *i.step = ++t;
+    ENTRY e;
+    e.p = i.p; e.g = i.g; e.c = i.c;
+    put_states(e, i);
+    e.numel = i.numel;
+    e.gtype = i.gtype; e.ctype = i.ctype; e.vec = i.vec; e.pad = 0;
+    e.coef = adam_coef((double)a.lr[0], a.log_b1, a.log_b2, (double)i.wd, t, factor, a.seed, (uint32_t)(b.base + k));
+    if (skip) e.coef.root = 0.f;
+    table[b.base + k] = e;
+    first[b.base + k] = i.first;
 }
 
 static bool hyper_ok(double beta1, double beta2, double eps) {
@@ -114,25 +132,13 @@ static AdamHyper hyper_of(double beta1, double beta2, double eps) {
 }
 
 // ---------------------------------------------------------------- states in 32 bits -------------------------------------------
-struct AdamEntry {
-    float* p; const void* g; float* m; float* v; void* c;
-    int64_t numel;
-    int index;                 // of its AdamCoef
-    uint8_t gtype, ctype, vec, pad;
-};
-struct AdamBatch {
-    AdamEntry t[ADAM_MAX_TENSORS];
-    uint32_t first[ADAM_MAX_TENSORS];
-    int n;
-};
-static_assert(sizeof(AdamBatch) <= 4000, "kernel arguments");
-
-__global__ __launch_bounds__(256) void adamw_kernel(const AdamBatch b, const AdamCoef* __restrict__ coef, AdamHyper h) {
-    const int k = tensor_of(b, blockIdx.x);
-    const AdamEntry t = b.t[k];
-    const AdamCoef c = coef[t.index];
+__global__ __launch_bounds__(256) void adamw_kernel(const AdamEntry* __restrict__ table, const uint32_t* __restrict__ first, int n,
+                                                    AdamHyper h) {
+    const int k = tensor_of(first, n, blockIdx.x);
+    const AdamEntry t = table[k];
+    const AdamCoef c = t.coef;
     if (c.root == 0.f) return;
-    const int64_t start = (int64_t)(blockIdx.x - b.first[k]) * ADAM_CHUNK;
+    const int64_t start = (int64_t)(blockIdx.x - first[k]) * ADAM_CHUNK;
     const int tid = threadIdx.x;
     if (t.vec && start + ADAM_CHUNK <= t.numel) {
         const int64_t q0 = (start >> 2) + tid;
@@ -218,68 +224,91 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamBatch b, const Ada
     }
 }
 
-extern "C" size_t semseg_adamw_workspace_bytes(int n) { return n > 0 ? coef_bytes(n) : 0; }
+static AdamItem item_of(const semseg_adamw_tensor& t) {
+    AdamItem i{};
+    i.p = (float*)t.param; i.g = t.grad; i.c = t.copy; i.m = (float*)t.exp_avg; i.v = (float*)t.exp_avg_sq; i.step = t.step;
+    i.vec = aligned16(t.param) && aligned16(t.exp_avg) && aligned16(t.exp_avg_sq);
+    return i;
+}
+static Adam8Item item_of(const semseg_adamw8_tensor& t) {
+    Adam8Item i{};
+    i.p = (float*)t.param; i.g = t.grad; i.c = t.copy; i.step = t.step;
+    i.m = (uint8_t*)t.m_codes; i.ms = (float*)t.m_scales; i.r = (uint8_t*)t.r_codes; i.rs = (float*)t.r_scales;
+    i.vec = aligned16(t.param) && aligned_to(t.m_codes, 4) && aligned_to(t.r_codes, 4);
+    return i;
+}
+static bool states_ok(const semseg_adamw_tensor& t) { return t.exp_avg && t.exp_avg_sq; }
+static bool states_ok(const semseg_adamw8_tensor& t) { return t.m_codes && t.m_scales && t.r_codes && t.r_scales; }
 
-extern "C" int semseg_adamw_step(const semseg_adamw_tensor* tensors_host, int n, const float* lr, double beta1, double beta2, double eps,
-                                 float grad_scale, const float* clip, void* workspace, size_t workspace_bytes, void* stream) {
-    if (n < 0 || (n && (!tensors_host || !lr)) || !hyper_ok(beta1, beta2, eps)) return SEMSEG_EINVAL;
+extern "C" size_t semseg_adamw_workspace_bytes(int n) {
+    static_assert(sizeof(Adam8Entry) >= sizeof(AdamEntry) && sizeof(Adam8Entry) % 8 == 0, "one size for both steps");
+    return n > 0 ? (size_t)n * (sizeof(Adam8Entry) + sizeof(uint32_t)) : 0;
+}
+
+// the steps' common host side: checks, the small kernel per batch of tensors, one launch of `kernel` per ADAM_MAX_TENSORS tensors
+template <class ITEM, class ENTRY, class TENSOR, class KERNEL>
+static int adam_step(const TENSOR* tensors, int n, const float* lr, double beta1, double beta2, double eps, float grad_scale, const float* clip,
+                     uint32_t seed, int chunk, KERNEL kernel, void* workspace, size_t workspace_bytes, hipStream_t st) {
+    typedef BeginBatch<ITEM> Batch;
+    static_assert(sizeof(Batch) + sizeof(BeginArgs) <= 4000 && Batch::MAX <= 64, "kernel arguments");
+    if (n < 0 || (n && (!tensors || !lr)) || !hyper_ok(beta1, beta2, eps)) return SEMSEG_EINVAL;
+    const int64_t most = (int64_t)1 << 30;                   // blocks of a launch
     for (int i = 0; i < n; ++i) {
-        const semseg_adamw_tensor& t = tensors_host[i];
-        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || !t.step || t.numel <= 0 || !type_ok(t.grad_type) ||
-            (t.copy && (!type_ok(t.copy_type) || t.copy_type == SEMSEG_TYPE_F32)))
+        const TENSOR& t = tensors[i];
+        if (!t.param || !t.grad || !states_ok(t) || !t.step || t.numel <= 0 || !type_ok(t.grad_type) ||
+            (t.copy && (!type_ok(t.copy_type) || t.copy_type == SEMSEG_TYPE_F32)) || (t.numel + chunk - 1) / chunk > most)
             return SEMSEG_EINVAL;
-        if ((t.numel + ADAM_CHUNK - 1) / ADAM_CHUNK > (int64_t)1 << 30) return SEMSEG_EINVAL;
     }
     if (n == 0) return 0;
-    if (!workspace || workspace_bytes < coef_bytes(n) || !aligned16(workspace)) return SEMSEG_EWORKSPACE;
-    hipStream_t st = (hipStream_t)stream;
-    AdamCoef* coef = (AdamCoef*)workspace;
-    if (int rc = begin_step(tensors_host, n, lr, beta1, beta2, grad_scale, clip, 0u, coef, st)) return rc;
+    if (!workspace || workspace_bytes < semseg_adamw_workspace_bytes(n) || !aligned16(workspace)) return SEMSEG_EWORKSPACE;
+    ENTRY* table = (ENTRY*)workspace;
+    uint32_t* first = (uint32_t*)((char*)workspace + (size_t)n * sizeof(ENTRY));
     const AdamHyper h = hyper_of(beta1, beta2, eps);
+    const BeginArgs a{lr, clip, log(beta1), log(beta2), grad_scale, seed};         // beta 0: -infinity, 1 - 0^t = 1
     for (int i = 0; i < n;) {
-        AdamBatch b;
-        b.n = 0;
+        const int start = i;
         uint32_t chunks = 0;
-        for (; i < n && b.n < ADAM_MAX_TENSORS; ++i) {
-            const semseg_adamw_tensor& t = tensors_host[i];
-            const int64_t c = (t.numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
-            if (chunks + c > (int64_t)1 << 30) break;       // (a launch of its own holds any tensor: checked above)
-            AdamEntry& e = b.t[b.n];
-            e.p = (float*)t.param; e.g = t.grad; e.m = (float*)t.exp_avg; e.v = (float*)t.exp_avg_sq; e.c = t.copy;
-            e.numel = t.numel;
-            e.index = i;
-            e.gtype = (uint8_t)t.grad_type; e.ctype = (uint8_t)t.copy_type;
-            e.vec = aligned16(t.param) && aligned16(t.exp_avg) && aligned16(t.exp_avg_sq) && aligned_to(t.grad, 4 * type_bytes(t.grad_type)) &&
-                    (!t.copy || aligned_to(t.copy, 8));
-            e.pad = 0;
-            b.first[b.n++] = chunks;
-            chunks += (uint32_t)c;
+        bool room = true;
+        while (room && i < n && i - start < ADAM_MAX_TENSORS) {
+            Batch b;
+            b.n = 0;
+            b.base = i;
+            for (; i < n && i - start < ADAM_MAX_TENSORS && b.n < Batch::MAX; ++i) {
+                const TENSOR& t = tensors[i];
+                const int64_t c = (t.numel + chunk - 1) / chunk;
+                room = chunks + c <= most;
+                if (!room) break;
+                ITEM e = item_of(t);
+                e.numel = t.numel;
+                e.wd = t.weight_decay;
+                e.first = chunks;
+                e.gtype = (uint8_t)t.grad_type; e.ctype = (uint8_t)t.copy_type;
+                e.vec = e.vec && aligned_to(t.grad, 4 * type_bytes(t.grad_type)) && (!t.copy || aligned_to(t.copy, 8));
+                b.item[b.n++] = e;
+                chunks += (uint32_t)c;
+            }
+            if (b.n == 0) break;
+            auto begin = adamw_begin_kernel<ITEM, ENTRY>;
+            hipLaunchKernelGGL(begin, dim3(1), dim3(64), 0, st, b, a, table, first);
+            SEMSEG_LAUNCH_CHECK();
         }
-        hipLaunchKernelGGL(adamw_kernel, dim3(chunks), dim3(256), 0, st, b, coef, h);
+        hipLaunchKernelGGL(kernel, dim3(chunks), dim3(256), 0, st, (const ENTRY*)(table + start), (const uint32_t*)(first + start), i - start, h);
         SEMSEG_LAUNCH_CHECK();
     }
     return 0;
 }
 
+extern "C" int semseg_adamw_step(const semseg_adamw_tensor* tensors_host, int n, const float* lr, double beta1, double beta2, double eps,
+                                 float grad_scale, const float* clip, void* workspace, size_t workspace_bytes, void* stream) {
+    return adam_step<AdamItem, AdamEntry>(tensors_host, n, lr, beta1, beta2, eps, grad_scale, clip, 0u, ADAM_CHUNK, adamw_kernel, workspace,
+                                          workspace_bytes, (hipStream_t)stream);
+}
+
 // ---------------------------------------------------------------- states in 8 bits --------------------------------------------
 // A wave owns a block of 256 elements (one scale): 4 elements a lane, the block's maxima of |m| and r by shuffles, so the states are
 // read and written once and never leave the registers in between.
-constexpr int ADAM8_MAX_TENSORS = 44;
 constexpr int ADAM8_PER_WAVE = 4;                                     // blocks of a wave, their loads in flight together
 constexpr int ADAM8_CHUNK = 4 * ADAM8_PER_WAVE * ADAM8_BLOCK;         // elements of a thread block
-
-struct Adam8Entry {
-    float* p; const void* g; void* c; uint8_t* m; float* ms; uint8_t* r; float* rs;
-    int64_t numel;
-    int index;
-    uint8_t gtype, ctype, vec, pad;
-};
-struct Adam8Batch {
-    Adam8Entry t[ADAM8_MAX_TENSORS];
-    uint32_t first[ADAM8_MAX_TENSORS];
-    int n;
-};
-static_assert(sizeof(Adam8Batch) <= 4000, "kernel arguments");
 
 // maximum over the wave, as a scalar.  Within a row of 16 lanes by lane permutations of the instruction itself, then across the rows:
 // 6 instructions and a read of lane 63 (shuffles through LDS take 18 and their waits).  All lanes must be active.
@@ -326,13 +355,14 @@ __device__ __forceinline__ void adam8_block(const float m[4], const float r[4], 
     rc = (uint32_t)wr;
 }
 
-__global__ __launch_bounds__(256) void adamw8_kernel(const Adam8Batch b, const AdamCoef* __restrict__ coef, AdamHyper h) {
-    const int k = tensor_of(b, blockIdx.x);
-    const Adam8Entry t = b.t[k];
-    const AdamCoef c = coef[t.index];
+__global__ __launch_bounds__(256) void adamw8_kernel(const Adam8Entry* __restrict__ table, const uint32_t* __restrict__ first, int n,
+                                                     AdamHyper h) {
+    const int k = tensor_of(first, n, blockIdx.x);
+    const Adam8Entry t = table[k];
+    const AdamCoef c = t.coef;
     if (c.root == 0.f) return;
     const int lane = threadIdx.x & 63;
-    const int64_t start = (int64_t)(blockIdx.x - b.first[k]) * ADAM8_CHUNK + (threadIdx.x >> 6) * (ADAM8_PER_WAVE * ADAM8_BLOCK);
+    const int64_t start = (int64_t)(blockIdx.x - first[k]) * ADAM8_CHUNK + (threadIdx.x >> 6) * (ADAM8_PER_WAVE * ADAM8_BLOCK);
     if (start >= t.numel) return;                            // the same for the whole wave, as everything about blocks here
     const int full = t.vec ? (int)min((t.numel - start) >> 8, (int64_t)ADAM8_PER_WAVE) : 0;
     if (full) {
@@ -424,58 +454,18 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Adam8Batch b, const A
 extern "C" int semseg_adamw8_step(const semseg_adamw8_tensor* tensors_host, int n, const float* lr, double beta1, double beta2, double eps,
                                   float grad_scale, const float* clip, uint32_t seed, void* workspace, size_t workspace_bytes,
                                   void* stream) {
-    if (n < 0 || (n && (!tensors_host || !lr)) || !hyper_ok(beta1, beta2, eps)) return SEMSEG_EINVAL;
-    for (int i = 0; i < n; ++i) {
-        const semseg_adamw8_tensor& t = tensors_host[i];
-        if (!t.param || !t.grad || !t.m_codes || !t.m_scales || !t.r_codes || !t.r_scales || !t.step || t.numel <= 0 ||
-            !type_ok(t.grad_type) || (t.copy && (!type_ok(t.copy_type) || t.copy_type == SEMSEG_TYPE_F32)))
-            return SEMSEG_EINVAL;
-        if ((t.numel + ADAM8_CHUNK - 1) / ADAM8_CHUNK > (int64_t)1 << 30) return SEMSEG_EINVAL;
-    }
-    if (n == 0) return 0;
-    if (!workspace || workspace_bytes < coef_bytes(n) || !aligned16(workspace)) return SEMSEG_EWORKSPACE;
-    hipStream_t st = (hipStream_t)stream;
-    AdamCoef* coef = (AdamCoef*)workspace;
-    if (int rc = begin_step(tensors_host, n, lr, beta1, beta2, grad_scale, clip, seed, coef, st)) return rc;
-    const AdamHyper h = hyper_of(beta1, beta2, eps);
-    for (int i = 0; i < n;) {
-        Adam8Batch b;
-        b.n = 0;
-        uint32_t chunks = 0;
-        for (; i < n && b.n < ADAM8_MAX_TENSORS; ++i) {
-            const semseg_adamw8_tensor& t = tensors_host[i];
-            const int64_t c = (t.numel + ADAM8_CHUNK - 1) / ADAM8_CHUNK;
-            if (chunks + c > (int64_t)1 << 30) break;
-            Adam8Entry& e = b.t[b.n];
-            e.p = (float*)t.param; e.g = t.grad; e.c = t.copy;
-            e.m = (uint8_t*)t.m_codes; e.ms = (float*)t.m_scales; e.r = (uint8_t*)t.r_codes; e.rs = (float*)t.r_scales;
-            e.numel = t.numel;
-            e.index = i;
-            e.gtype = (uint8_t)t.grad_type; e.ctype = (uint8_t)t.copy_type;
-            e.vec = aligned16(t.param) && aligned_to(t.m_codes, 4) && aligned_to(t.r_codes, 4) &&
-                    aligned_to(t.grad, 4 * type_bytes(t.grad_type)) && (!t.copy || aligned_to(t.copy, 8));
-            e.pad = 0;
-            b.first[b.n++] = chunks;
-            chunks += (uint32_t)c;
-        }
-        hipLaunchKernelGGL(adamw8_kernel, dim3(chunks), dim3(256), 0, st, b, coef, h);
-        SEMSEG_LAUNCH_CHECK();
-    }
-    return 0;
+    return adam_step<Adam8Item, Adam8Entry>(tensors_host, n, lr, beta1, beta2, eps, grad_scale, clip, seed, ADAM8_CHUNK, adamw8_kernel,
+                                            workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 // ---------------------------------------------------------------- global norm -------------------------------------------------
 // Squares are summed in 64 bits (an f32 square leaves the range at 2e19 and below 1e-23), one partial sum per chunk in a fixed order,
 // then one block sums the partials: the same bits every time.
-constexpr int NORM_MAX_TENSORS = 140;
+constexpr int NORM_MAX_TENSORS = 196;
 constexpr int NORM_CHUNK = 16384;
-struct NormEntry {
-    const void* g;
-    int64_t numel;
-    uint8_t type, vec, pad[6];
-};
 struct NormBatch {
-    NormEntry t[NORM_MAX_TENSORS];
+    const void* g[NORM_MAX_TENSORS];
+    uint64_t size[NORM_MAX_TENSORS];        // elements, type and alignment: numel * 8 + type * 2 + vec
     uint32_t first[NORM_MAX_TENSORS];
     int n;
 };
@@ -502,8 +492,9 @@ __device__ __forceinline__ void add_squares(double& s, u32x4 v, int type) {
 
 __global__ __launch_bounds__(256) void grad_norm_kernel(const NormBatch b, double* __restrict__ partial) {
     __shared__ double sum[4];
-    const int k = tensor_of(b, blockIdx.x);
-    const NormEntry t = b.t[k];
+    const int k = tensor_of(b.first, b.n, blockIdx.x);
+    const uint64_t size = b.size[k];
+    const struct { const void* g; int64_t numel; int type, vec; } t = {b.g[k], (int64_t)(size >> 3), (int)(size >> 1) & 3, (int)size & 1};
     const int64_t start = (int64_t)(blockIdx.x - b.first[k]) * NORM_CHUNK;
     const int64_t end = min(t.numel, start + NORM_CHUNK);
     double s = 0.0;
@@ -581,12 +572,8 @@ extern "C" int semseg_grad_norm(const semseg_grad_tensor* tensors_host, int n, f
             const semseg_grad_tensor& t = tensors_host[i];
             const int64_t c = norm_chunks(t.numel);
             if (chunks + c > (int64_t)1 << 30) break;
-            NormEntry& e = b.t[b.n];
-            e.g = t.grad;
-            e.numel = t.numel;
-            e.type = (uint8_t)t.grad_type;
-            e.vec = aligned16(t.grad);
-            for (int j = 0; j < 6; ++j) e.pad[j] = 0;
+            b.g[b.n] = t.grad;
+            b.size[b.n] = (uint64_t)t.numel << 3 | (uint64_t)t.grad_type << 1 | (aligned16(t.grad) ? 1u : 0u);
             b.first[b.n++] = chunks;
             chunks += (uint32_t)c;
         }

@@ -33,7 +33,6 @@ struct AdamCoef {
     float factor;      // what the gradient is multiplied with
     float decay;       // lr * weight decay
     uint32_t base;     // counter base of the random bits
-    uint32_t pad[3];
 };
 struct AdamHyper {
     float b1, c1, b2, c2, eps;      // c = 1 - b, formed in double
@@ -59,7 +58,6 @@ SEMSEG_HD AdamCoef adam_coef(double lr, double log_b1, double log_b2, double wd,
     c.factor = factor;
     c.decay = (float)(lr * wd);
     c.base = adam_mix(seed ^ adam_mix((uint32_t)t ^ adam_mix(ordinal)));
-    c.pad[0] = c.pad[1] = c.pad[2] = 0;
     return c;
 }
 

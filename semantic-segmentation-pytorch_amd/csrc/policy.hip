@@ -16,6 +16,7 @@
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 template <class T, int V>
 struct Vec {
@@ -115,8 +116,8 @@ __device__ __forceinline__ float lanes_max(float v) {
     for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
 }
-template <int L>
-__device__ __forceinline__ float lanes_sum(float v) {
+template <int L, class V>
+__device__ __forceinline__ V lanes_sum(V v) {
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
@@ -126,16 +127,16 @@ struct RowSums {
     double loss = 0.0, kl = 0.0;
     int clipped = 0, count = 0;
 };
-// one row's answer, by one lane
+// one row's answer, by one lane; returns d(loss * rows that count) / d lp
 template <bool POLICY>
-__device__ __forceinline__ void finish_row(int64_t row, float za, bool valid, float top, float logs, float* __restrict__ lp_out,
+__device__ __forceinline__ float finish_row(int64_t row, float za, bool valid, float top, float logs, float* __restrict__ lp_out,
                                            float2* __restrict__ stats, const PolicyArgs& pa, RowSums& acc) {
     const float lp = valid ? (za - top) - logs : 0.f;
     if (stats) stats[row] = make_float2(top, logs);
+    float coef = 0.f;
     if constexpr (!POLICY) {
         lp_out[row] = lp;
     } else {
-        float coef = 0.f;
         if (valid) {
             const float A = pa.advantage[pa.small_rows ? (int64_t)((uint32_t)row / (uint32_t)pa.rows_per_advantage) : row / pa.rows_per_advantage];
             const float ratio = expf(lp - pa.old_logp[row]);
@@ -158,6 +159,7 @@ __device__ __forceinline__ void finish_row(int64_t row, float za, bool valid, fl
         }
         pa.coef[row] = coef;
     }
+    return coef;
 }
 __device__ __forceinline__ void block_partial(const RowSums& acc, double* __restrict__ partial) {
     __shared__ double sum[4][4];
@@ -227,16 +229,30 @@ __global__ __launch_bounds__(256) void label_logp_kernel(const T* __restrict__ z
 // Dense rows of few classes: a block takes 256 / L rows, one stretch of memory, in 16-byte loads that no row's start or end interrupts,
 // through LDS; then L lanes read a row each.  A row alone is 300 to 600 bytes at 150 classes: loads of its own are 4 or 8 bytes wide.
 constexpr int TILE_BYTES = 20480;       // 8 blocks of a compute unit at once
-template <class T, int L, int W, bool POLICY>
+//
+// GRAD: the rows are in registers when the loss of a row is known, so their gradient for an upstream gradient of 1 is written at once,
+// through the same tile: the logits are read once and not again by a backward pass.  It needs 1 / (rows that count) beforehand
+// (count_rows_kernel, 8 bytes a row).
+constexpr int COUNT_BLOCKS = 256;
+template <class T, int L, int W, bool POLICY, bool GRAD>
 __global__ __launch_bounds__(256) void label_logp_tile_kernel(const T* __restrict__ z, const int64_t* __restrict__ label, int64_t ignore,
                                                               int64_t P, int C, float* __restrict__ lp_out, float2* __restrict__ stats,
-                                                              const PolicyArgs pa) {
+                                                              const PolicyArgs pa, const int* __restrict__ counts, T* __restrict__ dz) {
     constexpr int ROWS = 256 / L, PER = 16 / (int)sizeof(T);
     constexpr int HELD = TILE_BYTES / 256 / ((int)sizeof(T) * W);      // W: elements of a read from LDS (2 where C is even)
     __shared__ u32x4 tile[TILE_BYTES / 16];
     const int sub = threadIdx.x % L;
     const int64_t tiles = (P + ROWS - 1) / ROWS;
     RowSums acc;
+    float share = 0.f;                                                 // 1 / rows that count
+    if constexpr (GRAD) {
+        __shared__ int part[4];
+        const int s = lanes_sum<64>(counts[threadIdx.x]);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+        __syncthreads();
+        const int n = (part[0] + part[1]) + (part[2] + part[3]);
+        share = n > 0 ? 1.f / (float)n : 0.f;
+    }
     for (int64_t b = blockIdx.x; b < tiles; b += gridDim.x) {
         const int64_t row0 = b * ROWS, row = row0 + threadIdx.x / L;
         const int count = (int)min(P - row0, (int64_t)ROWS) * C;       // elements of this tile
@@ -278,12 +294,61 @@ __global__ __launch_bounds__(256) void label_logp_tile_kernel(const T* __restric
 #pragma unroll
         for (int k = 0; k < HELD; ++k)
 #pragma unroll
-            for (int j = 0; j < W; ++j) s += __expf(x[k][j] - top);
+            for (int j = 0; j < W; ++j) {
+                x[k][j] = __expf(x[k][j] - top);
+                s += x[k][j];
+            }
         s = lanes_sum<L>(s);
-        if (sub == 0 && live) finish_row<POLICY>(row, valid ? (float)tr[a] : 0.f, valid, top, logf(s), lp_out, stats, pa, acc);
+        float coef = 0.f;
+        if (sub == 0 && live) coef = finish_row<POLICY>(row, valid ? (float)tr[a] : 0.f, valid, top, logf(s), lp_out, stats, pa, acc);
+        if constexpr (GRAD) {
+            const float g = __shfl(coef, (threadIdx.x & 63) / L * L, 64) * share, over = 1.f / s;
+            T* tw = t + threadIdx.x / L * C;
+            if (live) {
+#pragma unroll
+                for (int k = 0; k < HELD; ++k) {
+                    const int c = (sub + k * L) * W;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) x[k][j] = valid ? g * ((c + j == (int)a ? 1.f : 0.f) - x[k][j] * over) : 0.f;
+                    if (c < C) store_vec<T, W>(tw + c, x[k]);
+                }
+            }
+            __syncthreads();
+            T* dst = dz + row0 * C;
+#pragma unroll
+            for (int u = 0; u < TILE_BYTES / 4096; ++u)
+                if ((int)threadIdx.x + u * 256 < vecs) reinterpret_cast<u32x4*>(dst)[threadIdx.x + u * 256] = tile[threadIdx.x + u * 256];
+            for (int i = vecs * PER + threadIdx.x; i < count; i += 256) dst[i] = t[i];
+        }
         __syncthreads();
     }
     if constexpr (POLICY) block_partial(acc, pa.partial);
+}
+
+// rows that count, per block
+__global__ __launch_bounds__(256) void count_rows_kernel(const int64_t* __restrict__ label, int64_t ignore, int64_t P, int C,
+                                                         int* __restrict__ counts) {
+    __shared__ int part[4];
+    int n = 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < P; i += (int64_t)COUNT_BLOCKS * 256) {
+        const int64_t a = label[i];
+        n += a != ignore && a >= 0 && a < C ? 1 : 0;
+    }
+    n = lanes_sum<64>(n);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) counts[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// x *= g[0]; nothing to do, and nothing read, where it is 1 (a loss that backward() is called on)
+__global__ __launch_bounds__(256) void scale_by_kernel(float* __restrict__ x, int64_t n, const float* __restrict__ g) {
+    const float f = g[0];
+    if (f == 1.f) return;
+    f32x4* x4 = reinterpret_cast<f32x4*>(x);
+    const int64_t stride = (int64_t)gridDim.x * 256, quads = n >> 2;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += stride) x4[i] = x4[i] * f;
+    const int64_t i = quads * 4 + (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) x[i] *= f;
 }
 
 struct PolicyOut {
@@ -380,7 +445,7 @@ static int lp_blocks(int64_t P, int G, int cap) {
 struct LpCall {
     const void* z; int64_t ld; const int64_t* label; int64_t ignore; int64_t P; int C; float2* stats; hipStream_t st;
     // forward
-    float* lp; const PolicyArgs* pa;
+    float* lp; const PolicyArgs* pa; void* grad; const int* counts;
     // backward
     const float* g; const float* gloss; const float* inv_count; void* dz;
 };
@@ -423,13 +488,21 @@ static int tile_lanes(int bytes, const void* z, int64_t ld, int64_t P, int C) {
 template <class T, int L, int W>
 static int tile_launch(const LpCall& c) {
     const int64_t tiles = (c.P + 256 / L - 1) / (256 / L);
-    const int grid = (int)(tiles < LP_MAX_BLOCKS ? tiles : LP_MAX_BLOCKS);
-    if (c.pa) {
-        auto k = label_logp_tile_kernel<T, L, W, true>;
-        hipLaunchKernelGGL(k, dim3(grid), dim3(256), 0, c.st, (const T*)c.z, c.label, c.ignore, c.P, c.C, (float*)nullptr, c.stats, *c.pa);
+    const dim3 grid((unsigned)(tiles < LP_MAX_BLOCKS ? tiles : LP_MAX_BLOCKS)), block(256);
+    const T* z = (const T*)c.z;
+    if (c.grad) {
+        if constexpr (sizeof(T) == 4) {
+            auto k = label_logp_tile_kernel<T, L, W, true, true>;
+            hipLaunchKernelGGL(k, grid, block, 0, c.st, z, c.label, c.ignore, c.P, c.C, (float*)nullptr, c.stats, *c.pa, c.counts, (T*)c.grad);
+        }
+    } else if (c.pa) {
+        auto k = label_logp_tile_kernel<T, L, W, true, false>;
+        hipLaunchKernelGGL(k, grid, block, 0, c.st, z, c.label, c.ignore, c.P, c.C, (float*)nullptr, c.stats, *c.pa, (const int*)nullptr,
+                           (T*)nullptr);
     } else {
-        auto k = label_logp_tile_kernel<T, L, W, false>;
-        hipLaunchKernelGGL(k, dim3(grid), dim3(256), 0, c.st, (const T*)c.z, c.label, c.ignore, c.P, c.C, c.lp, c.stats, PolicyArgs{});
+        auto k = label_logp_tile_kernel<T, L, W, false, false>;
+        hipLaunchKernelGGL(k, grid, block, 0, c.st, z, c.label, c.ignore, c.P, c.C, c.lp, c.stats, PolicyArgs{}, (const int*)nullptr,
+                           (T*)nullptr);
     }
     SEMSEG_LAUNCH_CHECK();
     return 0;
@@ -473,12 +546,27 @@ extern "C" int semseg_label_logp_fwd(const void* z, int type, int64_t ld, const 
     return lp_dispatch(c, type);
 }
 
-extern "C" size_t semseg_policy_loss_workspace_bytes(void) { return (size_t)LP_MAX_BLOCKS * 4 * sizeof(double); }
+extern "C" size_t semseg_policy_loss_workspace_bytes(void) { return (size_t)LP_MAX_BLOCKS * 4 * sizeof(double) + COUNT_BLOCKS * sizeof(int); }
+
+// Whether a loss whose gradient is wanted writes it in its forward pass.  float32 only: an upstream gradient other than 1 multiplies the
+// written values, and 16-bit ones would be rounded twice.
+constexpr int64_t ONE_PASS_BYTES = 8 << 20;
+extern "C" int semseg_policy_loss_one_pass(const void* z, int type, int64_t ld, int64_t P, int C) {
+    return z && type == SEMSEG_TYPE_F32 && P > 0 && P <= 1 << 30 && C > 0 && P * C >= ONE_PASS_BYTES / 4 && tile_lanes(4, z, ld, P, C) > 0;
+}
+
+extern "C" int semseg_scale_by(float* x, int64_t n, const float* g, void* stream) {
+    if (!x || !g || n <= 0 || !aligned16(x)) return SEMSEG_EINVAL;
+    const int64_t b = (n / 4 + 1023) / 1024;
+    hipLaunchKernelGGL(scale_by_kernel, dim3((unsigned)(b < 1 ? 1 : b > 2048 ? 2048 : b)), dim3(256), 0, (hipStream_t)stream, x, n, g);
+    SEMSEG_LAUNCH_CHECK();
+    return 0;
+}
 
 extern "C" int semseg_policy_loss_fwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, int64_t P, int C,
                                       const float* advantage, int64_t rows_per_advantage, const float* old_logp, const float* ref_logp,
                                       float clip_low, float clip_high, float kl_weight, float* stats, float* coef, float* loss, float* kl,
-                                      float* clipped, float* inv_count, void* workspace, size_t workspace_bytes, void* stream) {
+                                      float* clipped, float* inv_count, void* dz, void* workspace, size_t workspace_bytes, void* stream) {
     if (!lp_ok(z, ld, label, P, C) || !advantage || rows_per_advantage <= 0 || !old_logp || !stats || !coef || !loss || !kl || !clipped || !inv_count ||
         !(clip_low >= 0.f && clip_low <= 1.f) || !(clip_high >= 0.f) || !(kl_weight >= 0.f) || (kl_weight > 0.f && !ref_logp))
         return SEMSEG_EINVAL;
@@ -490,6 +578,14 @@ extern "C" int semseg_policy_loss_fwd(const void* z, int type, int64_t ld, const
     LpCall c{};
     c.z = z; c.ld = ld; c.label = label; c.ignore = ignore_index; c.P = P; c.C = C; c.stats = (float2*)stats; c.st = (hipStream_t)stream;
     c.pa = &pa;
+    if (dz) {
+        if (!semseg_policy_loss_one_pass(z, type, ld, P, C) || !aligned16(dz)) return SEMSEG_EINVAL;
+        int* counts = (int*)((char*)workspace + (size_t)LP_MAX_BLOCKS * 4 * sizeof(double));
+        hipLaunchKernelGGL(count_rows_kernel, dim3(COUNT_BLOCKS), dim3(256), 0, c.st, label, ignore_index, P, C, counts);
+        SEMSEG_LAUNCH_CHECK();
+        c.grad = dz;
+        c.counts = counts;
+    }
     if (int rc = lp_dispatch(c, type)) return rc;
     const int bytes = type == SEMSEG_TYPE_F32 ? 4 : 2;
     const int l = tile_lanes(bytes, z, ld, P, C);

@@ -2388,12 +2388,12 @@ def _upstream(g):
 
 class LabelLogProbFn(Function):
     @staticmethod
-    def forward(ctx, z, label, ignore_index):
+    def forward(ctx, z, label, ignore_index, wanted):
         shape, rows = tuple(z.shape), _row_shape('label_log_prob', z)
         label = _row_labels('label_log_prob', z, rows, label)
         z, ld, P, c = _logit_rows(z)
         lp = torch.empty(rows, device=z.device, dtype=torch.float32)
-        stats = torch.empty(2 * P, device=z.device, dtype=torch.float32) if ctx.needs_input_grad[0] else None
+        stats = torch.empty(2 * P, device=z.device, dtype=torch.float32) if wanted else None
         if P:
             with _device_guard(z.device):
                 _native.check(_native.lib().semseg_label_logp_fwd(z.data_ptr(), _TYPE_CODES[z.dtype], ld, label.data_ptr(), ignore_index, P,
@@ -2409,7 +2409,7 @@ class LabelLogProbFn(Function):
         z, label, stats = ctx.saved_tensors
         ld, shape, ignore_index = ctx.cfg
         g = _upstream(g)
-        return _label_logp_bwd(z, ld, shape, label, ignore_index, stats.data_ptr(), g.data_ptr(), 0, 0), None, None
+        return _label_logp_bwd(z, ld, shape, label, ignore_index, stats.data_ptr(), g.data_ptr(), 0, 0), None, None, None
 
 
 def label_log_prob(z, label, ignore_index=-1):
@@ -2417,7 +2417,7 @@ def label_log_prob(z, label, ignore_index=-1):
     pixel stride) or [P, C], float32 / bfloat16 / float16; label [N, H, W] or [P], integers.  Returns float32 of the label's shape;
     rows whose label is `ignore_index` or outside [0, C) give 0 and a zero gradient.  Log probabilities are logits too, so the
     output of log_softmax can be handed in.  Differentiable in z."""
-    return LabelLogProbFn.apply(z, label, int(ignore_index))
+    return LabelLogProbFn.apply(z, label, int(ignore_index), torch.is_grad_enabled() and z.requires_grad)
 
 
 def _row_constants(what, name, t, shapes, device):
@@ -2437,7 +2437,7 @@ def _row_constants(what, name, t, shapes, device):
 
 class PolicyLossFn(Function):
     @staticmethod
-    def forward(ctx, z, label, advantage, old_logp, ref_logp, clip_low, clip_high, kl_weight, ignore_index):
+    def forward(ctx, z, label, advantage, old_logp, ref_logp, clip_low, clip_high, kl_weight, ignore_index, wanted):
         what = 'policy_loss'
         shape, dev, rows = tuple(z.shape), z.device, _row_shape(what, z)
         label = _row_labels(what, z, rows, label)
@@ -2447,6 +2447,7 @@ class PolicyLossFn(Function):
             ref_logp = _row_constants(what, 'ref_logp', ref_logp, (rows,), dev)
         z, ld, P, c = _logit_rows(z)
         ctx.set_materialize_grads(False)
+        ctx.dz = None
         if P == 0:
             loss, kl, clipped = (torch.zeros((), device=dev) for _ in range(3))
             kept = torch.zeros(1, device=dev)
@@ -2460,12 +2461,16 @@ class PolicyLossFn(Function):
             ws = kept.data_ptr()
             stats = ws + scratch
             coef = stats + 8 * P
+            dz = None
+            if wanted and L.semseg_policy_loss_one_pass(z.data_ptr(), _TYPE_CODES[z.dtype], ld, P, c):
+                dz = _empty_like_rows(z, shape)
             with _device_guard(dev):
                 _native.check(L.semseg_policy_loss_fwd(z.data_ptr(), _TYPE_CODES[z.dtype], ld, label.data_ptr(), ignore_index, P, c,
                                                        advantage.data_ptr(), P // advantage.numel(), old_logp.data_ptr(), _p(ref_logp),
                                                        clip_low, clip_high, kl_weight, stats, coef, loss.data_ptr(), kl.data_ptr(),
-                                                       clipped.data_ptr(), coef + 4 * P, ws, scratch, _st()), 'policy_loss_fwd')
-        if ctx.needs_input_grad[0]:
+                                                       clipped.data_ptr(), coef + 4 * P, _p(dz), ws, scratch, _st()), 'policy_loss_fwd')
+            ctx.dz = dz
+        if wanted:
             ctx.save_for_backward(z, label, kept)
             ctx.cfg = (ld, shape, ignore_index)
         ctx.mark_non_differentiable(kl, clipped)
@@ -2475,14 +2480,19 @@ class PolicyLossFn(Function):
     @once_differentiable
     def backward(ctx, gloss, gkl, gclipped):
         if gloss is None:
-            return (None,) * 9
+            return (None,) * 10
         z, label, kept = ctx.saved_tensors
         ld, shape, ignore_index = ctx.cfg
         gloss = _upstream(gloss)
+        dz, ctx.dz = ctx.dz, None
+        if dz is not None:                            # written by the forward pass; handed out once, a second backward computes its own
+            with _device_guard(dz.device):
+                _native.check(_native.lib().semseg_scale_by(dz.data_ptr(), dz.numel(), gloss.data_ptr(), _st()), 'scale_by')
+            return (dz,) + (None,) * 9
         P = label.numel()
         inv = kept.data_ptr() + 4 * (kept.numel() - 1)
         coef = inv - 4 * P
-        return (_label_logp_bwd(z, ld, shape, label, ignore_index, coef - 8 * P, coef, gloss.data_ptr(), inv),) + (None,) * 8
+        return (_label_logp_bwd(z, ld, shape, label, ignore_index, coef - 8 * P, coef, gloss.data_ptr(), inv),) + (None,) * 9
 
 
 def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip_high=0.2, kl_weight=0.0, ignore_index=-1):
@@ -2502,7 +2512,8 @@ def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip
         raise ValueError('policy_loss: kl_weight must not be negative, got %r' % kl_weight)
     if kl_weight > 0.0 and ref_logp is None:
         raise ValueError('policy_loss: a KL term needs ref_logp')
-    return PolicyLossFn.apply(z, label, advantage, old_logp, ref_logp, clip_low, clip_high, kl_weight, int(ignore_index))
+    return PolicyLossFn.apply(z, label, advantage, old_logp, ref_logp, clip_low, clip_high, kl_weight, int(ignore_index),
+                              torch.is_grad_enabled() and z.requires_grad)
 
 
 # ------------------------------------------------------------------------------------------------

@@ -219,8 +219,15 @@ def reference_policy(z, label, adv, old, ref, lo, hi, w):
     return out, (pick(erow).sum() / count, ek), pick(g) / count, pick(eg) / count, (logp, x, top, valid)
 
 
-@pytest.mark.parametrize('dtype', TYPES, ids=str)
-@pytest.mark.parametrize('shape,layout', [c for c in ROW_CASES if c[0][1] < 60000], ids=str)
+# logits whose gradient the forward pass writes (float32, dense, at least 2 M of them): every number of lanes a row, whole and partial
+# last tiles, odd and even rows
+ONE_PASS = [((2, 150, 100, 80), 'nhwc'), ((1, 151, 121, 117), 'nhwc'), ((1, 2, 1000, 1100), 'nhwc'), ((1, 19, 333, 335), 'nhwc'),
+            ((2, 40, 180, 150), 'nhwc'), ((1, 77, 1, 27301), 'rows'), ((1, 300, 70, 101), 'nhwc'), ((1, 319, 80, 83), 'nhwc'),
+            ((1, 1, 1500, 1401), 'nhwc'), ((2, 64, 128, 130), 'nchw')]
+
+
+@pytest.mark.parametrize('shape,layout,dtype', [(*c, t) for c in ROW_CASES if c[0][1] < 60000 for t in TYPES] +
+                         [(*c, torch.float32) for c in ONE_PASS], ids=str)
 def test_policy_loss(shape, layout, dtype):
     from mit_semseg import ops
     gen = torch.Generator().manual_seed(sum(shape))
@@ -231,7 +238,7 @@ def test_policy_loss(shape, layout, dtype):
     loss, kl, clipped = ops.policy_loss(z, label, adv, old, ref, lo, hi, w)
     assert loss.shape == kl.shape == clipped.shape == () and not kl.requires_grad and not clipped.requires_grad
     want, err, g, eg, (logp, x, top, valid) = reference_policy(z, label, adv, old, ref, lo, hi, w)
-    for got, value, e in ((loss, want[0], err[0]), (kl, want[1], err[1]), (clipped, torch.tensor(want[2]), 0.0)):
+    for got, value, e in ((loss.detach(), want[0], err[0]), (kl, want[1], err[1]), (clipped, torch.tensor(want[2]), 0.0)):
         assert abs(float(got) - float(value)) <= float(e) + 2 * U32 * abs(float(value)), (float(got), float(value), float(e))
     up = 0.4
     dz = torch.autograd.grad(loss * up, z)[0]
@@ -248,6 +255,9 @@ def test_policy_loss(shape, layout, dtype):
         wantz.abs() * (half(dtype) + 4 * U32) + tiny(dtype) + 1e-37
     assert torch.all((got - wantz).abs() <= bound), float(((got - wantz).abs() / bound).max())
     assert torch.all(got[~valid] == 0)
+    loss, _, _ = ops.policy_loss(z, label, adv, old, ref, lo, hi, w)
+    one = as_rows(torch.autograd.grad(loss, z)[0]).cpu().double()         # upstream 1
+    assert torch.all((up * one - wantz).abs() <= bound + up * tiny(dtype))
 
 
 def test_policy_gradient_against_differences():
@@ -314,11 +324,24 @@ def test_backward_twice_and_shared_logits():
     """retain_graph gives the same gradient again; logits used by two operators get the sum"""
     from mit_semseg import ops
     gen = torch.Generator().manual_seed(9)
+    big = policy_inputs((2, 150, 96, 97), torch.float32, 'nhwc', gen)            # its gradient is written by the forward pass
     z, label, adv, old, ref = policy_inputs((2, 150, 6, 7), torch.float32, 'nhwc', gen)
-    loss, _, _ = ops.policy_loss(z, label, adv, old, ref, kl_weight=0.1)
-    a = torch.autograd.grad(loss, z, retain_graph=True)[0]
-    b = torch.autograd.grad(loss, z)[0]
-    assert torch.equal(a, b)
+    for zz, *rest in (big, (z, label, adv, old, ref)):
+        loss, _, _ = ops.policy_loss(zz, *rest, kl_weight=0.1)
+        a, b, c = [torch.autograd.grad(loss, zz, grad_outputs=torch.tensor(u, device=dev()), retain_graph=True)[0] for u in (1.0, 1.0, 3.0)]
+        # a second backward computes p from the kept parts instead of from the row's sum: within p's roundings
+        close = 2 * U32 * (3 * 24.0 + 3 * math.log(150) + log_sum_roundings(150) + 6)
+        scale = a.abs().amax(dim=1, keepdim=True)
+        assert torch.all((a - b).abs() <= close * scale) and torch.all((c - 3 * b).abs() <= 4 * U32 * (3 * b).abs() + 1e-37)
+        assert a.data_ptr() != b.data_ptr()
+        loss, _, _ = ops.policy_loss(zz, *rest, kl_weight=0.1)
+        d = torch.autograd.grad(2.0 * loss, zz)[0]
+        assert torch.all((d - 2 * b).abs() <= close * 2 * scale)
+        loss, _, _ = ops.policy_loss(zz, *rest, kl_weight=0.1)
+        with torch.no_grad():
+            zz.add_(0.0)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            torch.autograd.grad(loss, zz)
     lp = ops.label_log_prob(z, label)
     loss, _, _ = ops.policy_loss(z, label, adv, old, ref, kl_weight=0.1)
     both = torch.autograd.grad(loss + lp.sum(), z)[0]
@@ -507,7 +530,7 @@ def test_two_streams_at_once():
     """the same operators on two streams, without waiting in between, give what they give one after the other"""
     from mit_semseg import ops
     gen = torch.Generator().manual_seed(3)
-    sets = [policy_inputs((2, 150, 64, 64), torch.float32, 'nhwc', gen) for _ in range(2)]
+    sets = [policy_inputs(shape, torch.float32, 'nhwc', gen) for shape in ((2, 150, 64, 64), (2, 150, 96, 90))]
 
     def work(z, label, adv, old, ref):
         loss, kl, clipped = ops.policy_loss(z, label, adv, old, ref, kl_weight=0.1)
