@@ -84,9 +84,9 @@ struct Adam8Item {
 __device__ __forceinline__ void put_states(AdamEntry& e, const AdamItem& i) { e.m = i.m; e.v = i.v; }
 __device__ __forceinline__ void put_states(Adam8Entry& e, const Adam8Item& i) { e.m = i.m; e.ms = i.ms; e.r = i.r; e.rs = i.rs; }
 
-template <class ITEM>
+template <class ITEM, int MOST>
 struct BeginBatch {
-    static constexpr int MAX = 3800 / (int)sizeof(ITEM);
+    static constexpr int MAX = MOST;
     ITEM item[MAX];
     int n, base;                    // tensors of this batch, and the index of the first one in the call
 };
@@ -97,8 +97,8 @@ struct BeginArgs {
     uint32_t seed;
 };
 
-template <class ITEM, class ENTRY>
-__global__ __launch_bounds__(64) void adamw_begin_kernel(const BeginBatch<ITEM> b, const BeginArgs a, ENTRY* __restrict__ table,
+template <class ITEM, class ENTRY, int MOST>
+__global__ __launch_bounds__(64) void adamw_begin_kernel(const BeginBatch<ITEM, MOST> b, const BeginArgs a, ENTRY* __restrict__ table,
                                                          uint32_t* __restrict__ first) {
     const int k = threadIdx.x;
     if (k >= b.n) return;
@@ -249,7 +249,8 @@ extern "C" size_t semseg_adamw_workspace_bytes(int n) {
 template <class ITEM, class ENTRY, class TENSOR, class KERNEL>
 static int adam_step(const TENSOR* tensors, int n, const float* lr, double beta1, double beta2, double eps, float grad_scale, const float* clip,
                      uint32_t seed, int chunk, KERNEL kernel, void* workspace, size_t workspace_bytes, hipStream_t st) {
-    typedef BeginBatch<ITEM> Batch;
+    typedef BeginBatch<ITEM, 3800 / (int)sizeof(ITEM)> Batch;
+    typedef BeginBatch<ITEM, 8> SmallBatch;                  // few tensors: fewer arguments to hand over
     static_assert(sizeof(Batch) + sizeof(BeginArgs) <= 4000 && Batch::MAX <= 64, "kernel arguments");
     if (n < 0 || (n && (!tensors || !lr)) || !hyper_ok(beta1, beta2, eps)) return SEMSEG_EINVAL;
     const int64_t most = (int64_t)1 << 30;                   // blocks of a launch
@@ -288,8 +289,17 @@ static int adam_step(const TENSOR* tensors, int n, const float* lr, double beta1
                 chunks += (uint32_t)c;
             }
             if (b.n == 0) break;
-            auto begin = adamw_begin_kernel<ITEM, ENTRY>;
-            hipLaunchKernelGGL(begin, dim3(1), dim3(64), 0, st, b, a, table, first);
+            if (b.n <= SmallBatch::MAX) {
+                SmallBatch few;
+                few.n = b.n;
+                few.base = b.base;
+                for (int k = 0; k < b.n; ++k) few.item[k] = b.item[k];
+                auto begin = adamw_begin_kernel<ITEM, ENTRY, SmallBatch::MAX>;
+                hipLaunchKernelGGL(begin, dim3(1), dim3(64), 0, st, few, a, table, first);
+            } else {
+                auto begin = adamw_begin_kernel<ITEM, ENTRY, Batch::MAX>;
+                hipLaunchKernelGGL(begin, dim3(1), dim3(64), 0, st, b, a, table, first);
+            }
             SEMSEG_LAUNCH_CHECK();
         }
         hipLaunchKernelGGL(kernel, dim3(chunks), dim3(256), 0, st, (const ENTRY*)(table + start), (const uint32_t*)(first + start), i - start, h);

@@ -75,22 +75,36 @@ SEMSEG_HD void adam_update32(float& p, float g, float& m, float& v, const AdamCo
     p = adam_moved(p, m, sqrtf(v), c, h.eps);
 }
 
-// Root and reciprocal of the 8-bit step: the hardware's, off by at most one unit of the last place (the correctly rounded ones take
-// about 12 instructions each, and the 8-bit step has so few bytes an element that instructions bound it).  The root takes denormals as
-// zero: a second moment below 1e-38, a gradient below 1e-17.
+// Root and reciprocal of the 8-bit step, which has so few bytes an element that instructions bound it.
+// The root decides codes and is rounded to nearest: the hardware's is within one unit of the last place, and of it and its two neighbours
+// the one is taken whose half-unit interval holds x -- (s - u/2)^2 = s (s - u) up to u^2/4, so the sign of x - s (s - u), one rounding,
+// tells.  That is 8 instructions instead of the 17 of a root that also scales the denormals, which count as zero here (a second moment
+// below 1e-38).  The reciprocal only moves the parameter: the hardware's, one unit off at most.
 #if defined(__HIP_DEVICE_COMPILE__)
-SEMSEG_HD float adam_root(float x) { return __builtin_amdgcn_sqrtf(x); }
+SEMSEG_HD float adam_root(float x) {
+    const float s = __builtin_amdgcn_sqrtf(x);
+    const float down = adam_float(adam_bits(s) - 1u), up = adam_float(adam_bits(s) + 1u);
+    float r = fmaf(-down, s, x) <= 0.0f ? down : s;
+    r = fmaf(-up, s, x) > 0.0f ? up : r;
+    return x > 0.0f && x < INFINITY ? r : s;
+}
 SEMSEG_HD float adam_reciprocal(float x) { return __builtin_amdgcn_rcpf(x); }
 #else
 SEMSEG_HD float adam_root(float x) { return sqrtf(x); }
 SEMSEG_HD float adam_reciprocal(float x) { return 1.0f / x; }
 #endif
 
-// states in 8 bits, before they are coded again: m and r in 32 bits
+// states in 8 bits, before they are coded again: m and r in 32 bits.  Every product and sum of the states is rounded by itself (no
+// contraction): next to a border of the rounding the last bit decides the code, so the definition fixes it.
 SEMSEG_HD void adam_update8(float& p, float g, float& m, float& r, const AdamCoef& c, const AdamHyper& h) {
-    g *= c.factor;
-    m = fmaf(h.b1, m, h.c1 * g);
-    r = adam_root(fmaf(h.b2, r * r, (h.c2 * g) * g));
+#ifdef __clang__
+#pragma clang fp contract(off)
+#endif
+    g = g * c.factor;
+    const float m0 = h.b1 * m, m1 = h.c1 * g;
+    m = m0 + m1;
+    const float v0 = h.b2 * (r * r), v1 = (h.c2 * g) * g;
+    r = adam_root(v0 + v1);
     const float u = m * adam_reciprocal(fmaf(r, c.root, h.eps));
     p = p - fmaf(c.size, u, c.decay * p);
 }
@@ -101,7 +115,7 @@ SEMSEG_HD float adam8_scale(uint32_t top) {
     const float a = adam_float(top);
     return a < ADAM8_TINY ? 0.0f : a * (1.0f / 448.0f);
 }
-SEMSEG_HD float adam8_inverse(float scale) { return scale > 0.0f ? adam_reciprocal(scale) : 0.0f; }
+SEMSEG_HD float adam8_inverse(float scale) { return scale > 0.0f ? 1.0f / scale : 0.0f; }
 
 // what is coded: value / scale, limited to the range (the largest may come out a bit above); a positive r is at least the smallest code
 SEMSEG_HD float adam8_limited(float a, float low) { return fminf(fmaxf(a, low), ADAM8_MAX); }

@@ -219,8 +219,8 @@ def reference_policy(z, label, adv, old, ref, lo, hi, w):
     return out, (pick(erow).sum() / count, ek), pick(g) / count, pick(eg) / count, (logp, x, top, valid)
 
 
-# logits whose gradient the forward pass writes (float32, dense, at least 2 M of them): every number of lanes a row, whole and partial
-# last tiles, odd and even rows
+# more logits whose gradient the forward pass writes (float32, dense, 8 to 320 classes): every number of lanes a row, whole and partial last
+# tiles, odd and even rows, and neighbours of the rule
 ONE_PASS = [((2, 150, 100, 80), 'nhwc'), ((1, 151, 121, 117), 'nhwc'), ((1, 2, 1000, 1100), 'nhwc'), ((1, 19, 333, 335), 'nhwc'),
             ((2, 40, 180, 150), 'nhwc'), ((1, 77, 1, 27301), 'rows'), ((1, 300, 70, 101), 'nhwc'), ((1, 319, 80, 83), 'nhwc'),
             ((1, 1, 1500, 1401), 'nhwc'), ((2, 64, 128, 130), 'nchw')]
