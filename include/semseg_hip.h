@@ -628,17 +628,18 @@ int semseg_grad_norm(const semseg_grad_tensor* tensors_host, int n, float grad_s
  *   + kl_weight (exp(ref_logp - lp) - (ref_logp - lp) - 1), A = advantage[row / rows_per_advantage]; kl = the mean KL term, clipped =
  *   the share of rows that are clipped, inv_count = 1 / valid rows (one float each, all 0 without a valid row); coef: P floats for
  *   the backward call.
- * label_logp_bwd: dz (P x C dense, z's type) = g[row] * s * (1[c = label] - softmax(z)[c]), s = gloss[0] * inv_count[0] where gloss is
+ * label_logp_bwd: dz (P x C dense, 16-byte aligned, z's type) = g[row] * s * (1[c = label] - softmax(z)[c]), s = gloss[0] * inv_count[0] where gloss is
  *   given (the policy loss: g = coef, inv_count as it left it), else 1; rows that are not valid get zeros. */
+size_t semseg_label_logp_workspace_bytes(int type, int64_t ld, int64_t P, int C);      /* 0 unless few rows are long */
 int semseg_label_logp_fwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, int64_t P, int C, float* lp,
-                          float* stats, void* stream);
-size_t semseg_policy_loss_workspace_bytes(void);
+                          float* stats, void* workspace, size_t workspace_bytes, void* stream);
+size_t semseg_policy_loss_workspace_bytes(int type, int64_t ld, int64_t P, int C);
 int semseg_policy_loss_fwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, int64_t P, int C,
                            const float* advantage, int64_t rows_per_advantage, const float* old_logp, const float* ref_logp,
                            float clip_low, float clip_high, float kl_weight, float* stats, float* coef, float* loss, float* kl, float* clipped,
                            float* inv_count, void* dz, void* workspace, size_t workspace_bytes, void* stream);
 /* dz (may be NULL): the gradient of the logits for an upstream gradient of 1, written by the forward call where policy_loss_one_pass says
- * so (dense float32 rows of 8 to 320 classes); scale_by multiplies n floats (16-byte aligned) by a device scalar. */
+ * so (float32 rows of 8 to 320 classes that lie close together); scale_by multiplies n floats (16-byte aligned) by a device scalar. */
 int semseg_policy_loss_one_pass(const void* z, int type, int64_t ld, int64_t P, int C);
 int semseg_scale_by(float* x, int64_t n, const float* g, void* stream);
 int semseg_label_logp_bwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, const float* stats,

@@ -8,9 +8,14 @@
 //   dz[c] = g (1[c = a] - exp(z[c] - max z - log sum)),  g = upstream * (-(not clipped) ratio A + w (1 - exp(ref - lp))) / valid rows
 //
 // Rows are valid where the label is not ignore_index and inside [0, C); the others add nothing and get a zero gradient, whatever their
-// logits hold.  A row belongs to G lanes (G = 1, 4, 16, 64 or a block of 256): a running maximum and a running sum, one pass over the
-// logits.  The maximum and the logarithm of the sum are kept apart for the gradient (their sum loses the logarithm's bits once the
-// logits are large), which is a second pass over the logits and one write.  Bound: HBM.
+// logits hold.  The maximum and the logarithm of the sum are kept apart for the gradient: their sum loses the logarithm's bits once the
+// logits are large.
+//
+// Bound: HBM -- the logits read once, for a gradient read once more (or not, see GRAD) and the gradient written.  Three layouts:
+//  * rows of few classes that lie close together (a map's pixels): a block takes 256 / L rows as one stretch of memory, through LDS;
+//  * longer rows, or rows far apart: 16, 64 or 256 lanes a row, straight from memory, a running maximum and sum;
+//  * few long rows (one token over a vocabulary): several blocks a row, joined by a second kernel.
+// All memory accesses are 16 bytes wide wherever a row starts: the hardware takes them at any element's address.
 #include "common.h"
 
 typedef __bf16 bf16_t;
@@ -18,96 +23,131 @@ typedef _Float16 f16_t;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-template <class T, int V>
+// N elements, aligned as one of them
+template <class T, int N>
 struct Vec {
-    typedef T type __attribute__((ext_vector_type(V)));
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
-template <class T>
-struct Vec<T, 1> {
-    typedef T type;
-};
-template <class T, int V>
-__device__ __forceinline__ void unpack(const typename Vec<T, V>::type& v, float (&x)[V]) {
-    if constexpr (V == 1) {
-        x[0] = (float)v;
+template <class T, int N>
+__device__ __forceinline__ void load_vec(const T* p, float (&x)[N]) {
+    if constexpr (N == 1) {
+        x[0] = (float)*p;
     } else {
+        const typename Vec<T, N>::type v = *reinterpret_cast<const typename Vec<T, N>::type*>(p);
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = (float)v[j];
+        for (int j = 0; j < N; ++j) x[j] = (float)v[j];
     }
 }
-template <class T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&x)[V]) {
-    unpack<T, V>(*reinterpret_cast<const typename Vec<T, V>::type*>(p), x);
-}
-// H vectors of a row, a group of G lanes' apart; what lies behind the row is -infinity
-template <class T, int G, int V, int H>
-__device__ __forceinline__ void load_part(const T* __restrict__ zr, int c0, int C, typename Vec<T, V>::type (&raw)[H]) {
-#pragma unroll
-    for (int u = 0; u < H; ++u) {
-        const int c = c0 + u * (G * V);
-        if (c + V <= C) {
-            raw[u] = *reinterpret_cast<const typename Vec<T, V>::type*>(zr + c);
-        } else if constexpr (V == 1) {
-            raw[u] = (T)-INFINITY;
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) raw[u][j] = c + j < C ? zr[c + j] : (T)-INFINITY;
-        }
-    }
-}
-template <class T, int V>
-__device__ __forceinline__ void store_vec(T* p, const float (&x)[V]) {
-    typename Vec<T, V>::type v;
-    if constexpr (V == 1) {
-        v = (T)x[0];
+template <class T, int N>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
+    if constexpr (N == 1) {
+        *p = (T)x[0];
     } else {
+        typename Vec<T, N>::type v;
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = (T)x[j];
+        for (int j = 0; j < N; ++j) v[j] = (T)x[j];
+        *reinterpret_cast<typename Vec<T, N>::type*>(p) = v;
     }
-    *reinterpret_cast<typename Vec<T, V>::type*>(p) = v;
 }
 
-constexpr int LP_HELD = 8;              // vectors of a row that a lane holds at once
 constexpr int LP_MAX_BLOCKS = 2048;     // partial sums of the loss
+constexpr int COUNT_BLOCKS = 256;       // partial counts of the rows that count
+constexpr int TILE_BYTES = 20480;       // 8 blocks of a compute unit at once
+constexpr int MAX_SPLITS = 64;          // blocks of a long row
 
-struct PolicyArgs {
-    const float* advantage;             // [images]
-    const float* old_logp;              // [P]
-    const float* ref_logp;              // [P] or NULL
+enum Mode { LOGP, LOSS, GRAD, BACK };   // GRAD: the loss and, for an upstream gradient of 1, the gradient of the logits
+
+struct Rows {
+    int64_t ld, ignore, P;
+    const int64_t* label;
+    int C;
+};
+struct ForwardArgs {
+    float* lp;                          // LOGP: [P]
+    float2* stats;                      // [P] {maximum, logarithm of the sum}, or NULL
+    // the loss
+    const float* advantage;
+    const float* old_logp;
+    const float* ref_logp;              // or NULL
     int64_t rows_per_advantage;
     int small_rows;                     // row numbers fit 32 bits (a 64-bit division costs more than a row of 150 classes)
     float clip_low, clip_high, kl_weight;
-    float* coef;                        // [P] d(loss * valid rows) / d lp
-    double* partial;                    // [blocks][4]: loss, kl, clipped, valid
+    float* coef;                        // [P] d(loss * rows that count) / d lp
+    double* partial;                    // [blocks][4]: loss, kl, clipped, rows that count
+    const int* counts;                  // GRAD: [COUNT_BLOCKS]
+};
+struct BackArgs {
+    const float2* stats;
+    const float* g;                     // [P]
+    const float* gloss;                 // scalar, or NULL
+    const float* inv_count;             // scalar, with gloss
 };
 
-template <int G>
-__device__ __forceinline__ float group_max(float v, float* lds) {
-    if constexpr (G > 1) {
-#pragma unroll
-        for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+// what belongs to a row beside its logits, requested before them
+struct RowIn {
+    int64_t a;
+    bool valid;
+    float A, old, ref;                  // LOSS, GRAD: the row's first lane alone
+};
+template <int MODE>
+__device__ __forceinline__ RowIn row_in(const Rows& r, const ForwardArgs& f, int64_t row, bool live, bool lead) {
+    RowIn in;
+    in.A = in.old = in.ref = 0.f;
+    in.a = live ? r.label[row] : -1;
+    if (MODE != LOGP && lead && live) {
+        const int64_t image = f.small_rows ? (int64_t)((uint32_t)row / (uint32_t)f.rows_per_advantage) : row / f.rows_per_advantage;
+        in.A = f.advantage[image];
+        in.old = f.old_logp[row];
+        if (f.ref_logp) in.ref = f.ref_logp[row];
     }
-    if constexpr (G > 64) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
-    }
-    return v;
+    in.valid = live && in.a != r.ignore && in.a >= 0 && in.a < r.C;
+    return in;
 }
-template <int G>
-__device__ __forceinline__ float group_sum(float v, float* lds) {
-    if constexpr (G > 1) {
-#pragma unroll
-        for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+
+struct RowSums {
+    double loss = 0.0, kl = 0.0;
+    int clipped = 0, count = 0;
+};
+// one row's answer, by one lane; returns d(loss * rows that count) / d lp
+template <int MODE>
+__device__ __forceinline__ float finish_row(int64_t row, const RowIn& in, float za, float top, float logs, const ForwardArgs& f, RowSums& acc) {
+    const float lp = in.valid ? (za - top) - logs : 0.f;
+    if (f.stats) f.stats[row] = make_float2(top, logs);
+    float coef = 0.f;
+    if constexpr (MODE == LOGP) {
+        f.lp[row] = lp;
+    } else {
+        if (in.valid) {
+            const float ratio = expf(lp - in.old);
+            const float whole = ratio * in.A;
+            const float cut = fminf(fmaxf(ratio, 1.f - f.clip_low), 1.f + f.clip_high) * in.A;
+            const bool clip = cut < whole;
+            float l = clip ? -cut : -whole;
+            coef = clip ? 0.f : -whole;
+            if (f.ref_logp) {
+                const float d = in.ref - lp;
+                const float e = expm1f(d);                           // exp(d) - 1 - d cancels for small d
+                const float k = e - d;
+                l = fmaf(f.kl_weight, k, l);
+                coef = fmaf(-f.kl_weight, e, coef);
+                acc.kl += (double)k;
+            }
+            acc.loss += (double)l;
+            acc.clipped += clip ? 1 : 0;
+            acc.count += 1;
+        }
+        f.coef[row] = coef;
     }
-    if constexpr (G > 64) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) lds[4 + (threadIdx.x >> 6)] = v;
-        __syncthreads();
-        v = (lds[4] + lds[5]) + (lds[6] + lds[7]);
-    }
-    return v;
+    return coef;
+}
+__device__ __forceinline__ void block_partial(const RowSums& acc, double* __restrict__ partial) {
+    __shared__ double sum[4][4];
+    const double loss = wave_sum_d(acc.loss), kl = wave_sum_d(acc.kl);
+    const double clipped = wave_sum_d((double)acc.clipped), count = wave_sum_d((double)acc.count);
+    const int w = threadIdx.x >> 6, j = threadIdx.x;
+    if ((threadIdx.x & 63) == 0) { sum[w][0] = loss; sum[w][1] = kl; sum[w][2] = clipped; sum[w][3] = count; }
+    __syncthreads();
+    if (j < 4) partial[(int64_t)blockIdx.x * 4 + j] = (sum[0][j] + sum[1][j]) + (sum[2][j] + sum[3][j]);
 }
 
 template <int L>
@@ -122,217 +162,303 @@ __device__ __forceinline__ V lanes_sum(V v) {
     for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
-
-struct RowSums {
-    double loss = 0.0, kl = 0.0;
-    int clipped = 0, count = 0;
-};
-// one row's answer, by one lane; returns d(loss * rows that count) / d lp
-template <bool POLICY>
-__device__ __forceinline__ float finish_row(int64_t row, float za, bool valid, float top, float logs, float* __restrict__ lp_out,
-                                           float2* __restrict__ stats, const PolicyArgs& pa, RowSums& acc) {
-    const float lp = valid ? (za - top) - logs : 0.f;
-    if (stats) stats[row] = make_float2(top, logs);
-    float coef = 0.f;
-    if constexpr (!POLICY) {
-        lp_out[row] = lp;
-    } else {
-        if (valid) {
-            const float A = pa.advantage[pa.small_rows ? (int64_t)((uint32_t)row / (uint32_t)pa.rows_per_advantage) : row / pa.rows_per_advantage];
-            const float ratio = expf(lp - pa.old_logp[row]);
-            const float whole = ratio * A;
-            const float cut = fminf(fmaxf(ratio, 1.f - pa.clip_low), 1.f + pa.clip_high) * A;
-            const bool clip = cut < whole;
-            float l = clip ? -cut : -whole;
-            coef = clip ? 0.f : -whole;
-            if (pa.ref_logp) {
-                const float d = pa.ref_logp[row] - lp;
-                const float e = expm1f(d);                           // exp(d) - 1 - d cancels for small d
-                const float k = e - d;
-                l = fmaf(pa.kl_weight, k, l);
-                coef = fmaf(-pa.kl_weight, e, coef);
-                acc.kl += (double)k;
-            }
-            acc.loss += (double)l;
-            acc.clipped += clip ? 1 : 0;
-            acc.count += 1;
-        }
-        pa.coef[row] = coef;
+// the same over a group of G lanes, up to the block (lds: 8 floats; all threads of the block call)
+template <int G>
+__device__ __forceinline__ float group_max(float v, float* lds) {
+    v = lanes_max<(G < 64 ? G : 64)>(v);
+    if constexpr (G > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
     }
-    return coef;
+    return v;
 }
-__device__ __forceinline__ void block_partial(const RowSums& acc, double* __restrict__ partial) {
-    __shared__ double sum[4][4];
-    const double loss = wave_sum_d(acc.loss), kl = wave_sum_d(acc.kl);
-    const double clipped = wave_sum_d((double)acc.clipped), count = wave_sum_d((double)acc.count);
-    const int w = threadIdx.x >> 6, j = threadIdx.x;
-    if ((threadIdx.x & 63) == 0) { sum[w][0] = loss; sum[w][1] = kl; sum[w][2] = clipped; sum[w][3] = count; }
-    __syncthreads();
-    if (j < 4) partial[(int64_t)blockIdx.x * 4 + j] = (sum[0][j] + sum[1][j]) + (sum[2][j] + sum[3][j]);
-}
-
-// POLICY: the loss (lp is not written); otherwise lp of every row.  stats[row] = {max, log sum} (may be NULL)
-template <class T, int G, int V, bool POLICY>
-__global__ __launch_bounds__(256) void label_logp_kernel(const T* __restrict__ z, int64_t ld, const int64_t* __restrict__ label,
-                                                         int64_t ignore, int64_t P, int C, float* __restrict__ lp_out,
-                                                         float2* __restrict__ stats, const PolicyArgs pa) {
-    __shared__ float lds[8];
-    constexpr int ROWS = 256 / G;
-    const int sub = threadIdx.x % G;
-    RowSums acc;
-    for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < P; row0 += (int64_t)gridDim.x * ROWS) {
-        const int64_t row = row0 + threadIdx.x / G;
-        const bool live = row < P;
-        const T* zr = z + (live ? row : 0) * ld;
-        const int64_t a = live ? label[row] : -1;
-        const bool valid = live && a != ignore && a >= 0 && a < C;
-        const float za = valid ? (float)zr[a] : 0.f;
-        float m = -INFINITY, s = 0.f;
-        if (live) {
-            // a long row (a block's) has the next part on its way while one is summed
-            constexpr int HELD = G == 256 ? LP_HELD / 2 : LP_HELD;
-            typename Vec<T, V>::type raw[HELD], next[HELD];
-            load_part<T, G, V, HELD>(zr, sub * V, C, raw);
-            for (int c0 = sub * V; c0 < C; c0 += G * V * HELD) {
-                if (G == 256 && c0 + G * V * HELD < C) load_part<T, G, V, HELD>(zr, c0 + G * V * HELD, C, next);
-                __builtin_amdgcn_sched_barrier(0);
-                float x[HELD][V];
-                float top = -INFINITY;
-#pragma unroll
-                for (int u = 0; u < HELD; ++u) {
-                    unpack<T, V>(raw[u], x[u]);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) top = fmaxf(top, x[u][j]);
-                }
-                const float mn = fmaxf(m, top);
-                const float ref = mn == -INFINITY ? 0.f : mn;            // nothing but -infinity so far: exp(-inf) = 0, not NaN
-                s *= m == -INFINITY ? 0.f : __expf(m - ref);
-#pragma unroll
-                for (int u = 0; u < HELD; ++u)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) s += __expf(x[u][j] - ref);
-                m = mn;
-                if (G < 256) break;                                      // rows of a group fit its lanes' registers (group_of)
-#pragma unroll
-                for (int u = 0; u < HELD; ++u) raw[u] = next[u];
-            }
-        }
-        const float top = group_max<G>(m, lds);
-        const float ref = top == -INFINITY ? 0.f : top;
-        s = group_sum<G>(m == -INFINITY && s == 0.f ? 0.f : s * __expf(m - ref), lds);
-        const float logs = logf(s);
-        if (sub == 0 && live) finish_row<POLICY>(row, za, valid, ref, logs, lp_out, stats, pa, acc);
+template <int G>
+__device__ __forceinline__ float group_sum(float v, float* lds) {
+    v = lanes_sum<(G < 64 ? G : 64)>(v);
+    if constexpr (G > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[4 + (threadIdx.x >> 6)] = v;
+        __syncthreads();
+        v = (lds[4] + lds[5]) + (lds[6] + lds[7]);
     }
-    if constexpr (POLICY) block_partial(acc, pa.partial);
+    return v;
 }
 
-// Dense rows of few classes: a block takes 256 / L rows, one stretch of memory, in 16-byte loads that no row's start or end interrupts,
-// through LDS; then L lanes read a row each.  A row alone is 300 to 600 bytes at 150 classes: loads of its own are 4 or 8 bytes wide.
-constexpr int TILE_BYTES = 20480;       // 8 blocks of a compute unit at once
-//
-// GRAD: the rows are in registers when the loss of a row is known, so their gradient for an upstream gradient of 1 is written at once,
-// through the same tile: the logits are read once and not again by a backward pass.  It needs 1 / (rows that count) beforehand
-// (count_rows_kernel, 8 bytes a row).
-constexpr int COUNT_BLOCKS = 256;
-template <class T, int L, int W, bool POLICY, bool GRAD>
-__global__ __launch_bounds__(256) void label_logp_tile_kernel(const T* __restrict__ z, const int64_t* __restrict__ label, int64_t ignore,
-                                                              int64_t P, int C, float* __restrict__ lp_out, float2* __restrict__ stats,
-                                                              const PolicyArgs pa, const int* __restrict__ counts, T* __restrict__ dz) {
-    constexpr int ROWS = 256 / L, PER = 16 / (int)sizeof(T);
-    constexpr int HELD = TILE_BYTES / 256 / ((int)sizeof(T) * W);      // W: elements of a read from LDS (2 where C is even)
+// ---------------------------------------------------------------- rows of few classes, close together --------------------------
+// A block takes 256 / L rows, padding between them included, as one stretch of memory in 16-byte loads that no row's start or end
+// interrupts, through LDS; then L lanes read a row each and hold it in registers.  A row alone is 300 to 600 bytes at 150 classes.
+// Of 2 x 375 x 501 rows of 150 classes: f32 42 us, f16 25 us (5.4, 4.6 TB/s); a group of lanes per row straight from memory took 64 us in
+// f16.  A gradient leaves the same way.  GRAD: the row is in registers when its loss is known, so its gradient is written at once and the
+// logits are not read by a backward pass (2 x 512 x 512 x 150 f32: loss and gradient 139 us, with a second reading 208 us); it needs
+// 1 / (rows that count) beforehand (count_rows_kernel, 8 bytes a row).
+// W: elements of a read from LDS (2 where classes and pitch are even); HELD: reads of a lane, all unrolled (with a run-time bound the
+// compiler puts the row into scratch memory and f16 rows take five times as long)
+template <class T, int L, int W, int HELD, int MODE>
+__global__ __launch_bounds__(256) void logp_tile_kernel(const T* __restrict__ z, const Rows r, const ForwardArgs f, const BackArgs k,
+                                                        T* __restrict__ dz) {
+    constexpr int ROWS = 256 / L, PER = 16 / (int)sizeof(T), LOADS = TILE_BYTES / 4096;
     __shared__ u32x4 tile[TILE_BYTES / 16];
-    const int sub = threadIdx.x % L;
-    const int64_t tiles = (P + ROWS - 1) / ROWS;
+    T* t = reinterpret_cast<T*>(tile);
+    const int C = r.C, sub = threadIdx.x % L, mine = threadIdx.x / L;
+    const int64_t tiles = (r.P + ROWS - 1) / ROWS;
     RowSums acc;
-    float share = 0.f;                                                 // 1 / rows that count
-    if constexpr (GRAD) {
+    float share = 1.f;
+    if constexpr (MODE == GRAD) {                                      // 1 / rows that count
         __shared__ int part[4];
-        const int s = lanes_sum<64>(counts[threadIdx.x]);
+        const int s = lanes_sum<64>(f.counts[threadIdx.x]);
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
         __syncthreads();
         const int n = (part[0] + part[1]) + (part[2] + part[3]);
         share = n > 0 ? 1.f / (float)n : 0.f;
     }
+    if constexpr (MODE == BACK) {
+        if (k.gloss) share = k.gloss[0] * k.inv_count[0];
+    }
     for (int64_t b = blockIdx.x; b < tiles; b += gridDim.x) {
-        const int64_t row0 = b * ROWS, row = row0 + threadIdx.x / L;
-        const int count = (int)min(P - row0, (int64_t)ROWS) * C;       // elements of this tile
-        const T* src = z + row0 * C;                                   // ROWS * C elements are whole 16-byte pieces: L <= 16
+        const int64_t row0 = b * ROWS, row = row0 + mine;
+        const int rows = (int)min(r.P - row0, (int64_t)ROWS);
+        const bool live = mine < rows;
+        const int count = (rows - 1) * (int)r.ld + C;                  // elements of the stretch
+        const T* src = z + row0 * r.ld;
+        const RowIn in = row_in<MODE == BACK ? LOGP : MODE>(r, f, row, live, sub == 0);
+        float2 st = make_float2(0.f, 0.f);
+        float g = 0.f;
+        if (MODE == BACK && live) {
+            st = k.stats[row];
+            g = k.g[row];
+        }
         const int vecs = count / PER;
-        const bool live = row < P;
-        const int64_t a = live ? label[row] : -1;
-        u32x4 v[TILE_BYTES / 4096];
+        u32x4 v[LOADS];
 #pragma unroll
-        for (int u = 0; u < TILE_BYTES / 4096; ++u)
-            v[u] = vecs ? reinterpret_cast<const u32x4*>(src)[min((int)threadIdx.x + u * 256, vecs - 1)] : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int u = 0; u < TILE_BYTES / 4096; ++u)
-            if ((int)threadIdx.x + u * 256 < vecs) tile[threadIdx.x + u * 256] = v[u];
-        T* t = reinterpret_cast<T*>(tile);
-        for (int i = vecs * PER + threadIdx.x; i < count; i += 256) t[i] = src[i];         // the end of the last tile
-        __syncthreads();
-        const bool valid = live && a != ignore && a >= 0 && a < C;
-        const T* tr = t + (live ? threadIdx.x / L : 0) * C;
-        float x[HELD][W];
-        float m = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < HELD; ++k) {
-            const int c = (sub + k * L) * W;
-            if (c < C) {
-                load_vec<T, W>(tr + c, x[k]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < W; ++j) x[k][j] = -INFINITY;
-            }
+        for (int u = 0; u < LOADS; ++u) {
+            typedef typename Vec<T, PER>::type piece;
+            if (vecs) v[u] = __builtin_bit_cast(u32x4, *reinterpret_cast<const piece*>(src + (size_t)min((int)threadIdx.x + u * 256, vecs - 1) * PER));
         }
 #pragma unroll
-        for (int k = 0; k < HELD; ++k)
+        for (int u = 0; u < LOADS; ++u)
+            if ((int)threadIdx.x + u * 256 < vecs) tile[threadIdx.x + u * 256] = v[u];
+        for (int i = vecs * PER + threadIdx.x; i < count; i += 256) t[i] = src[i];         // what is no whole piece
+        __syncthreads();
+        const T* tr = t + (live ? mine : 0) * (int)r.ld;
+        float x[HELD][W];
 #pragma unroll
-            for (int j = 0; j < W; ++j) m = fmaxf(m, x[k][j]);
-        m = lanes_max<L>(m);
-        const float top = m == -INFINITY ? 0.f : m;
-        float s = 0.f;
+        for (int i = 0; i < HELD; ++i) {
+            const int c = (sub + i * L) * W;
+            if (c < C) {
+                load_vec<T, W>(tr + c, x[i]);
+            } else {
 #pragma unroll
-        for (int k = 0; k < HELD; ++k)
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                x[k][j] = __expf(x[k][j] - top);
-                s += x[k][j];
+                for (int j = 0; j < W; ++j) x[i][j] = -INFINITY;
             }
-        s = lanes_sum<L>(s);
-        float coef = 0.f;
-        if (sub == 0 && live) coef = finish_row<POLICY>(row, valid ? (float)tr[a] : 0.f, valid, top, logf(s), lp_out, stats, pa, acc);
-        if constexpr (GRAD) {
-            const float g = __shfl(coef, (threadIdx.x & 63) / L * L, 64) * share, over = 1.f / s;
-            T* tw = t + threadIdx.x / L * C;
+        }
+        float over = 1.f;                                              // 1 / sum
+        if constexpr (MODE != BACK) {
+            const float za = in.valid && sub == 0 ? (float)tr[in.a] : 0.f;
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) m = fmaxf(m, x[i][j]);
+            }
+            m = lanes_max<L>(m);
+            const float top = m == -INFINITY ? 0.f : m;                // nothing but -infinity: exp(-inf) = 0, not NaN
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    x[i][j] = __expf(x[i][j] - top);
+                    s += x[i][j];
+                }
+            }
+            s = lanes_sum<L>(s);
+            if (sub == 0 && live) g = finish_row<MODE>(row, in, za, top, logf(s), f, acc);
+            if constexpr (MODE == GRAD) {
+                g = __shfl(g, (threadIdx.x & 63) / L * L, 64);
+                over = 1.f / s;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) x[i][j] = __expf((x[i][j] - st.x) - st.y);
+            }
+        }
+        __syncthreads();                                               // every row has been read: the tile is free
+        if constexpr (MODE == GRAD || MODE == BACK) {
+            g *= share;
+            T* tw = t + mine * C;
             if (live) {
 #pragma unroll
-                for (int k = 0; k < HELD; ++k) {
-                    const int c = (sub + k * L) * W;
+                for (int i = 0; i < HELD; ++i) {
+                    const int c = (sub + i * L) * W;
 #pragma unroll
-                    for (int j = 0; j < W; ++j) x[k][j] = valid ? g * ((c + j == (int)a ? 1.f : 0.f) - x[k][j] * over) : 0.f;
-                    if (c < C) store_vec<T, W>(tw + c, x[k]);
+                    for (int j = 0; j < W; ++j) x[i][j] = in.valid ? g * ((c + j == (int)in.a ? 1.f : 0.f) - x[i][j] * over) : 0.f;
+                    if (c < C) store_vec<T, W>(tw + c, x[i]);
                 }
             }
             __syncthreads();
-            T* dst = dz + row0 * C;
+            T* dst = dz + row0 * C;                                    // 256 / L rows are whole 16-byte pieces: L <= 16
+            const int total = rows * C, pieces = total / PER;
 #pragma unroll
-            for (int u = 0; u < TILE_BYTES / 4096; ++u)
-                if ((int)threadIdx.x + u * 256 < vecs) reinterpret_cast<u32x4*>(dst)[threadIdx.x + u * 256] = tile[threadIdx.x + u * 256];
-            for (int i = vecs * PER + threadIdx.x; i < count; i += 256) dst[i] = t[i];
+            for (int u = 0; u < LOADS; ++u)
+                if ((int)threadIdx.x + u * 256 < pieces) reinterpret_cast<u32x4*>(dst)[threadIdx.x + u * 256] = tile[threadIdx.x + u * 256];
+            for (int i = pieces * PER + threadIdx.x; i < total; i += 256) dst[i] = t[i];
+            __syncthreads();
         }
-        __syncthreads();
     }
-    if constexpr (POLICY) block_partial(acc, pa.partial);
+    if constexpr (MODE == LOSS || MODE == GRAD) block_partial(acc, f.partial);
 }
 
+// ---------------------------------------------------------------- longer rows, rows far apart, few rows ------------------------
+// H vectors of a row, a group of G lanes' apart, from class c0 on; what lies at or behind `end` is -infinity
+template <class T, int G, int V, int H>
+__device__ __forceinline__ void load_part(const T* __restrict__ zr, int c0, int end, typename Vec<T, V>::type (&raw)[H]) {
+#pragma unroll
+    for (int u = 0; u < H; ++u) {
+        const int c = c0 + u * (G * V);
+        if (c + V <= end) {
+            raw[u] = *reinterpret_cast<const typename Vec<T, V>::type*>(zr + c);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) raw[u][j] = c + j < end ? zr[c + j] : (T)-INFINITY;
+        }
+    }
+}
+// H: vectors that a lane has in flight, 4, or 8 for the longer rows of a wave (8 for all took 93 us for 120000 x 600 f32, 4 take 59)
+// maximum (0 where there is nothing but -infinity) and sum of a lane's part of [begin, end)
+template <class T, int G, int H>
+__device__ __forceinline__ void lane_sum(const T* __restrict__ zr, int sub, int begin, int end, float& m, float& s) {
+    constexpr int V = 16 / (int)sizeof(T), STEP = G * V * H;
+    typename Vec<T, V>::type raw[H], next[H];
+    m = -INFINITY;
+    s = 0.f;
+    load_part<T, G, V, H>(zr, begin + sub * V, end, raw);
+    for (int c0 = begin + sub * V; c0 < end; c0 += STEP) {
+        // a block's row has the next part on its way while one is summed
+        if (G == 256 && c0 + STEP < end) load_part<T, G, V, H>(zr, c0 + STEP, end, next);
+        __builtin_amdgcn_sched_barrier(0);
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < H; ++u)
+#pragma unroll
+            for (int j = 0; j < V; ++j) top = fmaxf(top, (float)raw[u][j]);
+        const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn;
+        s *= m == -INFINITY ? 0.f : __expf(m - ref);
+#pragma unroll
+        for (int u = 0; u < H; ++u)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += __expf((float)raw[u][j] - ref);
+        m = mn;
+        if (G < 256) break;                                            // rows of a group fit its lanes' registers (group_of)
+#pragma unroll
+        for (int u = 0; u < H; ++u) raw[u] = next[u];
+    }
+}
+// part of a sum, taken relative to the maximum `m` of its own, relative to `ref`
+__device__ __forceinline__ float rescaled(float s, float m, float ref) { return m == -INFINITY && s == 0.f ? 0.f : s * __expf(m - ref); }
+
+template <class T, int G, int H, int MODE>
+__global__ __launch_bounds__(256) void logp_rows_kernel(const T* __restrict__ z, const Rows r, const ForwardArgs f) {
+    __shared__ float lds[8];
+    constexpr int ROWS = 256 / G;
+    const int sub = threadIdx.x % G;
+    RowSums acc;
+    for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < r.P; row0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = row0 + threadIdx.x / G;
+        const bool live = row < r.P;
+        const T* zr = z + (live ? row : 0) * r.ld;
+        const RowIn in = row_in<MODE>(r, f, row, live, sub == 0);
+        float m = -INFINITY, s = 0.f;
+        if (live) lane_sum<T, G, H>(zr, sub, 0, r.C, m, s);
+        const float za = in.valid && sub == 0 ? (float)zr[in.a] : 0.f;
+        const float top = group_max<G>(m, lds);
+        const float ref = top == -INFINITY ? 0.f : top;
+        s = group_sum<G>(rescaled(s, m, ref), lds);
+        if (sub == 0 && live) finish_row<MODE>(row, in, za, ref, logf(s), f, acc);
+    }
+    if constexpr (MODE == LOSS) block_partial(acc, f.partial);
+}
+
+// few long rows: block (x, y) sums part y of row x, join_rows_kernel the parts.  A row of 131072 f32 classes by one block: 18 us
+template <class T>
+__global__ __launch_bounds__(256) void logp_split_kernel(const T* __restrict__ z, const Rows r, int per, float2* __restrict__ parts) {
+    __shared__ float lds[8];
+    const int begin = (int)min((int64_t)blockIdx.y * per, (int64_t)r.C), end = (int)min((int64_t)begin + per, (int64_t)r.C);
+    float m, s;
+    lane_sum<T, 256, 4>(z + (int64_t)blockIdx.x * r.ld, threadIdx.x, begin, end, m, s);
+    const float top = group_max<256>(m, lds);
+    const float ref = top == -INFINITY ? 0.f : top;
+    s = group_sum<256>(rescaled(s, m, ref), lds);
+    if (threadIdx.x == 0) parts[(int64_t)blockIdx.x * gridDim.y + blockIdx.y] = make_float2(top, s);
+}
+template <class T, int MODE>
+__global__ __launch_bounds__(256) void join_rows_kernel(const T* __restrict__ z, const Rows r, const ForwardArgs f, const float2* __restrict__ parts,
+                                                        int splits) {
+    RowSums acc;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);      // a wave a row, a lane a part
+    const int lane = threadIdx.x & 63;
+    const bool live = row < r.P;
+    const RowIn in = row_in<MODE>(r, f, row, live, lane == 0);
+    float2 p = make_float2(-INFINITY, 0.f);
+    if (live && lane < splits) p = parts[row * splits + lane];
+    const float za = in.valid && lane == 0 ? (float)z[row * r.ld + in.a] : 0.f;
+    const float top = lanes_max<64>(p.x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    // a part of nothing but -infinity was summed relative to 0
+    const float s = lanes_sum<64>(p.x == -INFINITY ? (p.y == 0.f ? 0.f : p.y * __expf(0.f - ref)) : p.y * __expf(p.x - ref));
+    if (lane == 0 && live) finish_row<MODE>(row, in, za, ref, logf(s), f, acc);
+    if constexpr (MODE == LOSS) block_partial(acc, f.partial);
+}
+
+// dz of rows that are no tile; blockIdx.y: part of a long row
+template <class T, int G, int H>
+__global__ __launch_bounds__(256) void logp_rows_bwd_kernel(const T* __restrict__ z, const Rows r, const BackArgs k, int per, T* __restrict__ dz) {
+    constexpr int ROWS = 256 / G, V = 16 / (int)sizeof(T);
+    const int sub = threadIdx.x % G;
+    const float scale = k.gloss ? k.gloss[0] * k.inv_count[0] : 1.f;
+    const int begin = (int)min((int64_t)blockIdx.y * per, (int64_t)r.C), end = (int)min((int64_t)begin + per, (int64_t)r.C);
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; row < r.P; row += (int64_t)gridDim.x * ROWS) {
+        const T* zr = z + row * r.ld;
+        T* dr = dz + row * r.C;
+        const int64_t a = r.label[row];
+        const bool valid = a != r.ignore && a >= 0 && a < r.C;
+        const float2 st = k.stats[row];
+        const float g = valid ? k.g[row] * scale : 0.f;
+        for (int c0 = begin + sub * V; c0 < end; c0 += G * V * H) {
+            typename Vec<T, V>::type raw[H];
+            load_part<T, G, V, H>(zr, c0, end, raw);
+#pragma unroll
+            for (int u = 0; u < H; ++u) {
+                const int c = c0 + u * (G * V);
+                float x[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float p = __expf(((float)raw[u][j] - st.x) - st.y);
+                    x[j] = valid ? g * ((c + j == (int)a ? 1.f : 0.f) - p) : 0.f;
+                }
+                if (c + V <= end) {
+                    store_vec<T, V>(dr + c, x);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (c + j < end) dr[c + j] = (T)x[j];
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- sums, counts, scaling ----------------------------------------
 // rows that count, per block
-__global__ __launch_bounds__(256) void count_rows_kernel(const int64_t* __restrict__ label, int64_t ignore, int64_t P, int C,
-                                                         int* __restrict__ counts) {
+__global__ __launch_bounds__(256) void count_rows_kernel(const Rows r, int* __restrict__ counts) {
     __shared__ int part[4];
     int n = 0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < P; i += (int64_t)COUNT_BLOCKS * 256) {
-        const int64_t a = label[i];
-        n += a != ignore && a >= 0 && a < C ? 1 : 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < r.P; i += (int64_t)COUNT_BLOCKS * 256) {
+        const int64_t a = r.label[i];
+        n += a != r.ignore && a >= 0 && a < r.C ? 1 : 0;
     }
     n = lanes_sum<64>(n);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = n;
@@ -342,17 +468,17 @@ __global__ __launch_bounds__(256) void count_rows_kernel(const int64_t* __restri
 
 // x *= g[0]; nothing to do, and nothing read, where it is 1 (a loss that backward() is called on)
 __global__ __launch_bounds__(256) void scale_by_kernel(float* __restrict__ x, int64_t n, const float* __restrict__ g) {
-    const float f = g[0];
-    if (f == 1.f) return;
+    const float s = g[0];
+    if (s == 1.f) return;
     f32x4* x4 = reinterpret_cast<f32x4*>(x);
     const int64_t stride = (int64_t)gridDim.x * 256, quads = n >> 2;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += stride) x4[i] = x4[i] * f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += stride) x4[i] = x4[i] * s;
     const int64_t i = quads * 4 + (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) x[i] *= f;
+    if (i < n) x[i] *= s;
 }
 
 struct PolicyOut {
-    float* v[4];                        // loss, kl, clipped share, 1 / valid rows; all 0 where no row is valid
+    float* v[4];                        // loss, kl, clipped share, 1 / rows that count; all 0 where no row counts
 };
 __global__ __launch_bounds__(256) void policy_finish_kernel(const double* __restrict__ partial, int blocks, const PolicyOut out) {
     __shared__ double sum[4][4];
@@ -374,179 +500,182 @@ __global__ __launch_bounds__(256) void policy_finish_kernel(const double* __rest
     }
 }
 
-// dz = g * scale * (1[c = a] - p); scale = gloss[0] * inv_count[0] where given, else 1
-template <class T, int G, int V>
-__global__ __launch_bounds__(256) void label_logp_bwd_kernel(const T* __restrict__ z, int64_t ld, const int64_t* __restrict__ label,
-                                                             int64_t ignore, const float2* __restrict__ stats,
-                                                             const float* __restrict__ g, const float* __restrict__ gloss,
-                                                             const float* __restrict__ inv_count, T* __restrict__ dz, int64_t P, int C) {
-    constexpr int ROWS = 256 / G;
-    const int sub = threadIdx.x % G;
-    const float scale = gloss ? gloss[0] * inv_count[0] : 1.f;
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; row < P; row += (int64_t)gridDim.x * ROWS) {
-        const T* zr = z + row * ld;
-        T* dr = dz + row * C;
-        const int64_t a = label[row];
-        const bool valid = a != ignore && a >= 0 && a < C;
-        const float2 st = stats[row];
-        const float gr = valid ? g[row] * scale : 0.f;
-        for (int c0 = sub * V; c0 < C; c0 += G * V * LP_HELD) {
-            float x[LP_HELD][V];
-#pragma unroll
-            for (int u = 0; u < LP_HELD; ++u) {
-                const int c = c0 + u * (G * V);
-                if (c + V <= C) {
-                    load_vec<T, V>(zr + c, x[u]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) x[u][j] = c + j < C ? (float)zr[c + j] : 0.f;
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < LP_HELD; ++u) {
-                const int c = c0 + u * (G * V);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float p = __expf((x[u][j] - st.x) - st.y);
-                    x[u][j] = valid ? gr * ((c + j == (int)a ? 1.f : 0.f) - p) : 0.f;
-                }
-                if (c + V <= C) {
-                    store_vec<T, V>(dr + c, x[u]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        if (c + j < C) dr[c + j] = (T)x[u][j];
-                }
-            }
-        }
-    }
-}
-
 // ---------------------------------------------------------------- host ---------------------------------------------------------
-// lanes of a row: the fewest of 1, 4, 16, 64, 256 that hold it in LP_HELD vectors each; a longer row is walked by a block
-static int group_of(int C, int V) {
-    for (int g = 1; g < 256; g *= 4)
-        if ((int64_t)g * V * LP_HELD >= C) return g;
-    return 256;
-}
-// elements of a load: the widest that every row start (and, for the gradient, every row of dz) is aligned to
-static int vec_of(int bytes, const void* z, int64_t ld, const void* dz, int C) {
-    for (int v = 16 / bytes; v > 1; v >>= (bytes == 2 && v == 8 ? 2 : 1)) {
-        const int64_t a = (int64_t)v * bytes;
-        if (((uintptr_t)z % a) == 0 && (ld * bytes) % a == 0 && (!dz || (((uintptr_t)dz % a) == 0 && ((int64_t)C * bytes) % a == 0))) return v;
-    }
-    return 1;
-}
-static int lp_blocks(int64_t P, int G, int cap) {
-    const int64_t b = (P + 256 / G - 1) / (256 / G);
-    return (int)(b < cap ? b : cap);
-}
+static int bytes_of(int type) { return type == SEMSEG_TYPE_F32 ? 4 : 2; }
 
-struct LpCall {
-    const void* z; int64_t ld; const int64_t* label; int64_t ignore; int64_t P; int C; float2* stats; hipStream_t st;
-    // forward
-    float* lp; const PolicyArgs* pa; void* grad; const int* counts;
-    // backward
-    const float* g; const float* gloss; const float* inv_count; void* dz;
+// how a call's rows are laid out over lanes and blocks; one rule for the kernels and for the scratch that they need
+struct Plan {
+    int lanes;          // of a row in the tile kernel; 0: not a tile
+    int group;          // else lanes of a row: 16, 64, 256
+    int splits, per;    // blocks of a row, and classes of each
+    int64_t blocks;     // of the grid's first axis without a limit
+};
+static Plan plan_of(int bytes, int64_t ld, int64_t P, int C) {
+    Plan p{0, 0, 1, C, 0};
+    if (P == 1) ld = C;
+    // a tile reads the padding between rows too: up to a quarter of a row
+    for (int l = 1; l <= 16 && !p.lanes && ld <= C + C / 4; l *= 2)
+        if ((256 / l) * ld * bytes <= TILE_BYTES) p.lanes = l;
+    if (p.lanes) {
+        p.blocks = (P + 256 / p.lanes - 1) / (256 / p.lanes);
+        return p;
+    }
+    const int V = 16 / bytes;
+    p.group = C <= 16 * V * 4 ? 16 : C <= 64 * V * 8 ? 64 : 256;
+    p.blocks = (P + 256 / p.group - 1) / (256 / p.group);
+    if (p.group == 256 && P < 512) {                         // fewer blocks than the 1024 that fill the chip: several of a row
+        const int step = 256 * V * 4;
+        const int64_t parts = ((int64_t)C + step - 1) / step;
+        int64_t s = (1024 + P - 1) / P;
+        if (s > MAX_SPLITS) s = MAX_SPLITS;
+        if (s > parts) s = parts;
+        p.per = (int)((parts + s - 1) / s) * step;
+        p.splits = (int)(((int64_t)C + p.per - 1) / p.per);
+        if (p.splits == 1) p.per = C;
+    }
+    return p;
+}
+static size_t split_bytes(const Plan& p, int64_t P) { return p.splits > 1 ? (size_t)P * p.splits * sizeof(float2) : 0; }
+
+struct Call {
+    const void* z;
+    Rows r;
+    Plan p;
+    int mode;
+    ForwardArgs f;
+    BackArgs k;
+    void* dz;
+    float2* parts;
+    int grid;           // blocks of the kernel that leaves the partial sums of the loss
+    hipStream_t st;
 };
 
-template <class T, int G, int V>
-static int lp_launch(const LpCall& c) {
-    if (c.dz) {
-        auto k = label_logp_bwd_kernel<T, G, V>;
-        hipLaunchKernelGGL(k, dim3(lp_blocks(c.P, G, 1 << 20)), dim3(256), 0, c.st, (const T*)c.z, c.ld, c.label, c.ignore,
-                           (const float2*)c.stats, c.g, c.gloss, c.inv_count, (T*)c.dz, c.P, c.C);
-    } else if (c.pa) {
-        auto k = label_logp_kernel<T, G, V, true>;
-        hipLaunchKernelGGL(k, dim3(lp_blocks(c.P, G, LP_MAX_BLOCKS)), dim3(256), 0, c.st, (const T*)c.z, c.ld, c.label, c.ignore, c.P, c.C,
-                           (float*)nullptr, c.stats, *c.pa);
-    } else {
-        auto k = label_logp_kernel<T, G, V, false>;
-        hipLaunchKernelGGL(k, dim3(lp_blocks(c.P, G, 1 << 20)), dim3(256), 0, c.st, (const T*)c.z, c.ld, c.label, c.ignore, c.P, c.C, c.lp,
-                           c.stats, PolicyArgs{});
-    }
-    SEMSEG_LAUNCH_CHECK();
-    return 0;
-}
-template <class T, int V>
-static int lp_group(const LpCall& c, int G) {
-    switch (G) {
-        case 1: return lp_launch<T, 1, V>(c);
-        case 4: return lp_launch<T, 4, V>(c);
-        case 16: return lp_launch<T, 16, V>(c);
-        case 64: return lp_launch<T, 64, V>(c);
-        default: return lp_launch<T, 256, V>(c);
-    }
-}
-// lanes of a row in the tile kernel: the fewest whose rows fit the tile; 0: rows too long, not dense or not aligned
-static int tile_lanes(int bytes, const void* z, int64_t ld, int64_t P, int C) {
-    if ((ld != C && P > 1) || !aligned16(z)) return 0;
-    for (int l = 1; l <= 16; l *= 2)
-        if ((int64_t)(256 / l) * C * bytes <= TILE_BYTES) return l;
-    return 0;
-}
-template <class T, int L, int W>
-static int tile_launch(const LpCall& c) {
-    const int64_t tiles = (c.P + 256 / L - 1) / (256 / L);
-    const dim3 grid((unsigned)(tiles < LP_MAX_BLOCKS ? tiles : LP_MAX_BLOCKS)), block(256);
+template <class T, int L, int W, int HELD>
+static void tile_launch(Call& c) {
+    c.grid = (int)(c.p.blocks < LP_MAX_BLOCKS ? c.p.blocks : LP_MAX_BLOCKS);
     const T* z = (const T*)c.z;
-    if (c.grad) {
-        if constexpr (sizeof(T) == 4) {
-            auto k = label_logp_tile_kernel<T, L, W, true, true>;
-            hipLaunchKernelGGL(k, grid, block, 0, c.st, z, c.label, c.ignore, c.P, c.C, (float*)nullptr, c.stats, *c.pa, c.counts, (T*)c.grad);
-        }
-    } else if (c.pa) {
-        auto k = label_logp_tile_kernel<T, L, W, true, false>;
-        hipLaunchKernelGGL(k, grid, block, 0, c.st, z, c.label, c.ignore, c.P, c.C, (float*)nullptr, c.stats, *c.pa, (const int*)nullptr,
-                           (T*)nullptr);
-    } else {
-        auto k = label_logp_tile_kernel<T, L, W, false, false>;
-        hipLaunchKernelGGL(k, grid, block, 0, c.st, z, c.label, c.ignore, c.P, c.C, c.lp, c.stats, PolicyArgs{}, (const int*)nullptr,
-                           (T*)nullptr);
+    const dim3 grid(c.grid), block(256);
+    if (c.mode == LOGP) {
+        auto k = logp_tile_kernel<T, L, W, HELD, LOGP>;
+        hipLaunchKernelGGL(k, grid, block, 0, c.st, z, c.r, c.f, c.k, (T*)nullptr);
+    } else if (c.mode == LOSS) {
+        auto k = logp_tile_kernel<T, L, W, HELD, LOSS>;
+        hipLaunchKernelGGL(k, grid, block, 0, c.st, z, c.r, c.f, c.k, (T*)nullptr);
+    } else if (c.mode == BACK) {
+        auto k = logp_tile_kernel<T, L, W, HELD, BACK>;
+        hipLaunchKernelGGL(k, grid, block, 0, c.st, z, c.r, c.f, c.k, (T*)c.dz);
+    } else if constexpr (sizeof(T) == 4) {
+        auto k = logp_tile_kernel<T, L, W, HELD, GRAD>;
+        hipLaunchKernelGGL(k, grid, block, 0, c.st, z, c.r, c.f, c.k, (T*)c.dz);
     }
-    SEMSEG_LAUNCH_CHECK();
-    return 0;
+}
+// elements that a lane holds: what the tile has for it (L doubles from there on, so more than half are used), fewer for few classes
+template <class T, int L, int W>
+static void tile_held(Call& c) {
+    constexpr int MOST = TILE_BYTES / 256 / (int)sizeof(T);
+    if constexpr (L == 1) {
+        if (c.r.C <= 8) return tile_launch<T, L, W, 8 / W>(c);
+        if constexpr (MOST > 20) {
+            if (c.r.C <= 20) return tile_launch<T, L, W, 20 / W>(c);
+        }
+    }
+    tile_launch<T, L, W, MOST / W>(c);
+}
+template <class T, int L>
+static void tile_wide(Call& c) {
+    if (c.r.C % 2 == 0 && c.r.ld % 2 == 0) tile_held<T, L, 2>(c);
+    else tile_held<T, L, 1>(c);
+}
+template <class T, int G, int H>
+static void rows_launch(Call& c) {
+    const T* z = (const T*)c.z;
+    const dim3 block(256);
+    if (c.mode == BACK) {
+        const int64_t most = 1 << 20;
+        auto k = logp_rows_bwd_kernel<T, G, H>;
+        hipLaunchKernelGGL(k, dim3((unsigned)(c.p.blocks < most ? c.p.blocks : most), c.p.splits), block, 0, c.st, z, c.r, c.k, c.p.per, (T*)c.dz);
+        return;
+    }
+    if (c.p.splits > 1) {
+        auto k = logp_split_kernel<T>;
+        hipLaunchKernelGGL(k, dim3((unsigned)c.r.P, c.p.splits), block, 0, c.st, z, c.r, c.p.per, c.parts);
+        c.grid = (int)((c.r.P + 3) / 4);
+        if (c.mode == LOGP) {
+            auto j = join_rows_kernel<T, LOGP>;
+            hipLaunchKernelGGL(j, dim3(c.grid), block, 0, c.st, z, c.r, c.f, (const float2*)c.parts, c.p.splits);
+        } else {
+            auto j = join_rows_kernel<T, LOSS>;
+            hipLaunchKernelGGL(j, dim3(c.grid), block, 0, c.st, z, c.r, c.f, (const float2*)c.parts, c.p.splits);
+        }
+        return;
+    }
+    if (c.mode == LOGP) {
+        const int64_t most = 1 << 20;
+        auto k = logp_rows_kernel<T, G, H, LOGP>;
+        hipLaunchKernelGGL(k, dim3((unsigned)(c.p.blocks < most ? c.p.blocks : most)), block, 0, c.st, z, c.r, c.f);
+    } else {
+        c.grid = (int)(c.p.blocks < LP_MAX_BLOCKS ? c.p.blocks : LP_MAX_BLOCKS);
+        auto k = logp_rows_kernel<T, G, H, LOSS>;
+        hipLaunchKernelGGL(k, dim3(c.grid), block, 0, c.st, z, c.r, c.f);
+    }
 }
 template <class T>
-static int lp_typed(const LpCall& c) {
-    if (!c.dz) {
-        switch (tile_lanes((int)sizeof(T), c.z, c.ld, c.P, c.C)) {
-            case 1: return c.C % 2 ? tile_launch<T, 1, 1>(c) : tile_launch<T, 1, 2>(c);
-            case 2: return c.C % 2 ? tile_launch<T, 2, 1>(c) : tile_launch<T, 2, 2>(c);
-            case 4: return c.C % 2 ? tile_launch<T, 4, 1>(c) : tile_launch<T, 4, 2>(c);
-            case 8: return c.C % 2 ? tile_launch<T, 8, 1>(c) : tile_launch<T, 8, 2>(c);
-            case 16: return c.C % 2 ? tile_launch<T, 16, 1>(c) : tile_launch<T, 16, 2>(c);
-            default: break;
-        }
+static int typed(Call& c) {
+    switch (c.p.lanes) {
+        case 1: tile_wide<T, 1>(c); break;
+        case 2: tile_wide<T, 2>(c); break;
+        case 4: tile_wide<T, 4>(c); break;
+        case 8: tile_wide<T, 8>(c); break;
+        case 16: tile_wide<T, 16>(c); break;
+        default:
+            if (c.p.group == 16) rows_launch<T, 16, 4>(c);
+            else if (c.p.group == 64 && c.r.C <= 64 * 4 * (16 / (int)sizeof(T))) rows_launch<T, 64, 4>(c);
+            else if (c.p.group == 64) rows_launch<T, 64, 8>(c);
+            else rows_launch<T, 256, 4>(c);
     }
-    const int V = vec_of((int)sizeof(T), c.z, c.ld, c.dz, c.C);
-    const int G = group_of(c.C, V);
-    if constexpr (sizeof(T) == 4) {
-        return V == 4 ? lp_group<T, 4>(c, G) : V == 2 ? lp_group<T, 2>(c, G) : lp_group<T, 1>(c, G);
-    } else {
-        return V == 8 ? lp_group<T, 8>(c, G) : V == 2 ? lp_group<T, 2>(c, G) : lp_group<T, 1>(c, G);
-    }
+    SEMSEG_LAUNCH_CHECK();
+    return 0;
 }
-static int lp_dispatch(const LpCall& c, int type) {
-    if (type == SEMSEG_TYPE_F32) return lp_typed<float>(c);
-    if (type == SEMSEG_TYPE_BF16) return lp_typed<bf16_t>(c);
-    if (type == SEMSEG_TYPE_F16) return lp_typed<f16_t>(c);
-    return SEMSEG_EINVAL;
+static int dispatch(Call& c, int type) {
+    if (type == SEMSEG_TYPE_F32) return typed<float>(c);
+    if (type == SEMSEG_TYPE_BF16) return typed<bf16_t>(c);
+    return typed<f16_t>(c);
 }
-static bool lp_ok(const void* z, int64_t ld, const int64_t* label, int64_t P, int C) {
-    return z && label && P > 0 && P <= (int64_t)1 << 40 && C > 0 && C <= 1 << 30 && ld >= C && (P == 1 || ld <= INT64_MAX / 8 / P);
+static bool call_ok(const void* z, int type, int64_t ld, const int64_t* label, int64_t P, int C) {
+    return z && label && (type == SEMSEG_TYPE_F32 || type == SEMSEG_TYPE_BF16 || type == SEMSEG_TYPE_F16) && P > 0 && P <= (int64_t)1 << 40 &&
+           C > 0 && C <= 1 << 30 && ld >= C && (P == 1 || ld <= INT64_MAX / 8 / P);
+}
+static Call call_of(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore, int64_t P, int C, int mode, void* stream) {
+    Call c{};
+    c.z = z;
+    c.r = Rows{P == 1 ? (int64_t)C : ld, ignore, P, label, C};
+    c.p = plan_of(bytes_of(type), ld, P, C);
+    c.mode = mode;
+    c.st = (hipStream_t)stream;
+    return c;
+}
+
+extern "C" size_t semseg_label_logp_workspace_bytes(int type, int64_t ld, int64_t P, int C) {
+    return P > 0 && C > 0 ? split_bytes(plan_of(bytes_of(type), ld, P, C), P) : 0;
 }
 
 extern "C" int semseg_label_logp_fwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, int64_t P, int C,
-                                     float* lp, float* stats, void* stream) {
-    if (!lp_ok(z, ld, label, P, C) || !lp) return SEMSEG_EINVAL;
-    LpCall c{};
-    c.z = z; c.ld = ld; c.label = label; c.ignore = ignore_index; c.P = P; c.C = C; c.stats = (float2*)stats; c.st = (hipStream_t)stream;
-    c.lp = lp;
-    return lp_dispatch(c, type);
+                                     float* lp, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!call_ok(z, type, ld, label, P, C) || !lp) return SEMSEG_EINVAL;
+    Call c = call_of(z, type, ld, label, ignore_index, P, C, LOGP, stream);
+    const size_t need = split_bytes(c.p, P);
+    if (need && (!workspace || workspace_bytes < need)) return SEMSEG_EWORKSPACE;
+    c.parts = (float2*)workspace;
+    c.f.lp = lp;
+    c.f.stats = (float2*)stats;
+    return dispatch(c, type);
 }
 
-extern "C" size_t semseg_policy_loss_workspace_bytes(void) { return (size_t)LP_MAX_BLOCKS * 4 * sizeof(double) + COUNT_BLOCKS * sizeof(int); }
+// workspace: partial sums of the loss, counts of rows, parts of split rows
+constexpr size_t PARTIAL_BYTES = (size_t)LP_MAX_BLOCKS * 4 * sizeof(double);
+extern "C" size_t semseg_policy_loss_workspace_bytes(int type, int64_t ld, int64_t P, int C) {
+    return PARTIAL_BYTES + COUNT_BLOCKS * sizeof(int) + semseg_label_logp_workspace_bytes(type, ld, P, C);
+}
 
 // Whether a loss whose gradient is wanted writes it in its forward pass.  float32 only: an upstream gradient other than 1 multiplies the
 // written values, and 16-bit ones would be rounded twice.  From 8 classes on: counting the rows first costs 8 bytes a row, reading the
@@ -555,7 +684,7 @@ extern "C" size_t semseg_policy_loss_workspace_bytes(void) { return (size_t)LP_M
 // 2000000 x 2 49.4 against 54.5.
 constexpr int ONE_PASS_CLASSES = 8;
 static bool one_pass_able(const void* z, int type, int64_t ld, int64_t P, int C) {
-    return z && type == SEMSEG_TYPE_F32 && P > 0 && P <= 1 << 30 && C > 0 && tile_lanes(4, z, ld, P, C) > 0;
+    return z && type == SEMSEG_TYPE_F32 && P > 0 && P <= 1 << 30 && C > 0 && ld >= C && plan_of(4, ld, P, C).lanes > 0;
 }
 extern "C" int semseg_policy_loss_one_pass(const void* z, int type, int64_t ld, int64_t P, int C) {
     return one_pass_able(z, type, ld, P, C) && C >= ONE_PASS_CLASSES;
@@ -573,30 +702,29 @@ extern "C" int semseg_policy_loss_fwd(const void* z, int type, int64_t ld, const
                                       const float* advantage, int64_t rows_per_advantage, const float* old_logp, const float* ref_logp,
                                       float clip_low, float clip_high, float kl_weight, float* stats, float* coef, float* loss, float* kl,
                                       float* clipped, float* inv_count, void* dz, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!lp_ok(z, ld, label, P, C) || !advantage || rows_per_advantage <= 0 || !old_logp || !stats || !coef || !loss || !kl || !clipped || !inv_count ||
-        !(clip_low >= 0.f && clip_low <= 1.f) || !(clip_high >= 0.f) || !(kl_weight >= 0.f) || (kl_weight > 0.f && !ref_logp))
+    if (!call_ok(z, type, ld, label, P, C) || !advantage || rows_per_advantage <= 0 || !old_logp || !stats || !coef || !loss || !kl ||
+        !clipped || !inv_count || !(clip_low >= 0.f && clip_low <= 1.f) || !(clip_high >= 0.f) || !(kl_weight >= 0.f) ||
+        (kl_weight > 0.f && !ref_logp) || (dz && (!one_pass_able(z, type, ld, P, C) || !aligned16(dz))))
         return SEMSEG_EINVAL;
-    if (!workspace || workspace_bytes < semseg_policy_loss_workspace_bytes()) return SEMSEG_EWORKSPACE;
-    PolicyArgs pa{};
-    pa.advantage = advantage; pa.old_logp = old_logp; pa.ref_logp = ref_logp; pa.rows_per_advantage = rows_per_advantage;
-    pa.small_rows = P <= (int64_t)1 << 31 && rows_per_advantage <= (int64_t)1 << 31;
-    pa.clip_low = clip_low; pa.clip_high = clip_high; pa.kl_weight = kl_weight; pa.coef = coef; pa.partial = (double*)workspace;
-    LpCall c{};
-    c.z = z; c.ld = ld; c.label = label; c.ignore = ignore_index; c.P = P; c.C = C; c.stats = (float2*)stats; c.st = (hipStream_t)stream;
-    c.pa = &pa;
+    if (!workspace || workspace_bytes < semseg_policy_loss_workspace_bytes(type, ld, P, C) || !aligned16(workspace)) return SEMSEG_EWORKSPACE;
+    Call c = call_of(z, type, ld, label, ignore_index, P, C, dz ? GRAD : LOSS, stream);
+    int* counts = (int*)((char*)workspace + PARTIAL_BYTES);
+    c.parts = (float2*)((char*)workspace + PARTIAL_BYTES + COUNT_BLOCKS * sizeof(int));
+    c.dz = dz;
+    ForwardArgs& f = c.f;
+    f.stats = (float2*)stats;
+    f.advantage = advantage; f.old_logp = old_logp; f.ref_logp = ref_logp; f.rows_per_advantage = rows_per_advantage;
+    f.small_rows = P <= (int64_t)1 << 31 && rows_per_advantage <= (int64_t)1 << 31;
+    f.clip_low = clip_low; f.clip_high = clip_high; f.kl_weight = kl_weight;
+    f.coef = coef;
+    f.partial = (double*)workspace;
+    f.counts = counts;
     if (dz) {
-        if (!one_pass_able(z, type, ld, P, C) || !aligned16(dz)) return SEMSEG_EINVAL;
-        int* counts = (int*)((char*)workspace + (size_t)LP_MAX_BLOCKS * 4 * sizeof(double));
-        hipLaunchKernelGGL(count_rows_kernel, dim3(COUNT_BLOCKS), dim3(256), 0, c.st, label, ignore_index, P, C, counts);
+        hipLaunchKernelGGL(count_rows_kernel, dim3(COUNT_BLOCKS), dim3(256), 0, c.st, c.r, counts);
         SEMSEG_LAUNCH_CHECK();
-        c.grad = dz;
-        c.counts = counts;
     }
-    if (int rc = lp_dispatch(c, type)) return rc;
-    const int bytes = type == SEMSEG_TYPE_F32 ? 4 : 2;
-    const int l = tile_lanes(bytes, z, ld, P, C);
-    const int blocks = lp_blocks(P, l ? l : group_of(C, vec_of(bytes, z, ld, nullptr, C)), LP_MAX_BLOCKS);
-    hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(256), 0, c.st, (const double*)workspace, blocks,
+    if (int rc = dispatch(c, type)) return rc;
+    hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(256), 0, c.st, (const double*)workspace, c.grid,
                        PolicyOut{{loss, kl, clipped, inv_count}});
     SEMSEG_LAUNCH_CHECK();
     return 0;
@@ -604,9 +732,9 @@ extern "C" int semseg_policy_loss_fwd(const void* z, int type, int64_t ld, const
 
 extern "C" int semseg_label_logp_bwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, const float* stats,
                                      const float* g, const float* gloss, const float* inv_count, int64_t P, int C, void* dz, void* stream) {
-    if (!lp_ok(z, ld, label, P, C) || !stats || !g || !dz || (gloss && !inv_count)) return SEMSEG_EINVAL;
-    LpCall c{};
-    c.z = z; c.ld = ld; c.label = label; c.ignore = ignore_index; c.P = P; c.C = C; c.stats = (float2*)stats; c.st = (hipStream_t)stream;
-    c.g = g; c.gloss = gloss; c.inv_count = inv_count; c.dz = dz;
-    return lp_dispatch(c, type);
+    if (!call_ok(z, type, ld, label, P, C) || !stats || !g || !dz || !aligned16(dz) || (gloss && !inv_count)) return SEMSEG_EINVAL;
+    Call c = call_of(z, type, ld, label, ignore_index, P, C, BACK, stream);
+    c.k = BackArgs{(const float2*)stats, g, gloss, inv_count};
+    c.dz = dz;
+    return dispatch(c, type);
 }

@@ -170,8 +170,9 @@ SIGNATURES = {
     'semseg_adamw8_step': (c_int, [vp, c_int, vp, c_d, c_d, c_d, c_f, vp, ctypes.c_uint32, vp, c_sz, vp]),
     'semseg_grad_norm_workspace_bytes': (c_sz, [vp, c_int]),
     'semseg_grad_norm': (c_int, [vp, c_int, c_f, c_f, vp, vp, c_sz, vp]),
-    'semseg_label_logp_fwd': (c_int, [vp, c_int, c_l, vp, c_l, c_l, c_int, vp, vp, vp]),
-    'semseg_policy_loss_workspace_bytes': (c_sz, []),
+    'semseg_label_logp_workspace_bytes': (c_sz, [c_int, c_l, c_l, c_int]),
+    'semseg_label_logp_fwd': (c_int, [vp, c_int, c_l, vp, c_l, c_l, c_int, vp, vp, vp, c_sz, vp]),
+    'semseg_policy_loss_workspace_bytes': (c_sz, [c_int, c_l, c_l, c_int]),
     'semseg_policy_loss_fwd': (c_int, [vp, c_int, c_l, vp, c_l, c_l, c_int, vp, c_l, vp, vp, c_f, c_f, c_f] + [vp] * 8 + [c_sz, vp]),
     'semseg_policy_loss_one_pass': (c_int, [vp, c_int, c_l, c_l, c_int]),
     'semseg_scale_by': (c_int, [vp, c_l, vp, vp]),

@@ -2395,9 +2395,12 @@ class LabelLogProbFn(Function):
         lp = torch.empty(rows, device=z.device, dtype=torch.float32)
         stats = torch.empty(2 * P, device=z.device, dtype=torch.float32) if wanted else None
         if P:
+            L, code = _native.lib(), _TYPE_CODES[z.dtype]
+            need = L.semseg_label_logp_workspace_bytes(code, ld, P, c)
+            ws = torch.empty(need, device=z.device, dtype=torch.uint8) if need else None
             with _device_guard(z.device):
-                _native.check(_native.lib().semseg_label_logp_fwd(z.data_ptr(), _TYPE_CODES[z.dtype], ld, label.data_ptr(), ignore_index, P,
-                                                                  c, lp.data_ptr(), _p(stats), _st()), 'label_logp_fwd')
+                _native.check(L.semseg_label_logp_fwd(z.data_ptr(), code, ld, label.data_ptr(), ignore_index, P, c, lp.data_ptr(), _p(stats),
+                                                      _p(ws), need, _st()), 'label_logp_fwd')
         if stats is not None:
             ctx.save_for_backward(z, label, stats)
             ctx.cfg = (ld, shape, ignore_index)
@@ -2456,7 +2459,7 @@ class PolicyLossFn(Function):
             L = _native.lib()
             # one buffer of its own (the caching allocator orders its reuse by stream and by captured graph): what the backward pass
             # reads -- maximum and logarithm of the sum per row, gradient per row, 1 / rows that count -- and the partial sums
-            scratch = L.semseg_policy_loss_workspace_bytes()
+            scratch = L.semseg_policy_loss_workspace_bytes(_TYPE_CODES[z.dtype], ld, P, c)
             kept = torch.empty(scratch // 4 + 3 * P + 1, device=dev, dtype=torch.float32)
             ws = kept.data_ptr()
             stats = ws + scratch

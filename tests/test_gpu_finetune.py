@@ -39,6 +39,9 @@ def make_logits(shape, dtype, layout, gen, scale=3.0):
     z = (torch.randn(shape, generator=gen) * scale).to(dev(), dtype)
     if layout == 'nchw':
         return z.contiguous()
+    if layout == 'apart':                                            # pixels of a much wider buffer
+        buf = torch.zeros(n, h, w, 3 * c, device=dev(), dtype=dtype)
+        return buf[..., 1:1 + c].permute(0, 3, 1, 2).copy_(z)
     if layout == 'nhwc':
         return z.contiguous(memory_format=torch.channels_last) if c > 1 else z
     pad = {'slice': 7, 'slice8': 8}[layout]
@@ -106,7 +109,11 @@ ROW_CASES = [((1, 1, 1, 1), 'nhwc'), ((1, 2, 1, 1), 'nhwc'), ((2, 3, 5, 7), 'nhw
              ((1, 129, 16, 16), 'slice'), ((2, 513, 3, 5), 'nhwc'), ((1, 1000, 5, 5), 'slice8'), ((1, 8, 40, 50), 'nhwc'),
              ((1, 9, 40, 50), 'nhwc'), ((1, 33, 1, 700), 'rows'), ((1, 150, 3, 70), 'rows_slice'), ((1, 150, 3, 70), 'rows_t'),
              ((1, 2049, 1, 67), 'rows'), ((1, 4096, 1, 5), 'rows'), ((1, 50001, 1, 3), 'rows'), ((1, 131072, 1, 1), 'rows_slice'),
-             ((1, 1, 3, 50), 'rows_slice'), ((4, 21, 130, 131), 'nhwc')]
+             ((1, 1, 3, 50), 'rows_slice'), ((4, 21, 130, 131), 'nhwc'),
+             # rows far apart (16 lanes a row), the lengths around which the number of lanes and of loads changes, few long rows
+             ((1, 2, 5, 70), 'slice8'), ((1, 31, 9, 41), 'slice8'), ((1, 250, 3, 37), 'apart'), ((1, 300, 3, 37), 'apart'), ((1, 320, 7, 11), 'rows'),
+             ((1, 321, 7, 11), 'rows'), ((1, 641, 7, 11), 'rows_slice'), ((1, 1024, 7, 11), 'rows'), ((1, 1027, 7, 11), 'rows_slice'),
+             ((1, 2047, 5, 7), 'rows_slice'), ((1, 4097, 5, 7), 'rows_slice'), ((1, 8191, 1, 2), 'rows'), ((1, 32003, 1, 511), 'rows')]
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=str)
