@@ -11,8 +11,9 @@ CSRC = os.path.join(HERE, 'csrc')
 OUT_DIR = os.path.join(HERE, 'mit_semseg', '_native')
 LIB = os.path.join(OUT_DIR, 'libsemseg_hip.so')
 SOURCES = ['conv_igemm.hip', 'conv_wgrad.hip', 'conv_split.hip', 'weights_prep.hip', 'winograd.hip', 'bn.hip', 'pool_resize.hip', 'head.hip', 'adamw.hip', 'policy.hip', 'input_pipeline.hip', 'depthwise.hip', 'grouped.hip', 'comm.hip', 'peer.hip', 'probe.hip', 'batch.hip', 'api.hip']
-HOST_SRC = os.path.join(CSRC, 'host_table.cpp')      # CPython extension (host code only): tensor lists -> descriptor tables
+HOST_SRC = os.path.join(CSRC, 'host_ext.cpp')      # CPython extension (host code only): tables of tensor lists, backward node of the row losses
 HOST_LIB = os.path.join(OUT_DIR, '_host.so')
+ROCM = os.environ.get('ROCM_PATH', '/opt/rocm')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-I' + os.path.join(ROOT, 'include'), '-I' + CSRC,
          '-Wno-unused-result',
@@ -31,9 +32,9 @@ def _host_command(out, depfile):
     base = os.path.join(os.path.dirname(torch.__file__), 'include')
     return ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-D_GLIBCXX_USE_CXX11_ABI=%d' % int(torch._C._GLIBCXX_USE_CXX11_ABI),
             '-I' + os.path.join(ROOT, 'include'), '-isystem', base, '-isystem', os.path.join(base, 'torch', 'csrc', 'api', 'include'),
-            '-isystem', sysconfig.get_paths()['include'], '-MMD', '-MF', depfile, HOST_SRC, '-o', out,
+            '-isystem', sysconfig.get_paths()['include'], '-isystem', os.path.join(ROCM, 'include'), '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM', '-MMD', '-MF', depfile, HOST_SRC, '-o', out,
             # torch is imported first and has these loaded; named here so that the loader takes their symbols
-            '-L' + os.path.join(os.path.dirname(torch.__file__), 'lib'), '-ltorch_python', '-ltorch_cpu', '-lc10']
+            '-L' + os.path.join(os.path.dirname(torch.__file__), 'lib'), '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_hip']
 
 
 def _depfile_deps(depfile):

@@ -1,10 +1,22 @@
-// Host side of the multi-tensor entry points: reads lists of torch tensors, checks them and writes the descriptor tables of
-// include/semseg_hip.h.  An optimiser step over a few hundred tensors asks each of them for its address, type, device, size and
-// layout; from Python that costs about 2 us a tensor (0.48 ms for the 168 tensors of ResNet50dilated + PPM with 8-bit states, twice the
-// time of the kernels), here about 20 ns.  A CPython extension, no kernels and no GPU calls in it: the library that holds those stays a
-// plain C ABI.
+// Host work that Python is too slow for.  A CPython extension, no kernels in it: the library that holds those stays a plain C ABI, whose
+// functions are handed in by address.
+//
+// Tables of the multi-tensor entry points: reads lists of torch tensors, checks them and writes the descriptors of include/semseg_hip.h.
+// An optimiser step over a few hundred tensors asks each of them for its address, type, device, size and layout; from Python that
+// costs about 2 us a tensor (0.48 ms for the 168 tensors of ResNet50dilated + PPM with 8-bit states, twice the time of the kernels), here
+// about 20 ns.
+//
+// The backward node of the per-row losses (label log probability, policy loss): autograd runs it on a thread of its own, where a Python
+// node first has to get the interpreter lock from the thread that waits for it.  Loss and gradient of 2 x 64 x 64 pixels are 14 us of GPU
+// time.
 #include <Python.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <algorithm>
 #include <exception>
@@ -228,7 +240,104 @@ PyObject* grad_table(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
-PyMethodDef methods[] = {{"adamw_table", (PyCFunction)(void*)adamw_table, METH_FASTCALL, nullptr},
+// ---------------------------------------------------------------- backward of the per-row losses -------------------------------
+typedef int (*LogpBackward)(const void*, int, int64_t, const int64_t*, int64_t, const float*, const float*, const float*, const float*, int64_t,
+                            int, void*, void*);
+typedef int (*ScaleBy)(float*, int64_t, const float*, void*);
+
+void* stream_of(const at::Tensor& t) {
+    return t.is_cuda() ? (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream() : nullptr;
+}
+void check(int rc, const char* what) {
+    TORCH_CHECK(rc == 0, what, " failed with code ", rc, rc >= 900 && rc <= 908 ? " (stream capture)" : "");
+}
+
+// d logits of label_log_prob (kept: {maximum, log sum} per row) and of policy_loss (kept: scratch, the same, gradient per row, 1 / rows
+// that count; `written`: the gradient for an upstream gradient of 1, where the forward pass has written it)
+struct RowsBackward : public torch::autograd::Node {
+    torch::autograd::SavedVariable z, label, kept;
+    at::Tensor written;
+    std::vector<int64_t> shape;
+    int64_t ld = 0, ignore = 0;
+    bool loss = false;
+    LogpBackward logp_bwd = nullptr;
+    ScaleBy scale_by = nullptr;
+
+    std::string name() const override { return loss ? "PolicyLossBackward" : "LabelLogProbBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        z.reset_data();
+        label.reset_data();
+        kept.reset_data();
+        written.reset();
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        if (!grads[0].defined()) return {at::Tensor()};
+        at::Tensor zt, lab, keep, dz;
+        {
+            std::lock_guard<std::mutex> lock(mutex_);
+            zt = z.unpack(shared_from_this());
+            lab = label.unpack(shared_from_this());
+            keep = kept.unpack(shared_from_this());
+            std::swap(dz, written);
+        }
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const c10::DeviceGuard guard(zt.device());
+            const at::Tensor g = grads[0].to(at::kFloat).contiguous();
+            const int64_t P = lab.numel();
+            const float* kp = (const float*)keep.const_data_ptr();
+            const float* inv = loss && P ? kp + keep.numel() - 1 : nullptr;
+            const float* coef = loss ? inv - P : nullptr;
+            if (dz.defined()) {                       // handed out once: a second backward pass computes its own
+                check(scale_by((float*)dz.mutable_data_ptr(), dz.numel(), (const float*)g.const_data_ptr(), stream_of(zt)), "scale_by");
+            } else {
+                dz = shape.size() == 2 ? at::empty(shape, zt.options())
+                                       : at::empty({shape[0], shape[2], shape[3], shape[1]}, zt.options()).permute({0, 3, 1, 2});
+                if (P)
+                    check(logp_bwd(zt.const_data_ptr(), type_code(zt), ld, (const int64_t*)lab.const_data_ptr(), ignore,
+                                   loss ? coef - 2 * P : kp, loss ? coef : (const float*)g.const_data_ptr(),
+                                   loss ? (const float*)g.const_data_ptr() : nullptr, inv, P, (int)shape[1], dz.mutable_data_ptr(),
+                                   stream_of(zt)),
+                          "label_logp_bwd");
+            }
+        }
+        if (at::GradMode::is_enabled()) {             // create_graph: the result has no gradient of its own
+            auto refused = std::make_shared<torch::autograd::DelayedError>(name() + ": the gradient cannot be differentiated again", 1);
+            return (*refused)({dz.set_requires_grad(true)});
+        }
+        return {dz};
+    }
+};
+
+// (out, z, z as rows, label, kept, written or None, pitch, ignore_index, loss, address of label_logp_bwd, address of scale_by): `out`
+// becomes differentiable in z
+PyObject* attach_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 11) return PyErr_Format(PyExc_TypeError, "attach_rows: 11 arguments");
+    return guarded([&]() -> PyObject* {
+        const char* what = "attach_rows";
+        const at::Tensor& out = tensor(args[0], what);
+        const at::Tensor& z = tensor(args[1], what);
+        auto node = std::shared_ptr<RowsBackward>(new RowsBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(z));
+        node->shape = z.sizes().vec();
+        node->z = torch::autograd::SavedVariable(tensor(args[2], what), false);
+        node->label = torch::autograd::SavedVariable(tensor(args[3], what), false);
+        node->kept = torch::autograd::SavedVariable(tensor(args[4], what), false);
+        if (args[5] != Py_None) node->written = tensor(args[5], what);
+        node->ld = PyLong_AsLongLong(args[6]);
+        node->ignore = PyLong_AsLongLong(args[7]);
+        node->loss = PyObject_IsTrue(args[8]) == 1;
+        node->logp_bwd = (LogpBackward)PyLong_AsVoidPtr(args[9]);
+        node->scale_by = (ScaleBy)PyLong_AsVoidPtr(args[10]);
+        if (PyErr_Occurred()) throw Refused();
+        torch::autograd::set_history(out, node);
+        Py_RETURN_NONE;
+    });
+}
+
+PyMethodDef methods[] = {{"attach_rows", (PyCFunction)(void*)attach_rows, METH_FASTCALL, nullptr},
+                         {"adamw_table", (PyCFunction)(void*)adamw_table, METH_FASTCALL, nullptr},
                          {"adamw8_table", (PyCFunction)(void*)adamw8_table, METH_FASTCALL, nullptr},
                          {"grad_table", (PyCFunction)(void*)grad_table, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

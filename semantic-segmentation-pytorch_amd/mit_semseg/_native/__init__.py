@@ -238,13 +238,31 @@ def lib():
 
 
 def host():
-    """the CPython extension that turns lists of tensors into descriptor tables (csrc/host_table.cpp); raises if it is not built"""
+    """the CPython extension for host work that Python is too slow for (csrc/host_ext.cpp); raises if it is not built"""
     try:
         from . import _host
     except ImportError as e:
         raise NativeLibraryMissing('%s/_host.so not built or not loadable (%s): run `python '
                                    'semantic-segmentation-pytorch_amd/build_native.py`' % (_HERE, e))
     return _host
+
+
+_addresses = {}
+
+
+def address(name):
+    """where the entry point `name` of lib() starts, for the extension to call; an entry point that is a Python function (a stub of
+    the CPU tests) is wrapped"""
+    fn = getattr(lib(), name)
+    if isinstance(fn, ctypes._CFuncPtr):
+        got = _addresses.get((name, id(_lib)))
+        if got is None:
+            got = _addresses[name, id(_lib)] = ctypes.cast(fn, vp).value
+        return got
+    res, args = SIGNATURES[name]
+    wrapped = ctypes.CFUNCTYPE(res, *args)(fn)
+    _addresses.setdefault('stubs', []).append(wrapped)
+    return ctypes.cast(wrapped, vp).value
 
 
 class NativeError(RuntimeError):

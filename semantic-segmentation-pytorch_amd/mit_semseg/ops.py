@@ -2361,58 +2361,10 @@ def _row_labels(what, z, rows, label):
     return label if label.is_contiguous() else label.contiguous()
 
 
-def _empty_like_rows(z, shape):
-    """the gradient of logits: dense rows, the logits' logical shape"""
-    if len(shape) == 2:
-        return torch.empty(shape, device=z.device, dtype=z.dtype)
-    return empty_nhwc(*shape, z.device, z.dtype)
-
-
-def _label_logp_bwd(z, ld, shape, label, ignore_index, stats, g, gloss, inv_count):
-    """gradient of the logits; stats, g, gloss, inv_count: device addresses"""
-    dz = _empty_like_rows(z, shape)
-    P = label.numel()
-    if P:
-        with _device_guard(z.device):
-            _native.check(_native.lib().semseg_label_logp_bwd(z.data_ptr(), _TYPE_CODES[z.dtype], ld, label.data_ptr(), ignore_index, stats,
-                                                              g, gloss, inv_count, P, shape[1], dz.data_ptr(), _st()), 'label_logp_bwd')
-    return dz
-
-
-def _upstream(g):
-    """an upstream gradient as dense float32"""
-    if g.dtype is not torch.float32:
-        g = g.float()
-    return g if g.is_contiguous() else g.contiguous()
-
-
-class LabelLogProbFn(Function):
-    @staticmethod
-    def forward(ctx, z, label, ignore_index, wanted):
-        shape, rows = tuple(z.shape), _row_shape('label_log_prob', z)
-        label = _row_labels('label_log_prob', z, rows, label)
-        z, ld, P, c = _logit_rows(z)
-        lp = torch.empty(rows, device=z.device, dtype=torch.float32)
-        stats = torch.empty(2 * P, device=z.device, dtype=torch.float32) if wanted else None
-        if P:
-            L, code = _native.lib(), _TYPE_CODES[z.dtype]
-            need = L.semseg_label_logp_workspace_bytes(code, ld, P, c)
-            ws = torch.empty(need, device=z.device, dtype=torch.uint8) if need else None
-            with _device_guard(z.device):
-                _native.check(L.semseg_label_logp_fwd(z.data_ptr(), code, ld, label.data_ptr(), ignore_index, P, c, lp.data_ptr(), _p(stats),
-                                                      _p(ws), need, _st()), 'label_logp_fwd')
-        if stats is not None:
-            ctx.save_for_backward(z, label, stats)
-            ctx.cfg = (ld, shape, ignore_index)
-        return lp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        z, label, stats = ctx.saved_tensors
-        ld, shape, ignore_index = ctx.cfg
-        g = _upstream(g)
-        return _label_logp_bwd(z, ld, shape, label, ignore_index, stats.data_ptr(), g.data_ptr(), 0, 0), None, None, None
+def _differentiable(out, z, zr, label, kept, written, ld, ignore_index, loss):
+    """make `out` differentiable in z: its backward node is the extension's (csrc/host_ext.cpp)"""
+    _native.host().attach_rows(out, z, zr, label, kept, written, ld, ignore_index, loss, _native.address('semseg_label_logp_bwd'),
+                               _native.address('semseg_scale_by'))
 
 
 def label_log_prob(z, label, ignore_index=-1):
@@ -2420,7 +2372,23 @@ def label_log_prob(z, label, ignore_index=-1):
     pixel stride) or [P, C], float32 / bfloat16 / float16; label [N, H, W] or [P], integers.  Returns float32 of the label's shape;
     rows whose label is `ignore_index` or outside [0, C) give 0 and a zero gradient.  Log probabilities are logits too, so the
     output of log_softmax can be handed in.  Differentiable in z."""
-    return LabelLogProbFn.apply(z, label, int(ignore_index), torch.is_grad_enabled() and z.requires_grad)
+    ignore_index = int(ignore_index)
+    rows = _row_shape('label_log_prob', z)
+    label = _row_labels('label_log_prob', z, rows, label)
+    zr, ld, P, c = _logit_rows(z)
+    wanted = torch.is_grad_enabled() and z.requires_grad
+    lp = torch.empty(rows, device=z.device, dtype=torch.float32)
+    stats = torch.empty(2 * P, device=z.device, dtype=torch.float32) if wanted else None
+    if P:
+        L, code = _native.lib(), _TYPE_CODES[z.dtype]
+        need = L.semseg_label_logp_workspace_bytes(code, ld, P, c)
+        ws = torch.empty(need, device=z.device, dtype=torch.uint8) if need else None
+        with _device_guard(z.device):
+            _native.check(L.semseg_label_logp_fwd(zr.data_ptr(), code, ld, label.data_ptr(), ignore_index, P, c, lp.data_ptr(), _p(stats),
+                                                  _p(ws), need, _st()), 'label_logp_fwd')
+    if wanted:
+        _differentiable(lp, z, zr, label, stats, None, ld, ignore_index, False)
+    return lp
 
 
 def _row_constants(what, name, t, shapes, device):
@@ -2436,66 +2404,6 @@ def _row_constants(what, name, t, shapes, device):
     if t.dtype is not torch.float32:
         t = t.float()
     return t if t.is_contiguous() else t.contiguous()
-
-
-class PolicyLossFn(Function):
-    @staticmethod
-    def forward(ctx, z, label, advantage, old_logp, ref_logp, clip_low, clip_high, kl_weight, ignore_index, wanted):
-        what = 'policy_loss'
-        shape, dev, rows = tuple(z.shape), z.device, _row_shape(what, z)
-        label = _row_labels(what, z, rows, label)
-        advantage = _row_constants(what, 'advantage', advantage, ((rows[0],), rows) if len(rows) == 3 else (rows,), dev)
-        old_logp = _row_constants(what, 'old_logp', old_logp, (rows,), dev)
-        if ref_logp is not None:
-            ref_logp = _row_constants(what, 'ref_logp', ref_logp, (rows,), dev)
-        z, ld, P, c = _logit_rows(z)
-        ctx.set_materialize_grads(False)
-        ctx.dz = None
-        if P == 0:
-            loss, kl, clipped = (torch.zeros((), device=dev) for _ in range(3))
-            kept = torch.zeros(1, device=dev)
-        else:
-            loss, kl, clipped = (torch.empty((), device=dev) for _ in range(3))
-            L = _native.lib()
-            # one buffer of its own (the caching allocator orders its reuse by stream and by captured graph): what the backward pass
-            # reads -- maximum and logarithm of the sum per row, gradient per row, 1 / rows that count -- and the partial sums
-            scratch = L.semseg_policy_loss_workspace_bytes(_TYPE_CODES[z.dtype], ld, P, c)
-            kept = torch.empty(scratch // 4 + 3 * P + 1, device=dev, dtype=torch.float32)
-            ws = kept.data_ptr()
-            stats = ws + scratch
-            coef = stats + 8 * P
-            dz = None
-            if wanted and L.semseg_policy_loss_one_pass(z.data_ptr(), _TYPE_CODES[z.dtype], ld, P, c):
-                dz = _empty_like_rows(z, shape)
-            with _device_guard(dev):
-                _native.check(L.semseg_policy_loss_fwd(z.data_ptr(), _TYPE_CODES[z.dtype], ld, label.data_ptr(), ignore_index, P, c,
-                                                       advantage.data_ptr(), P // advantage.numel(), old_logp.data_ptr(), _p(ref_logp),
-                                                       clip_low, clip_high, kl_weight, stats, coef, loss.data_ptr(), kl.data_ptr(),
-                                                       clipped.data_ptr(), coef + 4 * P, _p(dz), ws, scratch, _st()), 'policy_loss_fwd')
-            ctx.dz = dz
-        if wanted:
-            ctx.save_for_backward(z, label, kept)
-            ctx.cfg = (ld, shape, ignore_index)
-        ctx.mark_non_differentiable(kl, clipped)
-        return loss, kl, clipped
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gloss, gkl, gclipped):
-        if gloss is None:
-            return (None,) * 10
-        z, label, kept = ctx.saved_tensors
-        ld, shape, ignore_index = ctx.cfg
-        gloss = _upstream(gloss)
-        dz, ctx.dz = ctx.dz, None
-        if dz is not None:                            # written by the forward pass; handed out once, a second backward computes its own
-            with _device_guard(dz.device):
-                _native.check(_native.lib().semseg_scale_by(dz.data_ptr(), dz.numel(), gloss.data_ptr(), _st()), 'scale_by')
-            return (dz,) + (None,) * 9
-        P = label.numel()
-        inv = kept.data_ptr() + 4 * (kept.numel() - 1)
-        coef = inv - 4 * P
-        return (_label_logp_bwd(z, ld, shape, label, ignore_index, coef - 8 * P, coef, gloss.data_ptr(), inv),) + (None,) * 9
 
 
 def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip_high=0.2, kl_weight=0.0, ignore_index=-1):
@@ -2515,8 +2423,39 @@ def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip
         raise ValueError('policy_loss: kl_weight must not be negative, got %r' % kl_weight)
     if kl_weight > 0.0 and ref_logp is None:
         raise ValueError('policy_loss: a KL term needs ref_logp')
-    return PolicyLossFn.apply(z, label, advantage, old_logp, ref_logp, clip_low, clip_high, kl_weight, int(ignore_index),
-                              torch.is_grad_enabled() and z.requires_grad)
+    ignore_index, what = int(ignore_index), 'policy_loss'
+    dev, rows = z.device, _row_shape(what, z)
+    label = _row_labels(what, z, rows, label)
+    advantage = _row_constants(what, 'advantage', advantage, ((rows[0],), rows) if len(rows) == 3 else (rows,), dev)
+    old_logp = _row_constants(what, 'old_logp', old_logp, (rows,), dev)
+    if ref_logp is not None:
+        ref_logp = _row_constants(what, 'ref_logp', ref_logp, (rows,), dev)
+    zr, ld, P, c = _logit_rows(z)
+    wanted = torch.is_grad_enabled() and z.requires_grad
+    dz = None
+    if P == 0:
+        loss, kl, clipped = (torch.zeros((), device=dev) for _ in range(3))
+        kept = torch.zeros(1, device=dev)
+    else:
+        loss, kl, clipped = (torch.empty((), device=dev, dtype=torch.float32) for _ in range(3))
+        L, code = _native.lib(), _TYPE_CODES[z.dtype]
+        # one buffer of its own (the caching allocator orders its reuse by stream and by captured graph): scratch, then what the backward
+        # pass reads -- maximum and logarithm of the sum per row, gradient per row, 1 / rows that count
+        scratch = L.semseg_policy_loss_workspace_bytes(code, ld, P, c)
+        kept = torch.empty(scratch // 4 + 3 * P + 1, device=dev, dtype=torch.float32)
+        ws = kept.data_ptr()
+        stats = ws + scratch
+        coef = stats + 8 * P
+        if wanted and L.semseg_policy_loss_one_pass(zr.data_ptr(), code, ld, P, c):
+            dz = torch.empty(z.shape, device=dev, dtype=z.dtype) if z.dim() == 2 else empty_nhwc(*z.shape, dev, z.dtype)
+        with _device_guard(dev):
+            _native.check(L.semseg_policy_loss_fwd(zr.data_ptr(), code, ld, label.data_ptr(), ignore_index, P, c, advantage.data_ptr(),
+                                                   P // advantage.numel(), old_logp.data_ptr(), _p(ref_logp), clip_low, clip_high, kl_weight,
+                                                   stats, coef, loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(), coef + 4 * P, _p(dz), ws,
+                                                   scratch, _st()), 'policy_loss_fwd')
+    if wanted:
+        _differentiable(loss, z, zr, label, kept, dz, ld, ignore_index, True)
+    return loss, kl, clipped
 
 
 # ------------------------------------------------------------------------------------------------
@@ -2591,7 +2530,7 @@ AdamW8State = collections.namedtuple('AdamW8State', 'm m_scale r r_scale')
 
 
 def _check_step(what, params, lr_tensor, betas, eps, clip):
-    """the arguments of an AdamW step that are not lists (the lists: csrc/host_table.cpp)"""
+    """the arguments of an AdamW step that are not lists (the lists: csrc/host_ext.cpp)"""
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0) or not 0.0 <= eps < float('inf'):
         raise ValueError('%s: betas must lie in [0, 1) and eps must not be negative, got %r, %r' % (what, betas, eps))

@@ -367,6 +367,36 @@ def test_backward_twice_and_shared_logits():
     assert torch.all((got - want).abs() <= U32 * n * (p * (log_sum_roundings(150) + 60) + 2) + 84 * U32 * n)
 
 
+def test_second_derivatives_are_refused_and_nodes_are_freed():
+    from mit_semseg import ops
+    gen = torch.Generator().manual_seed(10)
+    z, label, adv, old, ref = policy_inputs((2, 150, 6, 7), torch.float32, 'nhwc', gen)
+    for out in (ops.policy_loss(z, label, adv, old)[0], ops.label_log_prob(z, label).sum()):
+        dz = torch.autograd.grad(out, z, create_graph=True)[0]
+        with pytest.raises(RuntimeError, match='differentiated'):
+            torch.autograd.grad(dz.sum(), z)
+    out = ops.label_log_prob(z, label).sum()
+    torch.autograd.grad(out, z)
+    with pytest.raises(RuntimeError, match='second time'):
+        torch.autograd.grad(out, z)
+    del out, dz
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for backward in (True, False) * 5:
+        loss, _, _ = ops.policy_loss(z, label, adv, old)
+        lp = ops.label_log_prob(z, label)
+        if backward:
+            torch.autograd.grad(loss + lp.sum(), z)
+        del loss, lp, _
+    assert torch.cuda.memory_allocated() == before
+    # a leaf's .grad, accumulated
+    leaf = z.detach().clone(memory_format=torch.channels_last).requires_grad_(True)
+    for i in range(2):
+        ops.label_log_prob(leaf, label).sum().backward()
+    want = torch.autograd.grad(ops.label_log_prob(z, label).sum(), z)[0]
+    assert torch.equal(leaf.grad, want + want)
+
+
 # ------------------------------------------------------------------------------------------------------------------- norm
 @pytest.mark.parametrize('sizes', [[1], [3, 5], [16384], [16385, 7], [100001, 64, 1, 4096], [5] * 300], ids=lambda s: str(s[:4]))
 def test_grad_norm(sizes):
