@@ -34,7 +34,7 @@ def _host_command(out, depfile):
             '-I' + os.path.join(ROOT, 'include'), '-isystem', base, '-isystem', os.path.join(base, 'torch', 'csrc', 'api', 'include'),
             '-isystem', sysconfig.get_paths()['include'], '-isystem', os.path.join(ROCM, 'include'), '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM', '-MMD', '-MF', depfile, HOST_SRC, '-o', out,
             # torch is imported first and has these loaded; named here so that the loader takes their symbols
-            '-L' + os.path.join(os.path.dirname(torch.__file__), 'lib'), '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_hip']
+            '-L' + os.path.join(os.path.dirname(torch.__file__), 'lib'), '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_hip', '-lamdhip64']
 
 
 def _depfile_deps(depfile):

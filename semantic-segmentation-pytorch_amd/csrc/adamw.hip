@@ -17,7 +17,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int ADAM_MAX_TENSORS = 1024;     // of one launch of a step
-constexpr int ADAM_CHUNK = 4096;           // elements of a block: 4 quads a thread, all their loads in flight at once
+constexpr int ADAM_CHUNK = 4096;           // elements of a block: 4 quads a thread
 constexpr int ADAM_QUADS = ADAM_CHUNK / (256 * 4);
 
 static bool type_ok(int t) { return t == SEMSEG_TYPE_F32 || t == SEMSEG_TYPE_BF16 || t == SEMSEG_TYPE_F16; }
@@ -132,6 +132,9 @@ static AdamHyper hyper_of(double beta1, double beta2, double eps) {
 }
 
 // ---------------------------------------------------------------- states in 32 bits -------------------------------------------
+// One read and one write of everything, four 16-byte loads of each array under way per thread.  HBM-bound: 62 M elements in 168 tensors,
+// f32 gradients, 327 us = 5.3 TB/s; 112 M elements in 24 tensors, bf16 gradients and copies, 588 us = 5.3 TB/s (a large copy on the same
+// card: 4.9 TB/s).  Roots and divisions are the correctly rounded ones: about 50 instructions an element, a quarter of the time.
 __global__ __launch_bounds__(256) void adamw_kernel(const AdamEntry* __restrict__ table, const uint32_t* __restrict__ first, int n,
                                                     AdamHyper h) {
     const int k = tensor_of(first, n, blockIdx.x);
@@ -315,8 +318,10 @@ extern "C" int semseg_adamw_step(const semseg_adamw_tensor* tensors_host, int n,
 }
 
 // ---------------------------------------------------------------- states in 8 bits --------------------------------------------
-// A wave owns a block of 256 elements (one scale): 4 elements a lane, the block's maxima of |m| and r by shuffles, so the states are
-// read and written once and never leave the registers in between.
+// A wave owns a block of 256 elements (one scale): 4 elements a lane, the block's maxima of |m| and r across the lanes, so the states are
+// read and written once and never leave the registers in between.  62 M elements in 168 tensors, f32 gradients: 186 us = 5.3 TB/s of 16
+// bytes an element; 112 M elements in 24 tensors, bf16 gradients and copies: 338 us = 5.3 TB/s.  With correctly rounded divisions,
+// maxima by shuffles through LDS and codes rounded by bit operations it was bound by instructions (about 120 an element, now 70): 386 us.
 constexpr int ADAM8_PER_WAVE = 4;                                     // blocks of a wave, their loads in flight together
 constexpr int ADAM8_CHUNK = 4 * ADAM8_PER_WAVE * ADAM8_BLOCK;         // elements of a thread block
 
@@ -470,7 +475,8 @@ extern "C" int semseg_adamw8_step(const semseg_adamw8_tensor* tensors_host, int 
 
 // ---------------------------------------------------------------- global norm -------------------------------------------------
 // Squares are summed in 64 bits (an f32 square leaves the range at 2e19 and below 1e-23), one partial sum per chunk in a fixed order,
-// then one block sums the partials: the same bits every time.
+// then one block sums the partials: the same bits every time.  62 M f32 elements 44 us = 5.6 TB/s, 112 M bf16 39 us = 5.8 TB/s, and 4.7
+// us of the second kernel.
 constexpr int NORM_MAX_TENSORS = 196;
 constexpr int NORM_CHUNK = 16384;
 struct NormBatch {

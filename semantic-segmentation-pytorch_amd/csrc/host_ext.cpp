@@ -11,12 +11,14 @@
 // time.
 #include <Python.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <exception>
@@ -78,16 +80,21 @@ bool same_order(const at::Tensor& a, const at::Tensor& b) {
 void* address(const at::Tensor& t) { return const_cast<void*>(t.const_data_ptr()); }
 
 typedef std::vector<std::pair<uintptr_t, uintptr_t>> Ranges;
-void disjoint(Ranges& r, const char* what, const char* name) {
+// what a call writes: no element twice (blocks of two tensors would race)
+void disjoint(Ranges& r, const char* what) {
     std::sort(r.begin(), r.end());
     for (size_t i = 1; i < r.size(); ++i)
-        if (r[i].first < r[i - 1].second) refuse(PyExc_ValueError, "%s: the same %s twice in one call (or overlapping ones)", what, name);
+        if (r[i].first < r[i - 1].second)
+            refuse(PyExc_ValueError, "%s: the same tensor twice among parameters, states, copies and step counts of a call (or overlapping ones)", what);
+}
+void add(Ranges& r, const void* at, int64_t bytes) {
+    if (bytes) r.emplace_back((uintptr_t)at, (uintptr_t)at + (uintptr_t)bytes);
 }
 
 // the part that both AdamW tables share; returns false for a tensor without elements
 template <class ENTRY>
 bool common(ENTRY& e, const char* what, const at::Tensor& p, PyObject* grad, PyObject* step, PyObject* wd, PyObject* copy,
-            const at::Device& dev, Ranges& params, Ranges& steps) {
+            const at::Device& dev, Ranges& written) {
     const at::Tensor& g = tensor(grad, what);
     const at::Tensor& s = tensor(step, what);
     if (p.scalar_type() != at::kFloat)
@@ -117,8 +124,9 @@ bool common(ENTRY& e, const char* what, const at::Tensor& p, PyObject* grad, PyO
     e.weight_decay = (float)decay;
     e.grad_type = type_code(g);
     if (e.numel == 0) return false;
-    params.emplace_back((uintptr_t)e.param, (uintptr_t)e.param + 4 * (uintptr_t)e.numel);
-    steps.emplace_back((uintptr_t)e.step, (uintptr_t)e.step + 4);
+    add(written, e.param, 4 * e.numel);
+    add(written, e.copy, e.copy ? 2 * e.numel : 0);
+    add(written, e.step, 4);
     return true;
 }
 
@@ -140,26 +148,24 @@ PyObject* adam_table(PyObject* const* args, Py_ssize_t n_states, FILL fill) {
     if (!even) refuse(PyExc_ValueError, "%s: the lists differ in length", what);
     std::vector<ENTRY> table;
     table.reserve(n);
-    Ranges param_at, step_at;
-    param_at.reserve(n);
-    step_at.reserve(n);
+    Ranges written;
+    written.reserve(7 * n);
     for (Py_ssize_t i = 0; i < n; ++i) {
         const at::Tensor& p = tensor(params[i], what);
         const at::Device dev = THPVariable_Unpack(params[0]).device();
         ENTRY e{};
-        const bool live = common(e, what, p, grads[i], steps[i], wds[i], copying ? copies[i] : nullptr, dev, param_at, step_at);
-        fill(e, what, p, dev, states, i);
+        const bool live = common(e, what, p, grads[i], steps[i], wds[i], copying ? copies[i] : nullptr, dev, written);
+        fill(e, what, p, dev, states, i, written);
         if (live) table.push_back(e);
     }
-    disjoint(param_at, what, "parameter");
-    disjoint(step_at, what, "step count");
+    disjoint(written, what);
     PyObject* bytes = PyBytes_FromStringAndSize((const char*)table.data(), (Py_ssize_t)(table.size() * sizeof(ENTRY)));
     if (!bytes) throw Refused();
     return Py_BuildValue("Nn", bytes, (Py_ssize_t)table.size());
 }
 
 void fill32(semseg_adamw_tensor& e, const char* what, const at::Tensor& p, const at::Device& dev,
-            const std::vector<std::unique_ptr<Seq>>& states, Py_ssize_t i) {
+            const std::vector<std::unique_ptr<Seq>>& states, Py_ssize_t i, Ranges& written) {
     const at::Tensor& m = tensor((*states[0])[i], what);
     const at::Tensor& v = tensor((*states[1])[i], what);
     if (m.scalar_type() != at::kFloat || v.scalar_type() != at::kFloat || m.device() != dev || v.device() != dev || !same_order(p, m) ||
@@ -168,10 +174,12 @@ void fill32(semseg_adamw_tensor& e, const char* what, const at::Tensor& p, const
                (Py_ssize_t)p.numel());
     e.exp_avg = address(m);
     e.exp_avg_sq = address(v);
+    add(written, e.exp_avg, 4 * p.numel());
+    add(written, e.exp_avg_sq, 4 * p.numel());
 }
 
 void fill8(semseg_adamw8_tensor& e, const char* what, const at::Tensor& p, const at::Device& dev,
-           const std::vector<std::unique_ptr<Seq>>& states, Py_ssize_t i) {
+           const std::vector<std::unique_ptr<Seq>>& states, Py_ssize_t i, Ranges& written) {
     Seq state((*states[0])[i], "expected an AdamW8State");
     const int64_t n = p.numel(), blocks = (n + 255) / 256;
     bool ok = state.size() == 4;
@@ -191,6 +199,10 @@ void fill8(semseg_adamw8_tensor& e, const char* what, const at::Tensor& p, const
     e.m_scales = at_[1];
     e.r_codes = at_[2];
     e.r_scales = at_[3];
+    add(written, e.m_codes, n);
+    add(written, e.r_codes, n);
+    add(written, e.m_scales, 4 * blocks);
+    add(written, e.r_scales, 4 * blocks);
 }
 
 template <class F>
@@ -310,6 +322,19 @@ struct RowsBackward : public torch::autograd::Node {
     }
 };
 
+// Logits that are a leaf keep the node that accumulates their gradient as long as any graph made with them lives, and with it the stream
+// of that graph.  A backward pass that is being captured would draw that stream into the capture, which ends the process here: refused
+// while there is something to refuse.
+void refuse_foreign_leaf(const at::Tensor& z) {
+    if (!z.is_cuda() || z.grad_fn()) return;
+    const auto held = torch::autograd::impl::try_get_grad_accumulator(z);
+    if (!held || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto of = held->stream();
+    if (of && *of != c10::hip::getCurrentHIPStream(z.get_device()).unwrap())
+        refuse(PyExc_RuntimeError, "a backward pass of these logits cannot be captured while a graph that was made with them on another stream "
+               "is alive: drop the earlier loss, or detach() the logits first");
+}
+
 // (out, z, z as rows, label, kept, written or None, pitch, ignore_index, loss, address of label_logp_bwd, address of scale_by): `out`
 // becomes differentiable in z
 PyObject* attach_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -318,6 +343,7 @@ PyObject* attach_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const char* what = "attach_rows";
         const at::Tensor& out = tensor(args[0], what);
         const at::Tensor& z = tensor(args[1], what);
+        refuse_foreign_leaf(z);
         auto node = std::shared_ptr<RowsBackward>(new RowsBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(z));
         node->shape = z.sizes().vec();

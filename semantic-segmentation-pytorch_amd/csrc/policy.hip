@@ -382,7 +382,8 @@ __global__ __launch_bounds__(256) void logp_rows_kernel(const T* __restrict__ z,
     if constexpr (MODE == LOSS) block_partial(acc, f.partial);
 }
 
-// few long rows: block (x, y) sums part y of row x, join_rows_kernel the parts.  A row of 131072 f32 classes by one block: 18 us
+// few long rows: block (x, y) sums part y of row x, join_rows_kernel the parts.  One row of 131072 f32 classes: 18 us by one block, 5.5 us
+// by 32; its gradient 23 and 3 us
 template <class T>
 __global__ __launch_bounds__(256) void logp_split_kernel(const T* __restrict__ z, const Rows r, int per, float2* __restrict__ parts) {
     __shared__ float lds[8];

@@ -154,6 +154,25 @@ def test_adamw_refusals(host, bits):
             host.adamw_step([t(6), t(6)], [t(6), t(6)], [t(6), t(6)], [t(6), t(6)], [s, s], [0.0, 0.0], t(1))
         else:
             host.adamw8_step([t(6), t(6)], [t(6), t(6)], [host.adamw8_state(p) for _ in range(2)], [s, s], [0.0, 0.0], t(1))
+    # the same state, a state that is another's parameter, a copy that overlaps another
+    a, b, w = t(600), t(600), t(1000, dtype=torch.bfloat16)
+    two = dict(steps=list(t(2, dtype=torch.int32).unbind()), weight_decays=[0.0, 0.0], lr_tensor=t(1))
+    with pytest.raises(ValueError, match='twice'):
+        if bits == 32:
+            host.adamw_step([a, b], [t(600), t(600)], [t(600), t(600)], [s2 := t(600), s2], **two)
+        else:
+            st = host.adamw8_state(a)
+            host.adamw8_step([a, b], [t(600), t(600)], [st, host.adamw8_state(b)._replace(r=st.r)], **two)
+    with pytest.raises(ValueError, match='twice'):
+        if bits == 32:
+            host.adamw_step([a, b], [t(600), t(600)], [b, t(600)], [t(600), t(600)], **two)
+        else:
+            host.adamw8_step([a, b], [t(600), t(600)], [host.adamw8_state(a)._replace(m_scale=b[:3]), host.adamw8_state(b)], **two)
+    with pytest.raises(ValueError, match='twice'):
+        if bits == 32:
+            host.adamw_step([a, b], [t(600), t(600)], [t(600), t(600)], [t(600), t(600)], **two, copies=[w[:600], w[400:]])
+        else:
+            host.adamw8_step([a, b], [t(600), t(600)], [host.adamw8_state(a), host.adamw8_state(b)], **two, copies=[w[:600], w[400:]])
     # nothing to do is not an error
     if bits == 32:
         host.adamw_step([], [], [], [], [], [], t(1))

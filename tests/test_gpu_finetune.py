@@ -293,7 +293,7 @@ def test_policy_loss_edges(what):
         with torch.no_grad():
             z.fill_(math.nan)
         loss, kl, clipped = ops.policy_loss(z, label, adv, old, ref, kl_weight=0.1)
-        assert float(loss) == float(kl) == float(clipped) == 0
+        assert float(loss.detach()) == float(kl) == float(clipped) == 0
         assert torch.all(torch.autograd.grad(loss, z)[0] == 0)
         return
     if what == 'one valid':
@@ -518,6 +518,40 @@ def test_adamw8_is_repeatable():
 
 
 @pytest.mark.parametrize('bits', [32, 8])
+def test_adamw_more_tensors_than_a_launch_holds(bits):
+    """2500 tensors (a launch holds 1024, the small kernel before it about 50): every one as if it were alone"""
+    from mit_semseg import ops
+    gen = torch.Generator().manual_seed(2)
+    sizes = [1 + (i * 37) % 700 for i in range(2500)]
+    sizes[1030] = 9000
+    at = [0]
+    for n in sizes:
+        at.append(at[-1] + -(-n // 256) * 256)
+    flat = torch.randn(at[-1], generator=gen).to(dev())
+    p0, g = flat.clone(), torch.randn(at[-1], generator=gen).to(dev())
+    cut = lambda t: [t[a:a + n] for a, n in zip(at, sizes)]             # noqa: E731
+    steps, lr = torch.zeros(2500, dtype=torch.int32, device=dev()), torch.tensor([1e-2], device=dev())
+    if bits == 32:
+        m, v = torch.zeros_like(flat), torch.zeros_like(flat)
+        ops.adamw_step(cut(flat), cut(g), cut(m), cut(v), list(steps.unbind()), [0.1] * 2500, lr)
+    else:
+        m, v = (torch.zeros(at[-1], dtype=torch.uint8, device=dev()) for _ in range(2))
+        ms, vs = (torch.zeros(at[-1] // 256, device=dev()) for _ in range(2))
+        blocks = [slice(a // 256, a // 256 + -(-n // 256)) for a, n in zip(at, sizes)]
+        ops.adamw8_step(cut(flat), cut(g), [(a, ms[b], c, vs[b]) for a, b, c in zip(cut(m), blocks, cut(v))], list(steps.unbind()),
+                        [0.1] * 2500, lr)
+    assert torch.all(steps == 1)
+    # the first step from zero states moves by lr (sign(g) up to eps) + lr wd p
+    live = torch.zeros(at[-1], dtype=torch.bool)
+    for a, n in zip(at, sizes):
+        live[a:a + n] = True
+    want = p0.cpu().double() * (1 - 1e-2 * 0.1) - 1e-2 * g.cpu().double() / (g.cpu().double().abs() + 1e-8)
+    got = flat.cpu().double()
+    assert torch.all((got - want).abs()[live] <= U32 * got.abs()[live] + 20 * U32 * 1e-2 + U32 * 1e-3)
+    assert torch.equal(got[~live], p0.cpu().double()[~live])
+
+
+@pytest.mark.parametrize('bits', [32, 8])
 def test_adamw_writes_nothing_else(bits):
     """guard elements around every tensor of a call stay as they were"""
     from mit_semseg import ops
@@ -629,3 +663,36 @@ def test_captured_step_replays(bits):
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(eager['s'], cap['s']))
         torch.cuda.synchronize()
     assert int(cap['step']) == 5
+
+
+def test_capture_beside_a_living_graph_of_the_same_leaf_is_refused():
+    """a leaf's earlier graph on another stream: the capture is refused with an error, and works once that graph is gone"""
+    from mit_semseg import ops
+    gen = torch.Generator().manual_seed(12)
+    z, label, adv, old, ref = policy_inputs((2, 150, 6, 7), torch.float32, 'nhwc', gen)
+    z = z.detach().requires_grad_(True)
+    loss = ops.policy_loss(z, label, adv, old)[0]
+    want = torch.autograd.grad(loss, z, retain_graph=True)[0]
+    lp = ops.label_log_prob(z, label)
+    for call in (lambda: ops.policy_loss(z, label, adv, old), lambda: ops.label_log_prob(z, label)):
+        with pytest.raises(RuntimeError, match='another stream'):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        torch.cuda.synchronize()
+    ops.policy_loss(z, label, adv, old)                               # eager calls go on
+    with torch.no_grad():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):                                  # no gradient, nothing to refuse
+            value = ops.label_log_prob(z, label)
+        graph.replay()
+        assert torch.equal(value, lp)
+    del loss, lp
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.policy_loss(z, label, adv, old)[0]
+        dz = torch.autograd.grad(out, z)[0]
+    for _ in range(3):
+        dz.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dz, want)
