@@ -321,7 +321,7 @@ def check_codes(x, err, codes, scales, random16, positive):
     assert torch.equal(torch.sign(got)[nonzero], torch.sign(x)[nonzero])
 
 
-def check_step8(p0, g, m0, r0, p, state, t, lr, wd, betas, eps, seed, ordinal, factor=1.0):
+def check_step8(p0, g, m0, r0, p, state, t, lr, wd, betas, eps, seed, ordinal, factor=1.0, start=0):
     """one 8-bit step from the decoded states m0, r0 (float64).  m, r^2: as check_step, each with one rounding more (the decoding), a
     product of codes and scales; root and reciprocal are up to one unit (2 roundings) off."""
     n = p.numel()
@@ -331,7 +331,7 @@ def check_step8(p0, g, m0, r0, p, state, t, lr, wd, betas, eps, seed, ordinal, f
     terms = betas[0] * m0.abs() + (1 - betas[0]) * (g.double() * factor).abs()
     spread = terms / (1 - betas[0] ** t) * lr / ((rv / (1 - betas[1] ** t)).sqrt() + eps)
     assert torch.all((p.double() - rp).abs() <= U32 * rp.abs() + 20 * U32 * (spread + lr * wd * p0.double().abs()) + 2.0 ** -148)
-    bits = mix((torch.arange(n) + mix(seed ^ mix(t ^ mix(ordinal)))) & 0xFFFFFFFF)
+    bits = mix((torch.arange(start, start + n) + mix(seed ^ mix(t ^ mix(ordinal)))) & 0xFFFFFFFF)
     check_codes(rm, 6 * U32 * terms, state[0], state[1], bits & 0xFFFF, False)
     r = rv.sqrt()
     check_codes(r, 7 * U32 * r + 1.1e-19, state[2], state[3], bits >> 16, True)

@@ -696,3 +696,110 @@ def test_capture_beside_a_living_graph_of_the_same_leaf_is_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(dz, want)
+
+
+# ------------------------------------------------------------------------------------- offsets that do not fit 32 bits
+@pytest.mark.parametrize('rows,c', [(14400000, 150), (33000, 65601)])
+def test_more_than_2_31_logits(rows, c):
+    """the last rows of maps of more than 2^31 elements"""
+    from mit_semseg import ops
+    gen = torch.Generator().manual_seed(20)
+    assert rows * c > 2 ** 31
+    z = torch.zeros(rows, c, device=dev(), dtype=torch.bfloat16)
+    n = 70
+    z[-n:] = (3 * torch.randn(n, c, generator=gen)).to(dev(), torch.bfloat16)
+    z.requires_grad_(True)
+    label = torch.full((rows,), -1, device=dev())
+    label[-n:] = torch.randint(0, c, (n,), generator=gen).to(dev())
+    g = torch.randn(n, generator=gen)
+    up = torch.zeros(rows, device=dev())
+    up[-n:] = g.to(dev())
+    lp = ops.label_log_prob(z, label)
+    want, valid, logp, top, x = reference_logp(z.detach()[-n:], label[-n:])
+    za = x.gather(1, label[-n:].cpu().unsqueeze(1)).squeeze(1)
+    assert torch.all((lp.detach()[-n:].cpu().double() - want).abs() <= logp_bound(want, za, top, c))
+    assert float(lp.detach()[:-n].abs().max()) == 0
+    dz = torch.autograd.grad(lp, z, up)[0]
+    check_gradient(dz[-n:], g.double(), logp, x, top, label[-n:], valid, torch.bfloat16)
+    assert int(torch.count_nonzero(dz[:-n])) == 0
+    old = (want + 0.05).float()
+    olds = torch.zeros(rows, device=dev())
+    olds[-n:] = old.to(dev())
+    adv = torch.ones(rows, device=dev())
+    loss, _, clipped = ops.policy_loss(z.detach(), label, adv, olds)
+    value, err = reference_policy(z.detach()[-n:], label[-n:], adv[-n:], olds[-n:], None, 0.2, 0.2, 0.0)[:2]
+    assert abs(float(loss) - float(value[0])) <= float(err[0]) + 2 * U32 * abs(float(value[0])) and float(clipped) == 0.0
+    del z, dz
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_more_than_2_31_parameters(bits):
+    """the ends and the middle of a tensor of more than 2^31 elements (more than 2^32 in 8 bits: the counter of the random bits goes round)"""
+    from mit_semseg import ops
+    n = 2 ** 31 + 5003 if bits == 32 else 2 ** 32 + 5003
+    p = torch.full((n,), 0.5, device=dev())
+    g = torch.full((n,), 0.25, device=dev(), dtype=torch.bfloat16)
+    gen = torch.Generator().manual_seed(21)
+    spots = [slice(0, 512), slice(2 ** 31 - 256, 2 ** 31 + 256), slice(n - 5003 - 256, n)] + ([slice(2 ** 32 - 256, 2 ** 32 + 256)] if bits == 8 else [])
+    for s in spots:
+        k = len(range(*s.indices(n)))
+        p[s], g[s] = torch.randn(k, generator=gen).to(dev()), torch.randn(k, generator=gen).to(dev(), torch.bfloat16)
+    before = [(p[s].cpu(), g[s].cpu()) for s in spots]
+    step, lr = torch.zeros(1, dtype=torch.int32, device=dev()), torch.tensor([1e-2], device=dev())
+    norm = float(ops.grad_norm([g])[0])
+    apart = [before[0], before[2]] if bits == 32 else before[:3]       # the others lie inside the last one
+    want = sum(float(x[1].double().square().sum()) for x in apart) + (n - sum(x[1].numel() for x in apart)) * 0.0625
+    assert abs(norm - math.sqrt(want)) <= 2 * U32 * norm
+    if bits == 32:
+        m, v = torch.zeros(n, device=dev()), torch.zeros(n, device=dev())
+        ops.adamw_step([p], [g], [m], [v], [step], [0.1], lr)
+    else:
+        state = ops.adamw8_state(p)
+        ops.adamw8_step([p], [g], [state], [step], [0.1], lr, seed=3)
+    for s, (p0, g0) in zip(spots, before):
+        zero = torch.zeros_like(p0)
+        if bits == 32:
+            check_step(p0, g0, zero, zero, p[s].cpu(), m[s].cpu(), v[s].cpu(), 1, float(lr), 0.1, (0.9, 0.999), 1e-8)
+        else:
+            a, b, c = s.indices(n)
+            q = slice(a // 256, -(-b // 256))
+            got = [state.m[s].cpu(), state.m_scale[q].cpu(), state.r[s].cpu(), state.r_scale[q].cpu()]
+            check_step8(p0, g0, zero.double(), zero.double(), p[s].cpu(), got, 1, float(lr), 0.1, (0.9, 0.999), 1e-8, 3, 0, start=a)
+    middle = p[1 << 20:1 << 30]
+    assert float(middle.min()) == float(middle.max()) != 0.5
+    del p, g, middle
+    torch.cuda.empty_cache()
+
+
+def test_two_graphs_replayed_at_once():
+    """two captured steps on two streams share no scratch: every replay equals the eager result"""
+    from mit_semseg import ops
+    gen = torch.Generator().manual_seed(14)
+    sets = [policy_inputs(shape, t, 'nhwc', gen) for shape, t in (((2, 150, 48, 64), torch.float32), ((1, 9000, 5, 7), torch.bfloat16))]
+    sets = [(z.detach(), *rest) for z, *rest in sets]
+
+    def work(z, label, adv, old, ref):
+        z = z.clone(memory_format=torch.preserve_format).requires_grad_(True)
+        loss, kl, clipped = ops.policy_loss(z, label, adv, old, ref, kl_weight=0.1)
+        dz = torch.autograd.grad(loss, z)[0]
+        return [loss.detach(), kl, clipped, dz, ops.grad_norm([dz], 1e-3)]
+    want = [work(*s) for s in sets]
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in sets]
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(work(*s))
+    for _ in range(4):
+        for out in outs:
+            for t in out:
+                t.zero_()
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for graph, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, outs):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
