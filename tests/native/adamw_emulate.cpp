@@ -120,3 +120,17 @@ extern "C" int semseg_adamw8_step(const semseg_adamw8_tensor* t, int n, const fl
     }
     return 0;
 }
+
+extern "C" size_t semseg_grad_norm_workspace_bytes(const semseg_grad_tensor*, int) { return 8; }
+extern "C" int semseg_grad_norm(const semseg_grad_tensor* t, int n, float scale, float max_norm, float* out, void*, size_t, void*) {
+    double s = 0.0;
+    for (int i = 0; i < n; ++i)
+        for (int64_t j = 0; j < t[i].numel; ++j) {
+            const double x = (double)load(t[i].grad, t[i].grad_type, j);
+            s += x * x;
+        }
+    const double norm = sqrt(s) * fabs((double)scale);
+    out[0] = (float)norm;
+    out[1] = fabsf(out[0]) <= 3.402823466e38f ? (max_norm >= 0.f ? (float)fmin(1.0, (double)max_norm / (norm + 1e-6)) : 1.f) : 0.f;
+    return 0;
+}

@@ -20,7 +20,8 @@ def build_emulator(folder):
                     os.path.join(ROOT, 'tests', 'native', 'adamw_emulate.cpp'), '-o', out], check=True)
     from mit_semseg import _native
     lib = ctypes.CDLL(out)
-    for name in ('semseg_adamw_workspace_bytes', 'semseg_adamw_step', 'semseg_adamw8_step'):
+    for name in ('semseg_adamw_workspace_bytes', 'semseg_adamw_step', 'semseg_adamw8_step', 'semseg_grad_norm_workspace_bytes',
+                 'semseg_grad_norm'):
         getattr(lib, name).restype, getattr(lib, name).argtypes = _native.SIGNATURES[name]
     return lib
 
@@ -411,3 +412,65 @@ def test_adamw8_state_layout(host):
     m, v = host.adamw8_values(s, p)
     assert m.stride() == p.stride() and float(m.as_strided((180,), (1,))[7]) == 2.0 and float(m.sum()) == 2.0
     assert math.isclose(float(v.sum()), 0.0)
+
+
+def _train_ranks(rank, world, folder, port, bits):
+    """three steps of a small network on its own data, gradients in buckets, AdamW with clipping; the replicas go to a file"""
+    import ctypes as C
+    import torch.distributed as dist
+    from mit_semseg import _native, ops
+    from mit_semseg.engine import FusedAdamW
+    from mit_semseg.parallel import GradientBuckets
+    os.environ.update(MASTER_ADDR='127.0.0.1', MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world))
+    dist.init_process_group('gloo', rank=rank, world_size=world)
+    lib = C.CDLL(os.path.join(folder, 'libadamw_emulate.so'))
+    for name in ('semseg_adamw_workspace_bytes', 'semseg_adamw_step', 'semseg_adamw8_step', 'semseg_grad_norm_workspace_bytes',
+                 'semseg_grad_norm'):
+        getattr(lib, name).restype, getattr(lib, name).argtypes = _native.SIGNATURES[name]
+    _native.lib, ops._require_cuda, ops._st = (lambda: lib), (lambda *a: None), (lambda: ops.vp(0))
+    net, data = _network()
+    opt = FusedAdamW([dict(params=list(net.parameters()), lr=1e-2, weight_decay=0.1)], bits=bits, max_norm=0.5)
+    buckets = GradientBuckets(list(net.parameters()), 1 << 14) if world > 1 else None
+    for it in range(3):
+        opt.zero_grad()
+        if buckets is not None:
+            buckets.prepare()
+        x = data[it]
+        loss = net(x[rank::world]).square().mean()
+        loss.backward()
+        if buckets is not None:
+            buckets.finish()
+        opt.step(grad_scale=1.0 / world)
+    torch.save(dict(net=net.state_dict(), clip=opt.clip, counts=[int(opt.state[p][0]) for p in net.parameters()]),
+               os.path.join(folder, 'rank%d_of_%d_%d.pt' % (rank, world, bits)))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def _network():
+    torch.manual_seed(4)
+    net = torch.nn.Sequential(torch.nn.Linear(40, 120), torch.nn.ReLU(), torch.nn.Linear(120, 37))
+    return net, torch.randn(3, 16, 40, generator=torch.Generator().manual_seed(5))
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_adamw_on_two_ranks(bits, emulator, tmp_path):
+    """two ranks with half of the batch each end with the same replicas, and with those of one rank that sees the whole batch"""
+    import socket
+    import torch.multiprocessing as mp
+    build_emulator(tmp_path)
+    for world in (1, 2):
+        with socket.socket() as s:
+            s.bind(('127.0.0.1', 0))
+            port = s.getsockname()[1]
+        mp.spawn(_train_ranks, args=(world, str(tmp_path), port, bits), nprocs=world, join=True)
+    one, a, b = (torch.load(str(tmp_path / ('rank%d_of_%d_%d.pt' % (r, w, bits))), weights_only=True) for r, w in ((0, 1), (0, 2), (1, 2)))
+    assert a['counts'] == b['counts'] == one['counts'] == [3] * 4
+    assert torch.equal(a['clip'], b['clip']) and abs(float(a['clip'][0] - one['clip'][0])) <= 1e-5 * float(one['clip'][0])
+    for k in one['net']:
+        assert torch.equal(a['net'][k], b['net'][k])
+        if bits == 32:
+            # the halves' gradients and the whole one differ by the roundings of sums of 16 products.  A step is lr m / sqrt(v): it feels
+            # them as much as the gradient does, fully (up to 2 lr) where the sum cancels to nothing, which few elements' do
+            off = (a['net'][k] - one['net'][k]).abs() > 1e-2 * 1e-2
+            assert float(off.float().mean()) <= 0.02
