@@ -269,7 +269,7 @@ void check(int rc, const char* what) {
 struct RowsBackward : public torch::autograd::Node {
     torch::autograd::SavedVariable z, label, kept;
     at::Tensor written;
-    std::vector<int64_t> shape;
+    std::vector<int64_t> shape, strides;              // of the logits, and of `z`
     int64_t ld = 0, ignore = 0;
     bool loss = false;
     LogpBackward logp_bwd = nullptr;
@@ -296,6 +296,12 @@ struct RowsBackward : public torch::autograd::Node {
         {
             at::AutoDispatchBelowADInplaceOrView below;
             const c10::DeviceGuard guard(zt.device());
+            int64_t pitch = ld;
+            if (zt.strides() != strides) {            // saved through hooks (on the CPU, say) that keep values and not layouts
+                zt = shape.size() == 2 ? zt.contiguous()
+                                       : zt.permute({0, 2, 3, 1}).contiguous().permute({0, 3, 1, 2});
+                pitch = shape[1];
+            }
             const at::Tensor g = grads[0].to(at::kFloat).contiguous();
             const int64_t P = lab.numel();
             const float* kp = (const float*)keep.const_data_ptr();
@@ -307,7 +313,7 @@ struct RowsBackward : public torch::autograd::Node {
                 dz = shape.size() == 2 ? at::empty(shape, zt.options())
                                        : at::empty({shape[0], shape[2], shape[3], shape[1]}, zt.options()).permute({0, 3, 1, 2});
                 if (P)
-                    check(logp_bwd(zt.const_data_ptr(), type_code(zt), ld, (const int64_t*)lab.const_data_ptr(), ignore,
+                    check(logp_bwd(zt.const_data_ptr(), type_code(zt), pitch, (const int64_t*)lab.const_data_ptr(), ignore,
                                    loss ? coef - 2 * P : kp, loss ? coef : (const float*)g.const_data_ptr(),
                                    loss ? (const float*)g.const_data_ptr() : nullptr, inv, P, (int)shape[1], dz.mutable_data_ptr(),
                                    stream_of(zt)),
@@ -347,6 +353,7 @@ PyObject* attach_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
         auto node = std::shared_ptr<RowsBackward>(new RowsBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(z));
         node->shape = z.sizes().vec();
+        node->strides = tensor(args[2], what).strides().vec();
         node->z = torch::autograd::SavedVariable(tensor(args[2], what), false);
         node->label = torch::autograd::SavedVariable(tensor(args[3], what), false);
         node->kept = torch::autograd::SavedVariable(tensor(args[4], what), false);

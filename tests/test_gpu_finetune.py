@@ -803,3 +803,21 @@ def test_two_graphs_replayed_at_once():
         torch.cuda.synchronize()
         for a, b in zip(want, outs):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize('shape,layout', [((2, 150, 6, 7), 'slice'), ((2, 400, 6, 7), 'apart'), ((1, 33, 1, 50), 'rows_slice'), ((2, 19, 5, 6), 'nchw')], ids=str)
+def test_saved_tensor_hooks(shape, layout):
+    """what is kept for the backward pass may come back from a hook in another layout"""
+    from mit_semseg import ops
+    for dtype in TYPES:
+        gen = torch.Generator().manual_seed(16)
+        z, label, adv, old, ref = policy_inputs(shape, dtype, layout, gen)
+        calls = (lambda: ops.label_log_prob(z, label).sum(), lambda: ops.policy_loss(z, label, adv, old, ref, kl_weight=0.1)[0])
+        for call in calls:
+            out = call()
+            torch.autograd.grad(out, z, retain_graph=True)            # (what the forward pass has written is handed out)
+            want = torch.autograd.grad(out, z)[0]
+            with torch.autograd.graph.save_on_cpu():
+                out = call()
+            torch.autograd.grad(out, z, retain_graph=True)
+            assert torch.equal(torch.autograd.grad(out, z)[0], want)
