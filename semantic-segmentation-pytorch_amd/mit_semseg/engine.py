@@ -81,8 +81,8 @@ class FusedAdamW:
     most this global norm, and a step whose gradients are not finite changes nothing (`float('inf')`: only that).
 
     lr, step counts and the clip factor are device memory, the states exist from the start: a captured step can be replayed.  A
-    parameter without a gradient is left alone, its step count too.  `clip` is the [norm, factor] of the last step
-    (of a captured step: until the next one)."""
+    parameter without a gradient is left alone, its step count too.  `clip` holds the [norm, factor] of the
+    last step, replayed or not (None without `max_norm`)."""
 
     def __init__(self, groups, betas=(0.9, 0.999), eps=1e-8, bits=32, max_norm=None, min_8bit=4096, seed=0):
         """groups: list of dict(params=[...], lr=float, weight_decay=float)."""
@@ -93,7 +93,7 @@ class FusedAdamW:
         self.groups, self.betas, self.eps, self.max_norm, self.seed = groups, betas, eps, max_norm, seed
         self.state = {}                               # parameter -> (its step count, its state: two tensors or an ops.AdamW8State)
         self.steps = 0
-        self.clip = None
+        self.clip = None if max_norm is None else torch.zeros(2, device=groups[0]['params'][0].device, dtype=torch.float32)
         for g in groups:
             dev = g['params'][0].device
             g['lr_t'] = torch.full((1,), float(g['lr']), device=dev, dtype=torch.float32)
@@ -110,7 +110,8 @@ class FusedAdamW:
     def step(self, grad_scale=1.0):
         live = [[p for p in g['params'] if p.grad is not None] for g in self.groups]
         grads = [p.grad for ps in live for p in ps]
-        self.clip = ops.grad_norm(grads, self.max_norm, grad_scale) if self.max_norm is not None and grads else None
+        if self.clip is not None and grads:
+            ops.grad_norm(grads, self.max_norm, grad_scale, out=self.clip)
         for i, (g, ps) in enumerate(zip(self.groups, live)):
             wide = [p for p in ps if not isinstance(self.state[p][1], ops.AdamW8State)]
             coded = [p for p in ps if isinstance(self.state[p][1], ops.AdamW8State)]

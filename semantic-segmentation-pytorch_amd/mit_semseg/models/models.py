@@ -29,17 +29,24 @@ class PolicyLoss(nn.Module):
     """Criterion of SegmentationModule for tuning a trained network on a reward (a metric of whole label maps, say) instead of labels:
     the label map is one that was sampled from the network, `advantage` what it earned (per image or per pixel), and the loss is the
     clipped policy loss with a KL term of ops.policy_loss.  forward(scores, label, advantage, old_logp, ref_logp) -> loss; `kl` and
-    `clipped` hold the mean KL term and the share of clipped pixels of the last forward."""
+    `clipped` are the mean KL term and the share of clipped pixels of the last step, replayed or not (views of one buffer)."""
 
     def __init__(self, clip_low=0.2, clip_high=0.2, kl_weight=0.0, ignore_index=-1):
         super(PolicyLoss, self).__init__()
         self.clip_low, self.clip_high, self.kl_weight, self.ignore_index = clip_low, clip_high, kl_weight, ignore_index
-        self.kl = self.clipped = None
+        self.register_buffer('scalars', torch.zeros(2), persistent=False)
+
+    @property
+    def kl(self):
+        return self.scalars[0]
+
+    @property
+    def clipped(self):
+        return self.scalars[1]
 
     def forward(self, scores, label, advantage, old_logp, ref_logp=None):
-        loss, self.kl, self.clipped = ops.policy_loss(scores, label, advantage, old_logp, ref_logp, self.clip_low, self.clip_high,
-                                                      self.kl_weight, self.ignore_index)
-        return loss
+        return ops.policy_loss(scores, label, advantage, old_logp, ref_logp, self.clip_low, self.clip_high, self.kl_weight,
+                               self.ignore_index, self.scalars)[0]
 
 
 class SegmentationModule(SegmentationModuleBase):

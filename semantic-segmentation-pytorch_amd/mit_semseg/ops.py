@@ -2407,7 +2407,7 @@ def _row_constants(what, name, t, shapes, device):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip_high=0.2, kl_weight=0.0, ignore_index=-1):
+def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip_high=0.2, kl_weight=0.0, ignore_index=-1, scalars=None):
     """Clipped policy loss with a KL term over per-row categoricals (logits z as in label_log_prob): with lp the log probability of
     the chosen label under z and ratio = exp(lp - old_logp), the mean over the rows that count of
 
@@ -2417,7 +2417,8 @@ def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip
     (label_log_prob under no_grad gives them).  Rows whose label is `ignore_index` or outside [0, C) do not count.
     Returns three scalars: the loss (differentiable in z), the mean KL term (0 without ref_logp) and the share of rows whose clipped
     term is the smaller one; all 0 where no row counts.  For float32 logits of 8 to 320 classes whose rows lie close together the gradient
-    of the logits is written in the forward pass (and its memory taken then)."""
+    of the logits is written in the forward pass (and its memory taken then).  `scalars`: two float32 on the device that receive the KL
+    term and the share (and are returned as such), for a caller who replays captured steps and reads them in one place."""
     clip_low, clip_high, kl_weight = float(clip_low), float(clip_high), float(kl_weight)
     if not 0.0 <= clip_low <= 1.0 or not 0.0 <= clip_high < float('inf'):
         raise ValueError('policy_loss: clip_low must lie in [0, 1] and clip_high must not be negative, got %r, %r' % (clip_low, clip_high))
@@ -2432,14 +2433,19 @@ def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip
     old_logp = _row_constants(what, 'old_logp', old_logp, (rows,), dev)
     if ref_logp is not None:
         ref_logp = _row_constants(what, 'ref_logp', ref_logp, (rows,), dev)
+    if scalars is not None and (scalars.dtype is not torch.float32 or tuple(scalars.shape) != (2,) or not scalars.is_contiguous() or
+                                scalars.device != dev or scalars.requires_grad):
+        raise ValueError('policy_loss: scalars must be two float32 on %s' % dev)
     zr, ld, P, c = _logit_rows(z)
     wanted = torch.is_grad_enabled() and z.requires_grad
     dz = None
+    loss = torch.empty((), device=dev, dtype=torch.float32)
+    kl, clipped = (torch.empty((), device=dev, dtype=torch.float32) for _ in range(2)) if scalars is None else scalars.unbind()
     if P == 0:
-        loss, kl, clipped = (torch.zeros((), device=dev) for _ in range(3))
+        for t in (loss, kl, clipped):
+            t.zero_()
         kept = torch.zeros(1, device=dev)
     else:
-        loss, kl, clipped = (torch.empty((), device=dev, dtype=torch.float32) for _ in range(3))
         L, code = _native.lib(), _TYPE_CODES[z.dtype]
         # one buffer of its own (the caching allocator orders its reuse by stream and by captured graph): scratch, then what the backward
         # pass reads -- maximum and logarithm of the sum per row, gradient per row, 1 / rows that count
@@ -2617,10 +2623,11 @@ def adamw8_step(params, grads, states, steps, weight_decays, lr_tensor, betas=(0
     _weights_changed(params)
 
 
-def grad_norm(grads, max_norm=None, grad_scale=1.0):
+def grad_norm(grads, max_norm=None, grad_scale=1.0, out=None):
     """Global 2-norm of gradients (float32 / bfloat16 / float16, any mix, dense): float32 [2] on the device -- the norm of
     grad * grad_scale and the factor min(1, max_norm / (norm + 1e-6)) that brings it to max_norm (1 without max_norm, 0 where the norm
-    is not finite).  Nothing is scaled: adamw_step / adamw8_step take the result as `clip`.  Sums run in 64 bits in a fixed order."""
+    is not finite).  Nothing is scaled: adamw_step / adamw8_step take the result as `clip`.  `out`: the tensor to write to.
+    Sums run in 64 bits in a fixed order."""
     if max_norm is not None and not 0.0 <= max_norm:
         raise ValueError('grad_norm: max_norm must not be negative, got %r' % max_norm)
     if not grads:
@@ -2628,8 +2635,11 @@ def grad_norm(grads, max_norm=None, grad_scale=1.0):
     _require_cuda(grads[0])
     table, n = _native.host().grad_table(grads)
     L, dev = _native.lib(), grads[0].device
-    with _device_guard(dev):
+    if out is None:
         out = torch.empty(2, device=dev, dtype=torch.float32)
+    elif out.dtype is not torch.float32 or out.numel() != 2 or not out.is_contiguous() or out.device != dev:
+        raise ValueError('grad_norm: out must be two float32 on %s' % dev)
+    with _device_guard(dev):
         ws = torch.empty(L.semseg_grad_norm_workspace_bytes(table, n), device=dev, dtype=torch.uint8)
         _native.check(L.semseg_grad_norm(table, n, grad_scale, -1.0 if max_norm is None else max_norm, _p(out), _p(ws), ws.numel(),
                                          _st()), 'grad_norm')

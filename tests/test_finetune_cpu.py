@@ -88,6 +88,9 @@ def test_policy_loss_refusals(host):
         a = {**ok, **k}
         return host.policy_loss(a['z'], a['label'], a['advantage'], a['old_logp'], a['ref_logp'], a['clip_low'], a['clip_high'],
                                 a['kl_weight'])
+    for bad in (torch.zeros(3), torch.zeros(2, dtype=torch.float64), torch.zeros(4)[::2], torch.zeros(2, requires_grad=True)):
+        with pytest.raises(ValueError, match='scalars'):
+            host.policy_loss(z, label, adv, old, scalars=bad)
     for k, err in ((dict(advantage=torch.zeros(3)), ValueError), (dict(advantage=torch.zeros(2, dtype=torch.long)), TypeError),
                    (dict(advantage=torch.zeros(2, requires_grad=True)), ValueError), (dict(old_logp=torch.zeros(2, 12)), ValueError),
                    (dict(old_logp=torch.zeros(2, 3, 4, requires_grad=True)), ValueError), (dict(ref_logp=None), ValueError),
@@ -108,6 +111,9 @@ def test_grad_norm_refusals(host):
         host.grad_norm([g], max_norm=-1.0)
     with pytest.raises(ValueError):
         host.grad_norm([g], max_norm=float('nan'))
+    for bad in (torch.zeros(3), torch.zeros(2, dtype=torch.float64), torch.zeros(4)[::2]):
+        with pytest.raises(ValueError, match='out'):
+            host.grad_norm([g], out=bad)
 
 
 @pytest.mark.parametrize('bits', [32, 8])

@@ -155,6 +155,29 @@ def test_policy_tuning_run():
     assert all(float(oa[i][3]) == 0.0 for i in (0, 2, 4))
 
 
+def test_scalars_of_replayed_steps_of_two_shapes():
+    """the KL term, the clipped share and the gradient norm are those of the step that ran last, whichever recording it replayed"""
+    from mit_semseg.engine import TrainStep
+    from mit_semseg.models import PolicyLoss
+    out = []
+    for graph in (False, True):
+        sm = make(PolicyLoss(kl_weight=0.05))
+        ts = TrainStep(sm, lr_encoder=1e-5, lr_decoder=1e-4, max_iters=100, optim='AdamW', clip_grad_norm=1.0, graph=graph)
+        g = torch.Generator().manual_seed(13)
+        feeds = []
+        for w in (12, 8):
+            feeds.append({'img_data': torch.randn(2, 3, 64, 8 * w, generator=g).to(dev()), 'seg_label': torch.randint(-1, 150, (2, 8, w), generator=g).to(dev()),
+                          'advantage': torch.randn(2, generator=g).to(dev()), 'old_logp': (-5 + 0.5 * torch.randn(2, 8, w, generator=g)).to(dev()),
+                          'ref_logp': (-5 + 0.5 * torch.randn(2, 8, w, generator=g)).to(dev())})
+        seen = []
+        for i in range(8):
+            loss, _ = ts.step(feeds[i % 2])
+            seen.append(torch.stack([loss, sm.crit.kl, sm.crit.clipped, *ts.opt.clip]).clone())
+        out.append(torch.stack(seen))
+    assert ts.stats['replayed'] >= 5, ts.stats
+    assert torch.equal(out[0], out[1]) and len({tuple(r) for r in out[0].tolist()}) == 8
+
+
 def test_policy_module_loss_and_gradient():
     """loss and d loss / d scores through the module against float64"""
     from mit_semseg.models import PolicyLoss
