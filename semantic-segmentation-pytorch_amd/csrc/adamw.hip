@@ -492,14 +492,15 @@ __device__ __forceinline__ void add_square(double& s, float x) { const double d 
 __device__ __forceinline__ void add_squares(double& s, u32x4 v, int type) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+        const uint32_t w = v[j];            // a word of its own: bit_cast of the vector's element v[j] itself reads element 0 (hipcc 7.2)
         if (type == SEMSEG_TYPE_F32) {
-            add_square(s, adam_float(v[j]));
+            add_square(s, adam_float(w));
         } else if (type == SEMSEG_TYPE_BF16) {
-            add_square(s, adam_float(v[j] << 16));
-            add_square(s, adam_float(v[j] & 0xffff0000u));
+            add_square(s, adam_float(w << 16));
+            add_square(s, adam_float(w & 0xffff0000u));
         } else {
             typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-            const f16x2 x = __builtin_bit_cast(f16x2, v[j]);
+            const f16x2 x = __builtin_bit_cast(f16x2, w);
             add_square(s, (float)x[0]);
             add_square(s, (float)x[1]);
         }
