@@ -68,10 +68,9 @@ int type_code(const at::Tensor& t) {
 
 // elements of two tensors follow each other in memory in the same order; strides of axes of one element say nothing
 bool same_order(const at::Tensor& a, const at::Tensor& b) {
-    if (a.numel() != b.numel()) return false;
+    if (a.sizes() != b.sizes()) return false;          // equal strides alone may stand for other elements, or for fewer in memory
     const auto sa = a.strides(), sb = b.strides();
     if (sa == sb) return true;
-    if (a.sizes() != b.sizes()) return false;
     for (size_t i = 0; i < sa.size(); ++i)
         if (a.size(i) != 1 && sa[i] != sb[i]) return false;
     return true;

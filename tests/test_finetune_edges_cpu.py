@@ -1,0 +1,39 @@
+"""The fine-tuning operators without a GPU: calls that lie beside the documented ones (layouts that only look alike, memory that is read and
+written in one call, forward-mode derivatives, numbers at the ends of float32's range), and the host code around them."""
+import math
+
+import pytest
+import torch
+
+from tests.test_finetune_cpu import U32, emulated, emulator, host  # noqa: F401  (fixtures)
+from tests.test_host_logic_dryrun import stub  # noqa: F401  (fixture)
+
+
+def one(ops, bits, p, g, m=None, v=None, copy=None, more=()):
+    """an AdamW step over p (and `more` whole parameters)"""
+    ps = [p, *more]
+    gs = [g] + [torch.zeros_like(q) for q in more]
+    steps, wds = list(torch.zeros(len(ps), dtype=torch.int32).unbind()), [0.0] * len(ps)
+    copies = None if copy is None else [copy] + [None] * len(more)
+    if bits == 8:
+        return ops.adamw8_step(ps, gs, [ops.adamw8_state(q) for q in ps], steps, wds, torch.zeros(1), copies=copies)
+    ms = [torch.zeros_like(p) if m is None else m] + [torch.zeros_like(q) for q in more]
+    vs = [torch.zeros_like(p) if v is None else v] + [torch.zeros_like(q) for q in more]
+    return ops.adamw_step(ps, gs, ms, vs, steps, wds, torch.zeros(1), copies=copies)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_layouts_that_share_only_their_strides_are_refused(host, bits):  # noqa: F811
+    """[8, 2] and a [2, 8] view with the same strides (2, 1): the view covers 10 elements of memory, the parameter 16"""
+    p = torch.zeros(8, 2)
+    alike = torch.zeros(10).as_strided((2, 8), (2, 1))
+    apart = torch.zeros(8).as_strided((3, 2), (3, 1))                # not dense: [2, 3] has the same strides and 6 elements in 6 places
+    for q, g in ((p, alike), (torch.zeros(2, 3), apart)):
+        with pytest.raises(RuntimeError, match='layout'):
+            one(host, bits, q, g)
+    with pytest.raises(RuntimeError, match='copy'):
+        one(host, bits, p, torch.zeros(8, 2), copy=torch.zeros(10, dtype=torch.bfloat16).as_strided((2, 8), (2, 1)))
+    if bits == 32:
+        for k in ('m', 'v'):
+            with pytest.raises(RuntimeError, match='layout'):
+                one(host, bits, p, torch.zeros(8, 2), **{k: alike})
