@@ -86,6 +86,13 @@ void disjoint(Ranges& r, const char* what) {
         if (r[i].first < r[i - 1].second)
             refuse(PyExc_ValueError, "%s: the same tensor twice among parameters, states, copies and step counts of a call (or overlapping ones)", what);
 }
+// what it reads: nothing that it writes (`w`, sorted and disjoint) -- another block's results would be read as gradients
+void unwritten(const Ranges& w, const void* at, int64_t bytes, const char* what) {
+    const uintptr_t begin = (uintptr_t)at, end = begin + (uintptr_t)bytes;
+    const auto behind = std::lower_bound(w.begin(), w.end(), std::make_pair(end, (uintptr_t)0));
+    if (bytes && behind != w.begin() && std::prev(behind)->second > begin)
+        refuse(PyExc_ValueError, "%s: a gradient shares memory with a parameter, state, copy or step count of the call", what);
+}
 void add(Ranges& r, const void* at, int64_t bytes) {
     if (bytes) r.emplace_back((uintptr_t)at, (uintptr_t)at + (uintptr_t)bytes);
 }
@@ -158,6 +165,7 @@ PyObject* adam_table(PyObject* const* args, Py_ssize_t n_states, FILL fill) {
         if (live) table.push_back(e);
     }
     disjoint(written, what);
+    for (const ENTRY& e : table) unwritten(written, e.grad, e.numel * (e.grad_type == SEMSEG_TYPE_F32 ? 4 : 2), what);
     PyObject* bytes = PyBytes_FromStringAndSize((const char*)table.data(), (Py_ssize_t)(table.size() * sizeof(ENTRY)));
     if (!bytes) throw Refused();
     return Py_BuildValue("Nn", bytes, (Py_ssize_t)table.size());

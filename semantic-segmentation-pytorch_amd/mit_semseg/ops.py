@@ -2567,8 +2567,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, weight_decays, lr_te
     layout; grads: the same layout, float32 / bfloat16 / float16; steps: one int32 device scalar per tensor (views of one tensor
     will do), advanced by the call; lr_tensor: one float32 on the device; grad_scale multiplies the gradients; clip: what grad_norm
     returned -- its factor multiplies them too, and where its norm is not finite the call changes nothing; copies: optional list of
-    bfloat16 / float16 tensors (or None) that receive the updated parameters.  Everything the step reads that changes from step to
-    step is device memory, so a captured call can be replayed."""
+    bfloat16 / float16 tensors (or None) that receive the updated parameters.  No memory that the call writes may appear in it twice, as a
+    gradient neither.  Everything the step reads that changes from step to step is device memory, so a captured call can be replayed."""
     _check_step('adamw_step', params, lr_tensor, betas, eps, clip)
     table, n = _native.host().adamw_table('adamw_step', params, grads, steps, weight_decays, copies, exp_avgs, exp_avg_sqs)
     if n == 0:

@@ -37,3 +37,21 @@ def test_layouts_that_share_only_their_strides_are_refused(host, bits):  # noqa:
         for k in ('m', 'v'):
             with pytest.raises(RuntimeError, match='layout'):
                 one(host, bits, p, torch.zeros(8, 2), **{k: alike})
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_gradients_that_the_call_writes_are_refused(host, bits):  # noqa: F811
+    """a gradient that is (part of) a parameter, a state or a copy: which values are read would depend on which block runs first"""
+    p, q, w = torch.zeros(600), torch.zeros(600), torch.zeros(1000, dtype=torch.bfloat16)
+    both = torch.zeros(1000)
+    for a, g, more, copy in ((p, q, (q,), None), (p, p, (), None), (both[:600], both[400:], (), None), (both[400:], both[:600], (), None),
+                             (p, w[:600], (), w[400:]), (p, w[400:], (), w[:600])):
+        with pytest.raises(ValueError, match='gradient shares memory'):
+            one(host, bits, a, g, copy=copy, more=more)
+    if bits == 32:
+        m = torch.zeros(600)
+        with pytest.raises(ValueError, match='gradient shares memory'):
+            one(host, bits, p, m, m=m)
+    # neighbours in one buffer are no overlap: the call gets as far as the library
+    with pytest.raises(AssertionError, match='was reached'):
+        one(host, bits, both[:500], both[500:])
