@@ -54,6 +54,8 @@ const at::Tensor& tensor(PyObject* o, const char* what) {
     if (!THPVariable_Check(o)) refuse(PyExc_TypeError, "%s: expected a tensor, got %s", what, Py_TYPE(o)->tp_name);
     const at::Tensor& t = THPVariable_Unpack(o);
     if (!t.defined() || t.layout() != at::kStrided) refuse(PyExc_TypeError, "%s: tensors must be strided", what);
+    // a result without a tangent would say that the derivative is zero
+    if (t._fw_grad(0).defined()) refuse(PyExc_NotImplementedError, "%s: there is no forward-mode derivative", what);
     return t;
 }
 

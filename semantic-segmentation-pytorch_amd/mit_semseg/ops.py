@@ -2314,9 +2314,17 @@ def _device_guard(device):
     return torch.cuda.device(device)
 
 
+def _refuse_tangents(what, *tensors):
+    """a result without a tangent would say that the derivative is zero"""
+    for t in tensors:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError('%s: there is no forward-mode derivative' % what)
+
+
 def _row_shape(what, z):
     """shape of one number per row of logits [N, C, H, W] (rows = pixels) or [P, C]; refuses what is not such logits"""
     _require_cuda(z)
+    _refuse_tangents(what, z)
     if z.dtype not in _TYPE_CODES:
         raise TypeError('%s: logits must be float32, bfloat16 or float16, got %s' % (what, z.dtype))
     if z.dim() not in (2, 4):
@@ -2394,6 +2402,7 @@ def label_log_prob(z, label, ignore_index=-1):
 
 def _row_constants(what, name, t, shapes, device):
     _require_cuda(t)
+    _refuse_tangents(what, t)
     if t.requires_grad:
         raise ValueError('%s: %s is a constant of the loss: detach it' % (what, name))
     if not t.dtype.is_floating_point:

@@ -55,3 +55,27 @@ def test_gradients_that_the_call_writes_are_refused(host, bits):  # noqa: F811
     # neighbours in one buffer are no overlap: the call gets as far as the library
     with pytest.raises(AssertionError, match='was reached'):
         one(host, bits, both[:500], both[500:])
+
+
+def test_forward_mode_derivatives_are_refused(stub):  # noqa: F811
+    """a tangent that an operator does not carry on raises, as in the other operators: an output without one stands for a derivative of 0"""
+    import torch.autograd.forward_ad as fwd
+    from mit_semseg import ops
+    z, label, adv, rows = torch.randn(2, 5, 3, 4), torch.zeros(2, 3, 4, dtype=torch.long), torch.zeros(2), torch.zeros(2, 3, 4)
+    flat = torch.zeros(6)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t.clone(), torch.ones_like(t))           # noqa: E731
+        calls = [lambda: ops.label_log_prob(dual(z), label), lambda: ops.policy_loss(dual(z), label, adv, rows),
+                 lambda: ops.label_log_prob(dual(z.clone().requires_grad_(True)), label),
+                 lambda: ops.policy_loss(z, label, dual(adv), rows), lambda: ops.policy_loss(z, label, adv, dual(rows)),
+                 lambda: ops.policy_loss(z, label, adv, rows, dual(rows)), lambda: ops.grad_norm([flat, dual(flat)]),
+                 lambda: one(ops, 32, dual(flat), flat), lambda: one(ops, 32, flat, dual(flat)), lambda: one(ops, 8, flat, dual(flat)),
+                 lambda: one(ops, 32, flat, flat.clone(), m=dual(flat)), lambda: ops.log_softmax(dual(z))]
+        for grad in (True, False):
+            for call in calls if grad else calls[:-1]:
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    call()
+        # tensors without a tangent are taken inside the level too
+        assert ops.label_log_prob(z, label).shape == label.shape
+        ops.grad_norm([flat])
+    ops.label_log_prob(z, label)
