@@ -590,7 +590,8 @@ int semseg_adamw_step(const semseg_adamw_tensor* tensors_host, int n, const floa
 
 /* the same step with states in 8 bits: m_codes, r_codes: numel e4m3 codes of m and of r = sqrt(v); m_scales, r_scales: one float per
  * 256 elements (ceil(numel / 256)), value = code * scale.  Codes are rounded stochastically from a counter hash of (seed, step, index
- * of the tensor in the call, element): the same call leaves the same bits.  A block that is not finite gets a NaN scale. */
+ * of the tensor in the call, element): the same call leaves the same bits.  A block that is not finite gets a NaN scale.  eps: 0, or a
+ * normal float up to 2^126. */
 typedef struct {
     void* param;
     const void* grad;

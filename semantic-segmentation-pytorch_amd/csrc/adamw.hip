@@ -469,6 +469,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Adam8Entry* __restric
 extern "C" int semseg_adamw8_step(const semseg_adamw8_tensor* tensors_host, int n, const float* lr, double beta1, double beta2, double eps,
                                   float grad_scale, const float* clip, uint32_t seed, void* workspace, size_t workspace_bytes,
                                   void* stream) {
+    if (eps != 0.0 && !(eps >= 0x1p-126 && eps <= 0x1p126)) return SEMSEG_EINVAL;          // the hardware's reciprocal of it would be 0 or infinite
     return adam_step<Adam8Item, Adam8Entry>(tensors_host, n, lr, beta1, beta2, eps, grad_scale, clip, seed, ADAM8_CHUNK, adamw8_kernel,
                                             workspace, workspace_bytes, (hipStream_t)stream);
 }

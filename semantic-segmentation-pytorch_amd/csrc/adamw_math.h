@@ -78,15 +78,19 @@ SEMSEG_HD void adam_update32(float& p, float g, float& m, float& v, const AdamCo
 // Root and reciprocal of the 8-bit step, which has so few bytes an element that instructions bound it.
 // The root decides codes and is rounded to nearest: the hardware's is within one unit of the last place, and of it and its two neighbours
 // the one is taken whose half-unit interval holds x -- (s - u/2)^2 = s (s - u) up to u^2/4, so the sign of x - s (s - u), one rounding,
-// tells.  That is 8 instructions instead of the 17 of a root that also scales the denormals, which count as zero here (a second moment
-// below 1e-38).  The reciprocal only moves the parameter: the hardware's, one unit off at most.
+// tells.  Below 2^-96 that difference would leave the range (and the hardware takes a denormal for zero), so x is scaled by 2^64 there and
+// the root by 2^-32, both exact.  The reciprocal only moves the parameter: the hardware's, one unit off at most, of a sum that is never
+// denormal (the smallest root is 3.7e-23, and semseg_adamw8_step refuses an eps that is).
 #if defined(__HIP_DEVICE_COMPILE__)
-SEMSEG_HD float adam_root(float x) {
+SEMSEG_HD float adam_root(float value) {
+    const bool low = value < 0x1p-96f;
+    const float x = low ? value * 0x1p64f : value;
     const float s = __builtin_amdgcn_sqrtf(x);
     const float down = adam_float(adam_bits(s) - 1u), up = adam_float(adam_bits(s) + 1u);
     float r = fmaf(-down, s, x) <= 0.0f ? down : s;
     r = fmaf(-up, s, x) > 0.0f ? up : r;
-    return x > 0.0f && x < INFINITY ? r : s;
+    r = x > 0.0f && x < INFINITY ? r : s;
+    return low ? r * 0x1p-32f : r;
 }
 SEMSEG_HD float adam_reciprocal(float x) { return __builtin_amdgcn_rcpf(x); }
 #else

@@ -2619,8 +2619,11 @@ def adamw8_step(params, grads, states, steps, weight_decays, lr_tensor, betas=(0
                 copies=None, seed=0):
     """adamw_step with states in 8 bits: `states` holds one AdamW8State (adamw8_state) per parameter, blocks of ADAMW8_BLOCK
     elements share a scale.  The update itself is computed in 32 bits from the decoded states; they are coded again with stochastic
-    rounding whose random bits come from (seed, step count, index in the list, element): the same call gives the same states."""
+    rounding whose random bits come from (seed, step count, index in the list, element): the same call gives the same states.  eps: 0,
+    or a normal float32 up to 2^126."""
     _check_step('adamw8_step', params, lr_tensor, betas, eps, clip)
+    if eps != 0.0 and not 2.0 ** -126 <= eps <= 2.0 ** 126:
+        raise ValueError('adamw8_step: eps must be 0 or lie in [2^-126, 2^126], got %r' % eps)
     table, n = _native.host().adamw8_table('adamw8_step', params, grads, steps, weight_decays, copies, states)
     if n == 0:
         return

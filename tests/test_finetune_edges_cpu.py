@@ -79,3 +79,17 @@ def test_forward_mode_derivatives_are_refused(stub):  # noqa: F811
         assert ops.label_log_prob(z, label).shape == label.shape
         ops.grad_norm([flat])
     ops.label_log_prob(z, label)
+
+
+@pytest.mark.parametrize('eps', [1e-40, 1e-45, 2.0 ** 127])
+def test_adamw8_refuses_an_eps_that_has_no_reciprocal(host, eps):  # noqa: F811
+    """the 8-bit step multiplies by the hardware's reciprocal, which is 0 or infinite there; the 32-bit step divides and takes it"""
+    p = torch.zeros(6)
+    a = [[p], [torch.zeros(6)], [host.adamw8_state(p)], [torch.zeros((), dtype=torch.int32)], [0.0], torch.zeros(1)]
+    with pytest.raises(ValueError, match='eps'):
+        host.adamw8_step(*a, eps=eps)
+    for fine in (0.0, 2.0 ** -126, 2.0 ** 126):
+        with pytest.raises(AssertionError, match='was reached'):
+            host.adamw8_step(*a, eps=fine)
+    with pytest.raises(AssertionError, match='was reached'):
+        host.adamw_step([p], [torch.zeros(6)], [torch.zeros(6)], [torch.zeros(6)], *a[3:], eps=eps)

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.test_finetune_cpu import U32
+from tests.test_finetune_cpu import U32, check_codes, decoded, mix, reference_step
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,46 @@ def test_grad_norm_counts_every_element(dtype, n):
     more = [g, g[:1], g[: n // 2], g[n // 3:]]
     want = math.sqrt(sum(float(t.cpu().double().square().sum()) for t in more))
     assert abs(float(ops.grad_norm(more)[0]) - want) <= (U32 + 1e-10) * want
+
+
+# ----------------------------------------------------------------------------------------------------- AdamW, states in 8 bits
+def placed(t, odd):
+    """on the GPU; `odd`: one element behind an aligned address"""
+    t = t.to(dev())
+    return torch.cat([t[:1], t])[1:] if odd else t
+
+
+def state_of(n, odd):
+    from mit_semseg import ops
+    return ops.AdamW8State(*(placed(torch.zeros(k, dtype=d), odd and d == torch.uint8) for k, d in
+                             ((n, torch.uint8), (-(-n // 256), torch.float32)) * 2))
+
+
+@pytest.mark.parametrize('odd', [False, True])
+@pytest.mark.parametrize('eps', [0.0, 1e-30, 1e-20])
+def test_adamw8_small_second_moments(eps, odd):
+    """gradients whose squares are denormal numbers (below 1.2e-38, down to 1e-42 here), three steps each from the states the one before
+    left: parameters and root against float64.  Beside the roundings that check_step8 counts, the three products and the sum of v are
+    each rounded to a multiple of 2^-149: dv <= 4 * 2^-150, so r and what is divided by it are dv / (2 v) of themselves off"""
+    from mit_semseg import ops
+    n, lr, wd, betas = 900, 1e-2, 0.01, (0.9, 0.999)
+    gen = torch.Generator().manual_seed(31)
+    size = 10 ** (torch.arange(-(-n // 256)).repeat_interleave(256)[:n] * 0.7 - 19.4 + 0.3 * torch.rand(n, generator=gen))
+    g = torch.where(torch.rand(n, generator=gen) < 0.5, -size, size)
+    p, state, step = placed(torch.randn(n, generator=gen), odd), state_of(n, odd), torch.zeros(1, dtype=torch.int32, device=dev())
+    G, lr_t = placed(g, odd), torch.tensor([lr], device=dev())
+    for t in range(1, 4):
+        m0, r0 = decoded([x.cpu() for x in state])
+        p0 = p.cpu()
+        ops.adamw8_step([p], [G], [state], [step], [wd], lr_t, betas, eps, seed=9)
+        rp, rm, rv, move = reference_step(p0, g, m0, r0 * r0, t, float(lr_t), wd, betas, eps)
+        off = 4 * 2.0 ** -150 / (2 * rv)
+        assert float(off.max()) < 0.01 and float(rv.min()) < 1e-40
+        terms = betas[0] * m0.abs() + (1 - betas[0]) * g.double().abs()
+        spread = terms / (1 - betas[0] ** t) * lr / ((rv / (1 - betas[1] ** t)).sqrt() + eps)
+        bound = U32 * rp.abs() + (20 * U32 + 1.02 * off) * (spread + lr * wd * p0.double().abs())
+        assert torch.all((p.cpu().double() - rp).abs() <= bound), float(((p.cpu().double() - rp).abs() / bound).max())
+        bits = mix((torch.arange(n) + mix(9 ^ mix(t ^ mix(0)))) & 0xFFFFFFFF)
+        r = rv.sqrt()
+        check_codes(r, (7 * U32 + 1.02 * off) * r, state[2].cpu(), state[3].cpu(), bits >> 16, True)
+        check_codes(rm, 6 * U32 * terms, state[0].cpu(), state[1].cpu(), bits & 0xFFFF, False)
