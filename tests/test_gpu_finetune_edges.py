@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.test_finetune_cpu import U32, check_codes, decoded, mix, reference_step
+from tests.test_finetune_cpu import U32, check_codes, check_step8, decoded, mix, reference_step
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,84 @@ def test_adamw8_small_second_moments(eps, odd):
         r = rv.sqrt()
         check_codes(r, (7 * U32 + 1.02 * off) * r, state[2].cpu(), state[3].cpu(), bits >> 16, True)
         check_codes(rm, 6 * U32 * terms, state[0].cpu(), state[1].cpu(), bits & 0xFFFF, False)
+
+
+EDGES = ['zero gradient', 'beta 0', 'eps 0', 'inf in a block', 'nan in a block', 'below the smallest scale', 'large']
+
+
+@pytest.mark.parametrize('odd', [False, True])
+@pytest.mark.parametrize('n', [256, 1024, 4096, 5000, 700, 3])
+@pytest.mark.parametrize('case', EDGES)
+def test_adamw8_edges(case, n, odd):
+    """three steps of the kernel itself (its root, reciprocal, conversion and maxima differ from the host's form of the arithmetic)"""
+    from mit_semseg import ops
+    gen = torch.Generator().manual_seed(n)
+    p, g = torch.randn(n, generator=gen), torch.randn(n, generator=gen)
+    betas, eps, wd, hit = (0.9, 0.999), 1e-8, 0.01, n - 2
+    if case == 'zero gradient':
+        g.zero_()
+    elif case == 'beta 0':
+        betas = (0.0, 0.0)
+    elif case == 'eps 0':
+        eps = 0.0
+    elif case.endswith('block'):
+        g[hit] = math.inf if case.startswith('inf') else math.nan
+    elif case.startswith('below'):
+        g = torch.full((n,), 1e-38)
+    else:
+        g *= 1e18
+    P, G, S, step = placed(p, odd), placed(g, odd), state_of(n, odd), torch.zeros(1, dtype=torch.int32, device=dev())
+    lr = torch.tensor([1e-2], device=dev())
+    for t in range(1, 4):
+        m0, r0 = decoded([x.cpu() for x in S])
+        p0 = P.cpu()
+        ops.adamw8_step([P], [G], [S], [step], [wd], lr, betas, eps, seed=4)
+        assert int(step) == t
+        got = [x.cpu() for x in S]
+        if case == 'zero gradient':
+            assert all(torch.all(x.float() == 0) for x in got)
+            assert torch.all((P.cpu().double() - p0.double() * (1 - float(lr) * wd)).abs() <= 2 * U32 * p0.double().abs())
+            continue
+        if case.startswith('below'):
+            assert all(torch.all(x.float() == 0) for x in (got[0] & 0x7f, got[1], got[3])) and torch.isfinite(P).all()
+            continue
+        if not case.endswith('block'):
+            check_step8(p0, g, m0, r0, P.cpu(), got, t, float(lr), wd, betas, eps, 4, 0)
+            continue
+        # the block with the number that is not finite decodes to NaN, the others are right
+        b = hit // 256
+        m, r = decoded(got)
+        bad = torch.zeros(n, dtype=torch.bool)
+        bad[b * 256:b * 256 + 256] = True
+        assert torch.isnan(m[bad]).all() and torch.isnan(r[bad]).all() and torch.isnan(got[1][b]) and torch.isnan(got[3][b])
+        assert torch.isfinite(m[~bad]).all() and torch.isfinite(r[~bad]).all() and torch.isfinite(P.cpu()[~bad]).all()
+        if t == 1:                                                    # the step itself still takes the block's other elements
+            keep = torch.arange(n) != hit
+            assert torch.isfinite(P.cpu()[keep]).all()
+        if b:
+            check_step8(p0[:b * 256], g[:b * 256], m0[:b * 256], r0[:b * 256], P.cpu()[:b * 256],
+                        [x[:b * 256] if x.numel() == n else x[:b] for x in got], t, float(lr), wd, betas, eps, 4, 0)
+
+
+def test_adamw8_codes_are_the_definition_s():
+    """4 M values of each sign convention: with both betas 0 the states are the gradient and its size, and every code equals the rounding
+    of value / scale as bit operations define it (16 random bits added below the last of 3 mantissa bits), to the bit"""
+    from mit_semseg import ops
+    n = 1 << 22
+    gen = torch.Generator(device=dev()).manual_seed(3)
+    g = torch.randn(n, generator=gen, device=dev()) * 10 ** (4 * torch.rand(n, generator=gen, device=dev()) - 4)
+    p, step, S = torch.zeros(n, device=dev()), torch.zeros(1, dtype=torch.int32, device=dev()), state_of(n, False)
+    ops.adamw8_step([p], [g], [S], [step], [0.0], torch.zeros(1, device=dev()), (0.0, 0.0), 1e-8, seed=12)
+    bits = mix((torch.arange(n, device=dev()) + mix(12 ^ mix(1 ^ mix(0)))) & 0xFFFFFFFF)
+    r = (g * g).sqrt()
+    for x, u, codes, scale, low in ((g, bits & 0xFFFF, S[0], S[1], 0.0), (r, bits >> 16, S[2], S[3], 2.0 ** -9)):
+        top = x.abs().view(-1, 256).amax(1)
+        want = top * torch.tensor(1.0 / 448.0, device=dev())
+        assert torch.equal(scale, want)
+        a = (x * (1.0 / want).repeat_interleave(256)).clamp(-448.0, 448.0)
+        if low:
+            a = torch.where(x > 0, a.clamp(min=low), a)
+        add = torch.where(a.abs() < 2.0 ** -6, torch.full_like(a, 2.0 ** -6), torch.zeros_like(a))
+        size = ((((a.abs() + add).view(torch.int32).long() + (u << 4)) & ~0xFFFFF).int().view(torch.float32)) - add
+        got = codes.view(torch.float8_e4m3fn).float()
+        assert torch.equal(got, torch.copysign(size, a))
