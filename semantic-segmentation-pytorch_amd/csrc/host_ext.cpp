@@ -13,6 +13,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -269,17 +270,29 @@ typedef int (*ScaleBy)(float*, int64_t, const float*, void*);
 void* stream_of(const at::Tensor& t) {
     return t.is_cuda() ? (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream() : nullptr;
 }
+// number of the recording (stream capture) that calls on this tensor go into now, 0 for none
+unsigned long long recording_of(const at::Tensor& t) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (!t.is_cuda() || hipStreamGetCaptureInfo((hipStream_t)stream_of(t), &status, &id) != hipSuccess) return 0;
+    return status == hipStreamCaptureStatusActive ? id : 0;
+}
 void check(int rc, const char* what) {
     TORCH_CHECK(rc == 0, what, " failed with code ", rc, rc >= 900 && rc <= 908 ? " (stream capture)" : "");
 }
 
 // d logits of label_log_prob (kept: {maximum, log sum} per row) and of policy_loss (kept: scratch, the same, gradient per row, 1 / rows
-// that count; `written`: the gradient for an upstream gradient of 1, where the forward pass has written it)
+// that count; `written`: the gradient for an upstream gradient of 1, where the forward pass has written it).
+// `written` is scaled in place and handed out, so it is taken only where the forward pass runs once for every backward pass: both eager, or
+// both in one recording.  A recorded forward pass would write over a gradient that an eager backward pass has handed out.  A backward pass
+// that is recorded while its forward pass was eager is refused: every replay would scale `written` once more, and what is kept for it is the
+// eager pass's memory, free for other tensors once the node is gone.
 struct RowsBackward : public torch::autograd::Node {
     torch::autograd::SavedVariable z, label, kept;
     at::Tensor written;
     std::vector<int64_t> shape, strides;              // of the logits, and of `z`
     int64_t ld = 0, ignore = 0;
+    unsigned long long recording = 0;                 // of the forward pass
     bool loss = false;
     LogpBackward logp_bwd = nullptr;
     ScaleBy scale_by = nullptr;
@@ -300,7 +313,9 @@ struct RowsBackward : public torch::autograd::Node {
             zt = z.unpack(shared_from_this());
             lab = label.unpack(shared_from_this());
             keep = kept.unpack(shared_from_this());
-            std::swap(dz, written);
+            const auto now = recording_of(zt);
+            TORCH_CHECK(!now || recording, name(), ": a backward pass cannot be recorded apart from its forward pass: record both");
+            if (now == recording) std::swap(dz, written);
         }
         {
             at::AutoDispatchBelowADInplaceOrView below;
@@ -367,6 +382,7 @@ PyObject* attach_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
         node->label = torch::autograd::SavedVariable(tensor(args[3], what), false);
         node->kept = torch::autograd::SavedVariable(tensor(args[4], what), false);
         if (args[5] != Py_None) node->written = tensor(args[5], what);
+        node->recording = recording_of(z);
         node->ld = PyLong_AsLongLong(args[6]);
         node->ignore = PyLong_AsLongLong(args[7]);
         node->loss = PyObject_IsTrue(args[8]) == 1;

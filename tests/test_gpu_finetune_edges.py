@@ -161,3 +161,79 @@ def test_adamw8_codes_are_the_definition_s():
         size = ((((a.abs() + add).view(torch.int32).long() + (u << 4)) & ~0xFFFFF).int().view(torch.float32)) - add
         got = codes.view(torch.float8_e4m3fn).float()
         assert torch.equal(got, torch.copysign(size, a))
+
+
+# ----------------------------------------------------------------------------------- forward and backward pass recorded apart
+def loss_inputs(seed, shape=(2, 150, 24, 30)):
+    n, c, h, w = shape
+    g = torch.Generator().manual_seed(seed)
+    z = (2 * torch.randn(n, h, w, c, generator=g)).to(dev()).permute(0, 3, 1, 2).requires_grad_(True)       # its gradient is written by the forward pass
+    label = torch.randint(-1, c, (n, h, w), generator=g).to(dev())
+    return z, label, torch.randn(n, generator=g).to(dev()), (-5 + 0.3 * torch.randn(n, h, w, generator=g)).to(dev())
+
+
+def close(a, b):
+    """the same gradient, p from its row's sum in one and from the kept parts in the other: within the roundings of p that the tests of
+    the gradient count (its exponent's, up to 3 (d + log) + 2 log C + 90, with d below 20 here), per row of the largest factor"""
+    scale = b.abs().amax(dim=1, keepdim=True)
+    return bool(torch.all((a - b).abs() <= 2 * U32 * (3 * 20.0 + 3 * math.log(150) + 2 * math.log(150) + 90) * scale))
+
+
+def test_recorded_backward_of_an_eager_loss_is_refused():
+    """every replay would scale the gradient that the forward pass has written once more; the eager backward pass goes on"""
+    from mit_semseg import ops
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):                          # a leaf that has been used on the recording's stream alone
+        z, label, adv, old = loss_inputs(40)
+        x = z.detach().clone(memory_format=torch.preserve_format).requires_grad_(True)
+        want = torch.autograd.grad(ops.policy_loss(x, label, adv, old)[0], x)[0]
+        loss, lp = ops.policy_loss(z, label, adv, old)[0], ops.label_log_prob(z, label)
+        up, ups = torch.ones((), device=dev()), torch.ones_like(lp)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        for out, g in ((loss, up), (lp, ups)):
+            with pytest.raises(RuntimeError, match='recorded apart'):
+                torch.autograd.grad(out, z, grad_outputs=g, retain_graph=True)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = torch.autograd.grad(loss, z)[0]
+    torch.cuda.synchronize()
+    assert close(got, want)
+
+
+def test_eager_backward_of_a_recorded_loss():
+    """gradients that were handed out stay what they are when the recorded loss is replayed on other logits"""
+    from mit_semseg import ops
+    z, label, adv, old = loss_inputs(41)
+    values = [loss_inputs(s)[0].detach() for s in (42, 43, 44)]
+    ops.policy_loss(z, label, adv, old)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        loss = ops.policy_loss(z, label, adv, old)[0]
+    got = []
+    for v in values:
+        z.data.copy_(v)
+        graph.replay()
+        got.append(torch.autograd.grad(loss, z, retain_graph=True)[0])
+        torch.cuda.synchronize()
+    for v, dz in zip(values, got):
+        x = v.clone(memory_format=torch.preserve_format).requires_grad_(True)
+        assert close(dz, torch.autograd.grad(ops.policy_loss(x, label, adv, old)[0], x)[0])
+
+
+def test_one_recording_still_hands_out_what_the_forward_pass_wrote():
+    """forward and backward pass in one recording: the bits of the eager pass"""
+    from mit_semseg import ops
+    z, label, adv, old = loss_inputs(45)
+    values = [loss_inputs(s)[0].detach() for s in (46, 47, 48)]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        dz = torch.autograd.grad(0.25 * ops.policy_loss(z, label, adv, old)[0], z)[0]
+    for v in values:
+        z.data.copy_(v)
+        graph.replay()
+        x = v.clone(memory_format=torch.preserve_format).requires_grad_(True)
+        assert torch.equal(dz, torch.autograd.grad(0.25 * ops.policy_loss(x, label, adv, old)[0], x)[0])
+        torch.cuda.synchronize()
