@@ -95,7 +95,6 @@ def _build_locked(force, verbose):
         if force or _stale(src, obj):
             # -MMD: the compiler lists every user header it read (csrc/*.h, include/semseg_hip.h) in obj.d; no hand-kept list
             jobs.append((obj, [HIPCC] + FLAGS + ['-MMD', '-MF', obj + '.d' + tag, '-c', src, '-o', obj + tag]))
-    objects = len(jobs)
     if force or _stale(HOST_SRC, HOST_LIB):
         jobs.append((HOST_LIB, _host_command(HOST_LIB + tag, HOST_LIB + '.d' + tag)))
     if jobs:
@@ -106,7 +105,8 @@ def _build_locked(force, verbose):
             os.replace(obj + tag, obj)
         with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as ex:
             list(ex.map(run, jobs))
-    if objects or not os.path.exists(LIB):
+    # by the files' times and not by what this call has compiled: an earlier call may have ended between its objects and the link
+    if force or any(_newer(obj, LIB) for obj in objs):
         _run([HIPCC, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', LIB + tag] + objs + ['-ldl'], verbose)
         os.replace(LIB + tag, LIB)
     return LIB

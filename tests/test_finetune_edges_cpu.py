@@ -93,3 +93,59 @@ def test_adamw8_refuses_an_eps_that_has_no_reciprocal(host, eps):  # noqa: F811
             host.adamw8_step(*a, eps=fine)
     with pytest.raises(AssertionError, match='was reached'):
         host.adamw_step([p], [torch.zeros(6)], [torch.zeros(6)], [torch.zeros(6)], *a[3:], eps=eps)
+
+
+def test_a_failed_host_job_does_not_leave_a_stale_library(tmp_path, monkeypatch):
+    """both kinds of job are stale, the host extension's fails after the kernels' objects are in place: the next build links them"""
+    import importlib.util
+    import os
+    import subprocess
+    import time
+    from tests.conftest import PKG
+    spec = importlib.util.spec_from_file_location('build_native_under_test', os.path.join(PKG, 'build_native.py'))
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    for name in ('a.hip', 'b.hip', 'host_ext.cpp'):
+        (tmp_path / name).write_text('')
+    for name, value in dict(CSRC=str(tmp_path), OUT_DIR=str(tmp_path), LIB=str(tmp_path / 'lib.so'), SOURCES=['a.hip', 'b.hip'],
+                            HOST_SRC=str(tmp_path / 'host_ext.cpp'), HOST_LIB=str(tmp_path / '_host.so')).items():
+        monkeypatch.setattr(b, name, value)
+    ran, broken, clock = [], [], [time.time() + 100.0]
+
+    def touch(path):                                                  # every file written is a second younger than the one before
+        clock[0] += 1.0
+        with open(path, 'a'):
+            os.utime(path, (clock[0], clock[0]))
+
+    def run(cmd, verbose):
+        out = cmd[cmd.index('-o') + 1]
+        what = os.path.basename(out).split('.tmp')[0]
+        ran.append(what)
+        if what in broken:
+            raise subprocess.CalledProcessError(1, cmd)
+        touch(out)
+        if '-MF' in cmd:
+            with open(cmd[cmd.index('-MF') + 1], 'w') as f:
+                f.write('x: %s\n' % (cmd[cmd.index('-c') + 1] if '-c' in cmd else b.HOST_SRC))
+    monkeypatch.setattr(b, '_run', run)
+    monkeypatch.setattr(b.os, 'cpu_count', lambda: 1)                 # one job after the other
+
+    def build(fails=()):
+        ran.clear()
+        broken[:] = fails
+        if fails:
+            with pytest.raises(subprocess.CalledProcessError):
+                b.build(verbose=False)
+        else:
+            b.build(verbose=False)
+        return sorted(ran)
+    assert build() == ['_host.so', 'a.o', 'b.o', 'lib.so'] and build() == []
+    for name in ('a.hip', 'host_ext.cpp'):
+        touch(str(tmp_path / name))
+    assert build(['_host.so']) == ['_host.so', 'a.o']
+    assert build() == ['_host.so', 'lib.so'] and build() == []        # the object that is newer than the library goes into it
+    touch(str(tmp_path / 'b.hip'))
+    assert build(['lib.so']) == ['b.o', 'lib.so']                     # a link that failed is tried again
+    assert build() == ['lib.so'] and build() == []
+    touch(str(tmp_path / 'host_ext.cpp'))
+    assert build() == ['_host.so']                                    # the extension alone needs no link
