@@ -4,6 +4,7 @@ mit_semseg/models/models.py:9-586), executing on the HIP operators of mit_semseg
 
 Layout: tensors crossing this API keep the reference's logical [N,C,H,W] shape; memory is NHWC.
 """
+import contextlib
 import os
 
 import torch
@@ -25,11 +26,38 @@ class SegmentationModuleBase(nn.Module):
         return acc
 
 
+@contextlib.contextmanager
+def _repeatable(module, keep_statistics=False):
+    """a forward pass of a policy that can be made again on the same batch with the same result: the dropout of modules in training mode is
+    off (old log probabilities and the loss would each draw a mask of their own), and with `keep_statistics` their BatchNorms, which
+    normalise with the batch's statistics all the same, update scratch memory instead of the running statistics"""
+    dropped, kept = [], []
+    for m in module.modules():
+        if not m.training:
+            continue
+        if isinstance(m, (Dropout2d, nn.modules.dropout._DropoutNd)):
+            dropped.append(m)
+        elif keep_statistics and m._buffers.get('running_mean') is not None:
+            kept.append((m._buffers, {k: m._buffers[k] for k in ('running_mean', 'running_var', 'num_batches_tracked')}))
+    try:
+        for m in dropped:
+            m.training = False
+        for buffers, own in kept:
+            buffers.update({k: torch.empty_like(t) for k, t in own.items()})
+        yield
+    finally:
+        for m in dropped:
+            m.training = True
+        for buffers, own in kept:
+            buffers.update(own)
+
+
 class PolicyLoss(nn.Module):
     """Criterion of SegmentationModule for tuning a trained network on a reward (a metric of whole label maps, say) instead of labels:
     the label map is one that was sampled from the network, `advantage` what it earned (per image or per pixel), and the loss is the
     clipped policy loss with a KL term of ops.policy_loss.  forward(scores, label, advantage, old_logp, ref_logp) -> loss; `kl` and
-    `clipped` are the mean KL term and the share of clipped pixels of the last step, replayed or not (views of one buffer)."""
+    `clipped` are the mean KL term and the share of clipped pixels of the last step, replayed or not (views of one buffer).  Dropout takes
+    no part in a step with this criterion, so the first one on a fresh draw has ratios of 1."""
 
     def __init__(self, clip_low=0.2, clip_high=0.2, kl_weight=0.0, ignore_index=-1):
         super(PolicyLoss, self).__init__()
@@ -79,19 +107,27 @@ class SegmentationModule(SegmentationModuleBase):
 
     def label_log_prob(self, feed_dict):
         """[N, H, W] log probability of every pixel of feed_dict['seg_label'] under the network (its scores are at the labels' size);
-        pixels that the criterion ignores give 0"""
-        feats = self.encoder(feed_dict['img_data'], return_feature_maps=True)
-        return ops.label_log_prob(self._main_scores(feats), feed_dict['seg_label'], getattr(self.crit, 'ignore_index', -1))
+        pixels that the criterion ignores give 0.  In training mode it is the policy that a step with a PolicyLoss on the same batch starts
+        from: BatchNorm normalises with the batch's statistics, dropout is off, and the running statistics stay as they are.  In eval mode
+        (where a frozen reference network belongs) the running statistics are used."""
+        if isinstance(feed_dict, (list, tuple)):
+            feed_dict = feed_dict[0]
+        with _repeatable(self, keep_statistics=True):
+            feats = self.encoder(feed_dict['img_data'], return_feature_maps=True)
+            scores = self._main_scores(feats)
+        return ops.label_log_prob(scores, feed_dict['seg_label'], getattr(self.crit, 'ignore_index', -1))
 
     def forward(self, feed_dict, *, segSize=None):
         if isinstance(feed_dict, (list, tuple)):      # UserScatteredDataParallel passes a 1-element list per GPU
             feed_dict = feed_dict[0]
-        feats = self.encoder(feed_dict['img_data'], return_feature_maps=True)
+        policy = isinstance(self.crit, PolicyLoss) and segSize is None
+        with _repeatable(self) if policy else contextlib.nullcontext():
+            feats = self.encoder(feed_dict['img_data'], return_feature_maps=True)
+            pred = self._main_scores(feats) if policy else None
         if segSize is not None:                       # inference
             return self.decoder(feats, segSize=segSize)
         label = feed_dict['seg_label']
-        if isinstance(self.crit, PolicyLoss):         # the label map was drawn from the main head: an auxiliary one takes no part
-            pred = self._main_scores(feats)
+        if policy:                                    # the label map was drawn from the main head: an auxiliary one takes no part
             loss = self.crit(pred, label, feed_dict['advantage'], feed_dict['old_logp'], feed_dict.get('ref_logp'))
             return loss, self.pixel_acc(pred.detach(), label)
         if self.deep_sup_scale is not None:           # deep supervision

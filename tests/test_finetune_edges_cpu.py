@@ -149,3 +149,55 @@ def test_a_failed_host_job_does_not_leave_a_stale_library(tmp_path, monkeypatch)
     assert build() == ['lib.so'] and build() == []
     touch(str(tmp_path / 'host_ext.cpp'))
     assert build() == ['_host.so']                                    # the extension alone needs no link
+
+
+def _module(crit, arch='ppm_deepsup'):
+    from mit_semseg.models import ModelBuilder, SegmentationModule, resnet
+    from mit_semseg.models.models import ResnetDilated
+    enc = ResnetDilated(resnet.resnet18(pretrained=False), 8)
+    return SegmentationModule(enc, ModelBuilder.build_decoder(arch, fc_dim=512, num_class=150), crit, 0.4).train()
+
+
+def _feed():
+    return {'img_data': torch.randn(2, 3, 64, 64), 'seg_label': torch.randint(-1, 150, (2, 8, 8)), 'advantage': torch.randn(2),
+            'old_logp': torch.randn(2, 8, 8), 'ref_logp': torch.randn(2, 8, 8)}
+
+
+def test_log_probabilities_leave_the_module_as_it_was(stub, monkeypatch):  # noqa: F811
+    """in training mode: the running statistics that the kernels get are not the module's, no dropout mask is drawn, and everything is
+    back in its place afterwards, after an error too"""
+    from mit_semseg import ops
+    from mit_semseg.models import PolicyLoss
+    sm = _module(PolicyLoss())
+    own = {k: (t, t.clone()) for k, t in sm.named_buffers()}
+    statistics = {t.data_ptr() for k, (t, _) in own.items() if 'running' in k or 'num_batches' in k}
+    seen, real = [], ops._p
+    monkeypatch.setattr(ops, '_p', lambda t: (seen.append(t.data_ptr()) if t is not None else None, real(t))[1])
+    for call in (lambda: sm.label_log_prob(_feed()), lambda: sm.label_log_prob([_feed()])):
+        with torch.no_grad():
+            assert call().shape == (2, 8, 8)
+    assert seen and not statistics & set(seen)
+    assert not any('dropout' in n or 'scale_nc' in n for n in stub.calls)
+
+    def back():
+        for k, t in sm.named_buffers():
+            assert t is own[k][0] and torch.equal(t, own[k][1]), k
+        assert all(m.training for m in sm.modules())
+    back()
+    monkeypatch.setattr(sm.decoder, 'forward', lambda *a, **k: 1 // 0)
+    with pytest.raises(ZeroDivisionError):
+        sm.label_log_prob(_feed())
+    back()
+    monkeypatch.undo()
+
+
+def test_dropout_takes_no_part_in_a_policy_step(stub):  # noqa: F811
+    import torch.nn as nn
+    from mit_semseg.engine import TrainStep
+    from mit_semseg.models import PolicyLoss
+    for crit, dropped in ((PolicyLoss(), False), (nn.NLLLoss(ignore_index=-1), True)):
+        sm = _module(crit)
+        stub.calls.clear()
+        TrainStep(sm, max_iters=10, optim='AdamW', lr_encoder=1e-4, lr_decoder=1e-4).step(_feed())
+        assert any('scale_nc' in n for n in stub.calls) == dropped
+        assert all(m.training for m in sm.modules())

@@ -237,3 +237,34 @@ def test_one_recording_still_hands_out_what_the_forward_pass_wrote():
         x = v.clone(memory_format=torch.preserve_format).requires_grad_(True)
         assert torch.equal(dz, torch.autograd.grad(0.25 * ops.policy_loss(x, label, adv, old)[0], x)[0])
         torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------------------------ tuning a network
+@pytest.mark.parametrize('graph', [False, True])
+def test_a_fresh_draw_starts_from_ratio_one_whatever_the_decoder_drops(graph):
+    """ppm_deepsup drops channels in training: the first step after taking the log probabilities still has the policy that was asked.  Two
+    forward passes of one network differ by less than 5e-4 in a log probability (each is within 2.3e-4 of the reference's), so the KL
+    term against them is below 0.5 d^2 = 1.25e-7 and no ratio is near a border; and asking moves no running statistics"""
+    import torch.nn as nn
+    from mit_semseg.engine import TrainStep
+    from mit_semseg.models import ModelBuilder, PolicyLoss, SegmentationModule, resnet
+    from mit_semseg.models.models import ResnetDilated
+    torch.manual_seed(7)
+    enc = ResnetDilated(resnet.resnet18(pretrained=False), 8)
+    dec = ModelBuilder.build_decoder('ppm_deepsup', fc_dim=512, num_class=150)
+    sm = SegmentationModule(enc, dec, nn.NLLLoss(ignore_index=-1), 0.4).to(dev()).train()
+    sm.crit = PolicyLoss(kl_weight=0.1).to(dev())
+    ts = TrainStep(sm, lr_encoder=1e-5, lr_decoder=1e-4, max_iters=100, optim='AdamW', graph=graph)
+    g = torch.Generator().manual_seed(8)
+    for it in range(5):
+        feed = {'img_data': torch.randn(2, 3, 64, 96, generator=g).to(dev()), 'seg_label': torch.randint(-1, 150, (2, 8, 12), generator=g).to(dev()),
+                'advantage': torch.ones(2, device=dev())}
+        before = {k: t.clone() for k, t in sm.state_dict().items()}
+        with torch.no_grad():
+            lp = sm.label_log_prob(feed)
+        for k, t in sm.state_dict().items():
+            assert torch.equal(t, before[k]), k
+        loss, _ = ts.step(dict(feed, old_logp=lp, ref_logp=lp))
+        assert float(sm.crit.clipped) == 0.0 and 0.0 <= float(sm.crit.kl) <= 1.25e-7 and abs(float(loss) + 1.0) <= 5e-4
+        assert not torch.equal(sm.state_dict()['encoder.bn1.running_mean'], before['encoder.bn1.running_mean'])
+    assert not graph or ts.stats['replayed'] >= 3
