@@ -107,6 +107,11 @@ class FusedAdamW:
     set_lr = FusedSGD.set_lr
     zero_grad = FusedSGD.zero_grad
 
+    def host_numbers(self):
+        """what a step hands to the kernels as numbers (and a recording of it keeps): a change of one needs a new recording"""
+        return (*map(float, self.betas), float(self.eps), None if self.max_norm is None else float(self.max_norm), self.seed,
+                *(float(g['weight_decay']) for g in self.groups))
+
     def step(self, grad_scale=1.0):
         live = [[p for p in g['params'] if p.grad is not None] for g in self.groups]
         grads = [p.grad for ps in live for p in ps]
@@ -376,6 +381,13 @@ class TrainStep:
             tl.mark('step_end')
         return loss.detach(), acc.detach()
 
+    def _key(self, feed):
+        """what one recording stands for: the feed's shapes and the numbers that the criterion (a PolicyLoss) and the optimiser (AdamW)
+        hand to the kernels.  A number changed between steps is a new recording; what changes at every step belongs into device memory,
+        as the learning rate does."""
+        numbers = [n() for n in (getattr(o, 'host_numbers', None) for o in (getattr(self.sm, 'crit', None), self.opt)) if n is not None]
+        return feed_key(feed) + tuple(numbers)
+
     def _host_state(self):
         """what a recording pass changes on the HOST (it executes nothing on the device): restored before the eager retry of a
         refused first-sight recording, so that the retry is the step the caller asked for, not the one after it"""
@@ -431,7 +443,7 @@ class TrainStep:
         if mode == 'eager':
             self.stats['eager'] += 1
             return self._eager(feed)
-        key = feed_key(feed)
+        key = self._key(feed)
         rec = self._graphs.get(key)
         if rec is None:
             seen = self._seen.get(key, 0)

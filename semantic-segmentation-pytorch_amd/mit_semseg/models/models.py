@@ -72,6 +72,10 @@ class PolicyLoss(nn.Module):
     def clipped(self):
         return self.scalars[1]
 
+    def host_numbers(self):
+        """what the loss hands to its kernels as numbers: engine.TrainStep records a step anew when one is changed"""
+        return float(self.clip_low), float(self.clip_high), float(self.kl_weight), int(self.ignore_index)
+
     def forward(self, scores, label, advantage, old_logp, ref_logp=None):
         return ops.policy_loss(scores, label, advantage, old_logp, ref_logp, self.clip_low, self.clip_high, self.kl_weight,
                                self.ignore_index, self.scalars)[0]

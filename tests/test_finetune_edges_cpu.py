@@ -201,3 +201,33 @@ def test_dropout_takes_no_part_in_a_policy_step(stub):  # noqa: F811
         TrainStep(sm, max_iters=10, optim='AdamW', lr_encoder=1e-4, lr_decoder=1e-4).step(_feed())
         assert any('scale_nc' in n for n in stub.calls) == dropped
         assert all(m.training for m in sm.modules())
+
+
+def test_changed_numbers_are_another_recording(monkeypatch):
+    """what the criterion and AdamW hand to the kernels as numbers is part of what a recorded step is looked up by"""
+    import torch.nn as nn
+    from mit_semseg.models import PolicyLoss
+    from tests import test_graph_policy_cpu as policy
+    ts, log = policy._step(monkeypatch, True)
+    from mit_semseg.engine import FusedAdamW
+    p = [[nn.Parameter(torch.zeros(3))] for _ in range(2)]
+    ts.sm.crit = PolicyLoss(kl_weight=0.1)
+    ts.opt = FusedAdamW([dict(params=q, lr=0.1, weight_decay=0.0) for q in p], max_norm=1.0)
+    changes = [(ts.sm.crit, 'kl_weight', 0.2), (ts.sm.crit, 'clip_low', 0.3), (ts.sm.crit, 'clip_high', 0.1), (ts.sm.crit, 'ignore_index', 255),
+               (ts.opt, 'max_norm', 2.0), (ts.opt, 'betas', (0.8, 0.999)), (ts.opt, 'eps', 1e-6), (ts.opt.groups[1], 'weight_decay', 0.5)]
+    for _ in range(4):
+        policy._run(ts, log, [(4, 4)])
+    recorded = [e for e in log if e[0] == 'capture']
+    assert len(recorded) == 1 and log[-1][0] == 'replay'
+    for k, (of, name, value) in enumerate(changes):
+        old = of[name] if isinstance(of, dict) else getattr(of, name)
+        put = of.__setitem__ if isinstance(of, dict) else lambda n, v: setattr(of, n, v)
+        put(name, value)
+        policy._run(ts, log, [(4, 4), (4, 4)])
+        assert len([e for e in log if e[0] == 'capture']) == 2 + k, name
+        put(name, old)
+        policy._run(ts, log, [(4, 4)])                                # the first recording still stands for the first numbers
+        assert len([e for e in log if e[0] == 'capture']) == 2 + k and log[-1][0] == 'replay', name
+    ts.opt.set_lr(0, 0.7)
+    policy._run(ts, log, [(4, 4)])
+    assert len([e for e in log if e[0] == 'capture']) == 1 + len(changes)         # the learning rate is device memory

@@ -268,3 +268,34 @@ def test_a_fresh_draw_starts_from_ratio_one_whatever_the_decoder_drops(graph):
         assert float(sm.crit.clipped) == 0.0 and 0.0 <= float(sm.crit.kl) <= 1.25e-7 and abs(float(loss) + 1.0) <= 5e-4
         assert not torch.equal(sm.state_dict()['encoder.bn1.running_mean'], before['encoder.bn1.running_mean'])
     assert not graph or ts.stats['replayed'] >= 3
+
+
+def test_numbers_changed_between_replays():
+    """KL weight, clip range and gradient bound that a program changes between steps act on the next step, recorded or not"""
+    import torch.nn as nn
+    from mit_semseg.engine import TrainStep
+    from mit_semseg.models import ModelBuilder, PolicyLoss, SegmentationModule, resnet
+    from mit_semseg.models.models import ResnetDilated
+    rows = []
+    for graph in (False, True):
+        torch.manual_seed(9)
+        enc = ResnetDilated(resnet.resnet18(pretrained=False), 8)
+        sm = SegmentationModule(enc, ModelBuilder.build_decoder('c1', fc_dim=512, num_class=150), PolicyLoss(kl_weight=0.05)).to(dev()).train()
+        ts = TrainStep(sm, lr_encoder=1e-5, lr_decoder=1e-4, max_iters=100, optim='AdamW', clip_grad_norm=0.5, graph=graph)
+        g = torch.Generator().manual_seed(10)
+        feed = {'img_data': torch.randn(2, 3, 64, 96, generator=g).to(dev()), 'seg_label': torch.randint(-1, 150, (2, 8, 12), generator=g).to(dev()),
+                'advantage': torch.randn(2, generator=g).to(dev()), 'old_logp': (-5 + 0.5 * torch.randn(2, 8, 12, generator=g)).to(dev()),
+                'ref_logp': (-5 + 0.5 * torch.randn(2, 8, 12, generator=g)).to(dev())}
+        seen = []
+        for it in range(9):
+            if it == 4:
+                sm.crit.kl_weight = 5.0
+            elif it == 6:
+                sm.crit.clip_low, ts.opt.max_norm = 0.9, 0.01
+            elif it == 8:
+                sm.crit.kl_weight, sm.crit.clip_low, ts.opt.max_norm = 0.05, 0.2, 0.5
+            loss, _ = ts.step(feed)
+            seen.append(torch.stack([loss, sm.crit.kl, sm.crit.clipped, *ts.opt.clip]).clone())
+        rows.append(torch.stack(seen))
+    assert ts.stats['captured'] == 3 and ts.stats['replayed'] == 7, ts.stats
+    assert torch.equal(rows[0], rows[1])
