@@ -139,6 +139,18 @@ def train_epoch(step, iterator, history, epoch, cfg, rank, group=None):
         tic = time.time()
 
 
+def optimiser_of(cfg, rank=0):
+    """TRAIN.optim as TrainStep takes it.  The reference keeps the option and never reads it (its optimiser is SGD whatever it says,
+    train.py:115-127), so a configuration that names another one than those built here goes on training with SGD, and is told so."""
+    from .engine import OPTIMISERS
+    name = str(cfg.TRAIN.optim)
+    if name.lower() in OPTIMISERS:
+        return name
+    if rank == 0:
+        print('TRAIN.optim {} is none of SGD, AdamW, AdamW8bit: training with SGD'.format(name))
+    return 'SGD'
+
+
 def train_worker(rank, world, cfg, gpus, port):
     """one rank of train.py:142-205"""
     import random
@@ -165,7 +177,7 @@ def train_worker(rank, world, cfg, gpus, port):
         print('1 Epoch = {} iters'.format(cfg.TRAIN.epoch_iters))
     max_iters = cfg.TRAIN.epoch_iters * cfg.TRAIN.num_epoch
     step = TrainStep(sm, lr_encoder=cfg.TRAIN.lr_encoder, lr_decoder=cfg.TRAIN.lr_decoder, momentum=cfg.TRAIN.beta1,
-                     weight_decay=cfg.TRAIN.weight_decay, lr_pow=cfg.TRAIN.lr_pow, max_iters=max_iters, graph=True, optim=cfg.TRAIN.optim,
+                     weight_decay=cfg.TRAIN.weight_decay, lr_pow=cfg.TRAIN.lr_pow, max_iters=max_iters, graph=True, optim=optimiser_of(cfg, rank),
                      beta2=cfg.TRAIN.beta2, eps=cfg.TRAIN.eps, clip_grad_norm=cfg.TRAIN.clip_grad_norm or None)
     step.iter = cfg.TRAIN.start_epoch * cfg.TRAIN.epoch_iters          # cur_iter of train.py:35
     history = {'train': {'epoch': [], 'loss': [], 'acc': []}}

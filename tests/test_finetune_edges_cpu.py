@@ -231,3 +231,18 @@ def test_changed_numbers_are_another_recording(monkeypatch):
     ts.opt.set_lr(0, 0.7)
     policy._run(ts, log, [(4, 4)])
     assert len([e for e in log if e[0] == 'capture']) == 1 + len(changes)         # the learning rate is device memory
+
+
+@pytest.mark.parametrize('name,taken', [('SGD', 'SGD'), ('AdamW8bit', 'AdamW8bit'), ('adamw', 'adamw'), ('Adam', 'SGD'), ('', 'SGD')])
+def test_configurations_that_trained_before_still_do(stub, name, taken, capsys):  # noqa: F811
+    """the reference ignores TRAIN.optim, and so did train.py: a name that is not built here means SGD, with a line that says so"""
+    from mit_semseg import drivers
+    from mit_semseg.config import load
+    from mit_semseg.engine import TrainStep
+    cfg = load('preset:ade20k-resnet18dilated-ppm_deepsup', ['TRAIN.optim', name])
+    assert drivers.optimiser_of(cfg) == taken
+    said = capsys.readouterr().out
+    assert ('training with SGD' in said) == (name in ('Adam', ''))
+    drivers.optimiser_of(cfg, 1)
+    assert capsys.readouterr().out == ''
+    TrainStep(_module(None), optim=drivers.optimiser_of(cfg, 1))
