@@ -247,22 +247,22 @@ def host():
     return _host
 
 
-_addresses = {}
+_addresses = {}             # (name, entry point) -> (its address, what keeps that alive)
 
 
 def address(name):
-    """where the entry point `name` of lib() starts, for the extension to call; an entry point that is a Python function (a stub of
-    the CPU tests) is wrapped"""
+    """where the entry point `name` of lib() starts, for the extension to call.  An entry point that is a Python function (lib() replaced by
+    an object of such) gets one C wrapper, kept like the address itself."""
     fn = getattr(lib(), name)
-    if isinstance(fn, ctypes._CFuncPtr):
-        got = _addresses.get((name, id(_lib)))
-        if got is None:
-            got = _addresses[name, id(_lib)] = ctypes.cast(fn, vp).value
-        return got
-    res, args = SIGNATURES[name]
-    wrapped = ctypes.CFUNCTYPE(res, *args)(fn)
-    _addresses.setdefault('stubs', []).append(wrapped)
-    return ctypes.cast(wrapped, vp).value
+    got = _addresses.get((name, fn))
+    if got is None:
+        if isinstance(fn, ctypes._CFuncPtr):
+            entry = fn
+        else:
+            res, args = SIGNATURES[name]
+            entry = ctypes.CFUNCTYPE(res, *args)(fn)
+        got = _addresses[name, fn] = (ctypes.cast(entry, vp).value, entry)
+    return got[0]
 
 
 class NativeError(RuntimeError):

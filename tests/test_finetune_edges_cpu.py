@@ -246,3 +246,15 @@ def test_configurations_that_trained_before_still_do(stub, name, taken, capsys):
     drivers.optimiser_of(cfg, 1)
     assert capsys.readouterr().out == ''
     TrainStep(_module(None), optim=drivers.optimiser_of(cfg, 1))
+
+
+def test_one_address_per_entry_point(stub, monkeypatch):  # noqa: F811
+    """as many losses as one likes: nothing is added after the first"""
+    from mit_semseg import _native, ops
+    monkeypatch.setattr(_native, '_addresses', {})
+    z, label = torch.randn(2, 5, 3, 4, requires_grad=True), torch.zeros(2, 3, 4, dtype=torch.long)
+    counts = []
+    for _ in range(3):
+        torch.autograd.grad(ops.label_log_prob(z, label).sum(), z)
+        counts.append(sum(len(v) if isinstance(v, list) else 1 for v in _native._addresses.values()))
+    assert counts == [2, 2, 2]
