@@ -247,21 +247,21 @@ def host():
     return _host
 
 
-_addresses = {}             # (name, entry point) -> (its address, what keeps that alive)
+_addresses = {}             # (name, id of the entry point) -> (its address, the entry point and what was made of it, which keep both alive)
 
 
 def address(name):
     """where the entry point `name` of lib() starts, for the extension to call.  An entry point that is a Python function (lib() replaced by
     an object of such) gets one C wrapper, kept like the address itself."""
     fn = getattr(lib(), name)
-    got = _addresses.get((name, fn))
+    got = _addresses.get((name, id(fn)))
     if got is None:
         if isinstance(fn, ctypes._CFuncPtr):
             entry = fn
         else:
             res, args = SIGNATURES[name]
             entry = ctypes.CFUNCTYPE(res, *args)(fn)
-        got = _addresses[name, fn] = (ctypes.cast(entry, vp).value, entry)
+        got = _addresses[name, id(fn)] = (ctypes.cast(entry, vp).value, fn, entry)
     return got[0]
 
 

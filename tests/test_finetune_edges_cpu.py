@@ -258,3 +258,14 @@ def test_one_address_per_entry_point(stub, monkeypatch):  # noqa: F811
         torch.autograd.grad(ops.label_log_prob(z, label).sum(), z)
         counts.append(sum(len(v) if isinstance(v, list) else 1 for v in _native._addresses.values()))
     assert counts == [2, 2, 2]
+
+
+def test_addresses_of_the_built_library():
+    import ctypes
+    import os
+    from mit_semseg import _native
+    if not os.path.exists(_native.LIB_PATH):
+        pytest.skip('the library is not built')
+    for name in ('semseg_label_logp_bwd', 'semseg_scale_by'):
+        first = _native.address(name)
+        assert first == _native.address(name) == ctypes.cast(getattr(_native.lib(), name), ctypes.c_void_p).value
