@@ -394,7 +394,19 @@ PyObject* attach_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
-PyMethodDef methods[] = {{"attach_rows", (PyCFunction)(void*)attach_rows, METH_FASTCALL, nullptr},
+// (what, *tensors or None): refuses tensors that carry a tangent
+PyObject* no_tangents(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const char* what = n ? PyUnicode_AsUTF8(args[0]) : "";
+        if (!what) throw Refused();
+        for (Py_ssize_t i = 1; i < n; ++i)
+            if (args[i] != Py_None) tensor(args[i], what);
+        Py_RETURN_NONE;
+    });
+}
+
+PyMethodDef methods[] = {{"no_tangents", (PyCFunction)(void*)no_tangents, METH_FASTCALL, nullptr},
+                         {"attach_rows", (PyCFunction)(void*)attach_rows, METH_FASTCALL, nullptr},
                          {"adamw_table", (PyCFunction)(void*)adamw_table, METH_FASTCALL, nullptr},
                          {"adamw8_table", (PyCFunction)(void*)adamw8_table, METH_FASTCALL, nullptr},
                          {"grad_table", (PyCFunction)(void*)grad_table, METH_FASTCALL, nullptr},

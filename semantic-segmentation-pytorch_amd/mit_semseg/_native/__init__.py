@@ -237,13 +237,20 @@ def lib():
     return _lib
 
 
+_host_ext = None
+
+
 def host():
     """the CPython extension for host work that Python is too slow for (csrc/host_ext.cpp); raises if it is not built"""
+    global _host_ext
+    if _host_ext is not None:
+        return _host_ext
     try:
         from . import _host
     except ImportError as e:
         raise NativeLibraryMissing('%s/_host.so not built or not loadable (%s): run `python '
                                    'semantic-segmentation-pytorch_amd/build_native.py`' % (_HERE, e))
+    _host_ext = _host
     return _host
 
 

@@ -2314,17 +2314,9 @@ def _device_guard(device):
     return torch.cuda.device(device)
 
 
-def _refuse_tangents(what, *tensors):
-    """a result without a tangent would say that the derivative is zero"""
-    for t in tensors:
-        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
-            raise NotImplementedError('%s: there is no forward-mode derivative' % what)
-
-
 def _row_shape(what, z):
     """shape of one number per row of logits [N, C, H, W] (rows = pixels) or [P, C]; refuses what is not such logits"""
     _require_cuda(z)
-    _refuse_tangents(what, z)
     if z.dtype not in _TYPE_CODES:
         raise TypeError('%s: logits must be float32, bfloat16 or float16, got %s' % (what, z.dtype))
     if z.dim() not in (2, 4):
@@ -2383,6 +2375,7 @@ def label_log_prob(z, label, ignore_index=-1):
     output of log_softmax can be handed in.  Differentiable in z."""
     ignore_index = int(ignore_index)
     rows = _row_shape('label_log_prob', z)
+    _native.host().no_tangents('label_log_prob', z)
     label = _row_labels('label_log_prob', z, rows, label)
     zr, ld, P, c = _logit_rows(z)
     wanted = torch.is_grad_enabled() and z.requires_grad
@@ -2402,7 +2395,6 @@ def label_log_prob(z, label, ignore_index=-1):
 
 def _row_constants(what, name, t, shapes, device):
     _require_cuda(t)
-    _refuse_tangents(what, t)
     if t.requires_grad:
         raise ValueError('%s: %s is a constant of the loss: detach it' % (what, name))
     if not t.dtype.is_floating_point:
@@ -2426,8 +2418,9 @@ def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip
     (label_log_prob under no_grad gives them).  Rows whose label is `ignore_index` or outside [0, C) do not count.
     Returns three scalars: the loss (differentiable in z), the mean KL term (0 without ref_logp) and the share of rows whose clipped
     term is the smaller one; all 0 where no row counts.  For float32 logits of 8 to 320 classes whose rows lie close together the gradient
-    of the logits is written in the forward pass (and its memory taken then).  `scalars`: two float32 on the device that receive the KL
-    term and the share (and are returned as such), for a caller who replays captured steps and reads them in one place."""
+    of the logits is written in the forward pass (and its memory taken then); a second backward pass (retain_graph) computes its own, equal
+    up to rounding.  A backward pass is recorded into a graph only together with its forward pass.  `scalars`: two float32 on the device
+    that receive the KL term and the share (and are returned as such), for a caller who replays captured steps and reads them in one place."""
     clip_low, clip_high, kl_weight = float(clip_low), float(clip_high), float(kl_weight)
     if not 0.0 <= clip_low <= 1.0 or not 0.0 <= clip_high < float('inf'):
         raise ValueError('policy_loss: clip_low must lie in [0, 1] and clip_high must not be negative, got %r, %r' % (clip_low, clip_high))
@@ -2437,6 +2430,7 @@ def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip
         raise ValueError('policy_loss: a KL term needs ref_logp')
     ignore_index, what = int(ignore_index), 'policy_loss'
     dev, rows = z.device, _row_shape(what, z)
+    _native.host().no_tangents(what, z, advantage, old_logp, ref_logp)
     label = _row_labels(what, z, rows, label)
     advantage = _row_constants(what, 'advantage', advantage, ((rows[0],), rows) if len(rows) == 3 else (rows,), dev)
     old_logp = _row_constants(what, 'old_logp', old_logp, (rows,), dev)
