@@ -5,9 +5,9 @@
 //
 // States in 8 bits: m and r = sqrt(v) are e4m3 codes (4 exponent bits, 3 mantissa bits, largest value 448) of blocks of 256 elements
 // with one f32 scale each, scale = absmax / 448.  r and not v: v spans the square of r's range, which 8 bits do not.
-// Rounding is stochastic: between two steps r moves by at most (1 - b2) / 2 = 0.05 % of itself towards a new level, a nearest
-// rounding of 3 mantissa bits moves only at 6 %, so r would stay where it is for ever; a rounding that goes up with the probability of
-// the cut-off fraction is right on average.  Its random bits are a counter hash of (seed, step, tensor, element): the same call gives
+// Rounding is stochastic: from one step to the next r falls by at most (1 - b2) / 2 = 0.05 % of itself (it rises without such a limit, under
+// a gradient much larger than r), a nearest rounding of 3 mantissa bits moves only at 6 %, so r would never come down again; a rounding that
+// goes up with the probability of the cut-off fraction is right on average.  Its random bits are a counter hash of (seed, step, tensor, element): the same call gives
 // the same bits on every machine.  A positive r never rounds to zero (it divides).
 #pragma once
 #include <stdint.h>

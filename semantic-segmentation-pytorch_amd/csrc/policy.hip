@@ -15,7 +15,11 @@
 //  * rows of few classes that lie close together (a map's pixels): a block takes 256 / L rows as one stretch of memory, through LDS;
 //  * longer rows, or rows far apart: 16, 64 or 256 lanes a row, straight from memory, a running maximum and sum;
 //  * few long rows (one token over a vocabulary): several blocks a row, joined by a second kernel.
-// All memory accesses are 16 bytes wide wherever a row starts: the hardware takes them at any element's address.
+// All memory accesses are 16 bytes wide wherever a row starts: the hardware takes them at any element's address, at full rate where that
+// is a multiple of 4 (30100 x 2005 f32, every fourth row aligned: 5.0 TB/s read) and slower where it is not (1024 x 50257 bf16, every other
+// row: 3.2 TB/s; 2048 x 32000, all rows aligned: 4.1).
+// Exponentials are the hardware's exp2 of x log2 e: their relative error grows by 2^-24 for every unit below the row's maximum, where the
+// terms are small.
 #include "common.h"
 
 typedef __bf16 bf16_t;
@@ -52,7 +56,7 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
 
 constexpr int LP_MAX_BLOCKS = 2048;     // partial sums of the loss
 constexpr int COUNT_BLOCKS = 256;       // partial counts of the rows that count
-constexpr int TILE_BYTES = 20480;       // 8 blocks of a compute unit at once
+constexpr int TILE_BYTES = 20480;       // 8 blocks of a compute unit at once, 7 with the 128 to 144 bytes more of the loss's partial sums
 constexpr int MAX_SPLITS = 64;          // blocks of a long row
 
 enum Mode { LOGP, LOSS, GRAD, BACK };   // GRAD: the loss and, for an upstream gradient of 1, the gradient of the logits
@@ -189,9 +193,11 @@ __device__ __forceinline__ float group_sum(float v, float* lds) {
 // ---------------------------------------------------------------- rows of few classes, close together --------------------------
 // A block takes 256 / L rows, padding between them included, as one stretch of memory in 16-byte loads that no row's start or end
 // interrupts, through LDS; then L lanes read a row each and hold it in registers.  A row alone is 300 to 600 bytes at 150 classes.
-// Of 2 x 375 x 501 rows of 150 classes: f32 42 us, f16 25 us (5.4, 4.6 TB/s); a group of lanes per row straight from memory took 64 us in
-// f16.  A gradient leaves the same way.  GRAD: the row is in registers when its loss is known, so its gradient is written at once and the
-// logits are not read by a backward pass (2 x 512 x 512 x 150 f32: loss and gradient 139 us, with a second reading 208 us); it needs
+// Of 2 x 375 x 501 rows of 150 classes: f32 43 us, f16 27 us (5.2, 4.2 TB/s); a group of lanes per row straight from memory took 64 us in
+// f16.  Rows of few classes are far from that rate: a tile has 256 / L rows however short they are, so 375750 rows of 19 classes take 9 to 11
+// us in f32 and 7 in bf16 (2.6 to 3.2 and 2.1 TB/s of logits), 1048576 rows of 2 classes 8 us in both (1.1, 0.5).
+// A gradient leaves the same way.  GRAD: the row is in registers when its loss is known, so its gradient is written at once and the logits
+// are not read by a backward pass (2 x 512 x 512 x 150 f32: loss and gradient 139 us, with a second reading 219 us); it needs
 // 1 / (rows that count) beforehand (count_rows_kernel, 8 bytes a row).
 // W: elements of a read from LDS (2 where classes and pitch are even); HELD: reads of a lane, all unrolled (with a run-time bound the
 // compiler puts the row into scratch memory and f16 rows take five times as long)
@@ -680,9 +686,10 @@ extern "C" size_t semseg_policy_loss_workspace_bytes(int type, int64_t ld, int64
 
 // Whether a loss whose gradient is wanted writes it in its forward pass.  float32 only: an upstream gradient other than 1 multiplies the
 // written values, and 16-bit ones would be rounded twice.  From 8 classes on: counting the rows first costs 8 bytes a row, reading the
-// logits again 4 C.  GPU time of loss and gradient, two passes against one: 262144 x 150 108 against 77 us, 65536 x 150 35.7 against 32.5,
-// 400000 x 19 37.4 against 34.2, 1024 x 150 13.8 against 14.2 (its backward pass is cheaper to issue: 127 against 119 us of wall time),
-// 2000000 x 2 49.4 against 54.5.
+// logits again 4 C.  GPU time of loss and gradient of logits that are in no cache, two passes against one: 524288 x 150 219 against 139 us,
+// 262144 x 150 113 against 75, 65536 x 150 34.6 against 33.3; maps that the cache holds lose by the two launches more: 400000 x 19 32.0 against 33.3,
+// 375750 x 8 23.9 against 25.0, 8192 x 150 14.6 against 15.0, 1024 x 150 13.2 against 13.5 (and 5 us of wall time, of 50 to 75); below 8
+// classes it is 1048576 x 2 29.7 against 35.9.
 constexpr int ONE_PASS_CLASSES = 8;
 static bool one_pass_able(const void* z, int type, int64_t ld, int64_t P, int C) {
     return z && type == SEMSEG_TYPE_F32 && P > 0 && P <= 1 << 30 && C > 0 && ld >= C && plan_of(4, ld, P, C).lanes > 0;
