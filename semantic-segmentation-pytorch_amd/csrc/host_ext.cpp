@@ -14,6 +14,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -51,12 +52,14 @@ struct Seq {                            // a list or tuple, held
     throw Refused();
 }
 
+thread_local bool duals = false;        // whether tensors with a forward-mode tangent exist at all: asked once a call (20 ns a tensor otherwise)
+
 const at::Tensor& tensor(PyObject* o, const char* what) {
     if (!THPVariable_Check(o)) refuse(PyExc_TypeError, "%s: expected a tensor, got %s", what, Py_TYPE(o)->tp_name);
     const at::Tensor& t = THPVariable_Unpack(o);
     if (!t.defined() || t.layout() != at::kStrided) refuse(PyExc_TypeError, "%s: tensors must be strided", what);
     // a result without a tangent would say that the derivative is zero
-    if (t._fw_grad(0).defined()) refuse(PyExc_NotImplementedError, "%s: there is no forward-mode derivative", what);
+    if (duals && t._fw_grad(0).defined()) refuse(PyExc_NotImplementedError, "%s: there is no forward-mode derivative", what);
     return t;
 }
 
@@ -218,6 +221,7 @@ void fill8(semseg_adamw8_tensor& e, const char* what, const at::Tensor& p, const
 template <class F>
 PyObject* guarded(F f) {
     try {
+        duals = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
         return f();
     } catch (const Refused&) {
         return nullptr;
@@ -274,7 +278,11 @@ void* stream_of(const at::Tensor& t) {
 unsigned long long recording_of(const at::Tensor& t) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     unsigned long long id = 0;
-    if (!t.is_cuda() || hipStreamGetCaptureInfo((hipStream_t)stream_of(t), &status, &id) != hipSuccess) return 0;
+    if (!t.is_cuda()) return 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream_of(t), &status, &id) != hipSuccess) {
+        (void)hipGetLastError();                      // the default stream beside another one's capture: nothing is recorded on it
+        return 0;
+    }
     return status == hipStreamCaptureStatusActive ? id : 0;
 }
 void check(int rc, const char* what) {
