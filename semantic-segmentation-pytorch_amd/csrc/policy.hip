@@ -131,9 +131,11 @@ __device__ __forceinline__ float finish_row(int64_t row, const RowIn& in, float 
             if (f.ref_logp) {
                 const float d = in.ref - lp;
                 const float e = expm1f(d);                           // exp(d) - 1 - d cancels for small d
-                const float k = e - d;
-                l = fmaf(f.kl_weight, k, l);
-                coef = fmaf(-f.kl_weight, e, coef);
+                const float k = d < INFINITY ? e - d : d;             // a chosen class of probability 0: infinite, not infinity - infinity
+                if (f.kl_weight > 0.f) {                              // a term that is only watched may be infinite: 0 times it is not 0
+                    l = fmaf(f.kl_weight, k, l);
+                    coef = fmaf(-f.kl_weight, e, coef);
+                }
                 acc.kl += (double)k;
             }
             acc.loss += (double)l;

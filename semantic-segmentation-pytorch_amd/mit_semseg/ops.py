@@ -2417,7 +2417,7 @@ def policy_loss(z, label, advantage, old_logp, ref_logp=None, clip_low=0.2, clip
     advantage: one number per image [N] or one per row (the label's shape); old_logp, ref_logp: the label's shape, constants
     (label_log_prob under no_grad gives them).  Rows whose label is `ignore_index` or outside [0, C) do not count.
     Returns three scalars: the loss (differentiable in z), the mean KL term (0 without ref_logp) and the share of rows whose clipped
-    term is the smaller one; all 0 where no row counts.  For float32 logits of 8 to 320 classes whose rows lie close together the gradient
+    term is the smaller one; all 0 where no row counts.  With kl_weight 0 the KL term is reported only, infinite or not.  For float32 logits of 8 to 320 classes whose rows lie close together the gradient
     of the logits is written in the forward pass (and its memory taken then); a second backward pass (retain_graph) computes its own, equal
     up to rounding.  A backward pass is recorded into a graph only together with its forward pass.  `scalars`: two float32 on the device
     that receive the KL term and the share (and are returned as such), for a caller who replays captured steps and reads them in one place."""
@@ -2613,8 +2613,8 @@ def adamw8_step(params, grads, states, steps, weight_decays, lr_tensor, betas=(0
                 copies=None, seed=0):
     """adamw_step with states in 8 bits: `states` holds one AdamW8State (adamw8_state) per parameter, blocks of ADAMW8_BLOCK
     elements share a scale.  The update itself is computed in 32 bits from the decoded states; they are coded again with stochastic
-    rounding whose random bits come from (seed, step count, index in the list, element): the same call gives the same states.  eps: 0,
-    or a normal float32 up to 2^126."""
+    rounding whose random bits come from (seed, step count, index among the tensors that have elements, element): the same call gives
+    the same states.  eps: 0, or a normal float32 up to 2^126."""
     _check_step('adamw8_step', params, lr_tensor, betas, eps, clip)
     if eps != 0.0 and not 2.0 ** -126 <= eps <= 2.0 ** 126:
         raise ValueError('adamw8_step: eps must be 0 or lie in [2^-126, 2^126], got %r' % eps)

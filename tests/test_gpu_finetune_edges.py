@@ -299,3 +299,23 @@ def test_numbers_changed_between_replays():
         rows.append(torch.stack(seen))
     assert ts.stats['captured'] == 3 and ts.stats['replayed'] == 7, ts.stats
     assert torch.equal(rows[0], rows[1])
+
+
+# ------------------------------------------------------------------------------------------------------ a KL term that is only watched
+@pytest.mark.parametrize('shape', [(2, 150, 9, 13), (2, 2, 9, 13), (1, 700, 9, 13), (1, 40000, 1, 3)], ids=str)
+def test_a_kl_term_of_weight_0_does_not_reach_the_loss(shape):
+    """rows whose reference is e^100 times as likely (exp overflows) or has probability 0, and a chosen class that is masked: with weight 0
+    loss and gradient are, to the bit, those without a reference"""
+    from mit_semseg import ops
+    z, label, adv, old = loss_inputs(50, shape)
+    label.clamp_(min=0)
+    with torch.no_grad():
+        z[0, int(label[0, 0, 0]), 0, 0] = -math.inf
+    ref = old.clone()
+    ref.view(-1)[1], ref.view(-1)[2] = 100.0, -math.inf
+    want, _, clipped = ops.policy_loss(z, label, adv, old)
+    dz = torch.autograd.grad(want, z)[0]
+    loss, kl, share = ops.policy_loss(z, label, adv, old, ref)
+    assert torch.isfinite(want) and torch.equal(loss, want) and torch.equal(share, clipped) and float(kl) == math.inf
+    got = torch.autograd.grad(loss, z)[0]
+    assert torch.isfinite(got).all() and torch.equal(got, dz)
