@@ -475,15 +475,22 @@ __global__ __launch_bounds__(256) void count_rows_kernel(const Rows r, int* __re
     if (threadIdx.x == 0) counts[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// x *= g[0]; nothing to do, and nothing read, where it is 1 (a loss that backward() is called on)
+// x *= g[0]; nothing to do, and nothing read, where it is 1 (a loss that backward() is called on).  A zero stays one under a factor that is not
+// finite (an overflowed loss scale): most are the gradients of rows that do not count
 __global__ __launch_bounds__(256) void scale_by_kernel(float* __restrict__ x, int64_t n, const float* __restrict__ g) {
     const float s = g[0];
     if (s == 1.f) return;
+    const bool plain = fabsf(s) < INFINITY;
     f32x4* x4 = reinterpret_cast<f32x4*>(x);
     const int64_t stride = (int64_t)gridDim.x * 256, quads = n >> 2;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += stride) x4[i] = x4[i] * s;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += stride) {
+        f32x4 v = x4[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = plain || v[j] != 0.f ? v[j] * s : v[j];
+        x4[i] = v;
+    }
     const int64_t i = quads * 4 + (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) x[i] *= s;
+    if (i < n && (plain || x[i] != 0.f)) x[i] *= s;
 }
 
 struct PolicyOut {

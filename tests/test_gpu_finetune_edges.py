@@ -319,3 +319,21 @@ def test_a_kl_term_of_weight_0_does_not_reach_the_loss(shape):
     assert torch.isfinite(want) and torch.equal(loss, want) and torch.equal(share, clipped) and float(kl) == math.inf
     got = torch.autograd.grad(loss, z)[0]
     assert torch.isfinite(got).all() and torch.equal(got, dz)
+
+
+@pytest.mark.parametrize('up', [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize('shape,dtype', [((2, 150, 9, 13), torch.float32), ((1, 9, 5, 7), torch.float32), ((2, 150, 9, 13), torch.bfloat16),
+                                         ((1, 700, 9, 13), torch.float32)], ids=str)
+def test_rows_that_do_not_count_have_no_gradient_under_an_overflowed_scale(shape, dtype, up):
+    """an upstream gradient that is not finite (a loss scale that overflowed): zero for rows that do not count, not finite for the others,
+    whichever pass writes the gradient"""
+    from mit_semseg import ops
+    z, label, adv, old = loss_inputs(51, shape)
+    label[0, 0, :3] = -1
+    z = z.detach().to(dtype).requires_grad_(True)
+    loss = ops.policy_loss(z, label, adv, old)[0]
+    for _ in range(2):                                                # what the forward pass wrote, and a pass of its own
+        dz = torch.autograd.grad(loss, z, grad_outputs=torch.tensor(up, device=dev()), retain_graph=True)[0].permute(0, 2, 3, 1)
+        out = label < 0
+        assert torch.all(dz[out] == 0)
+        assert not torch.isfinite(dz[~out]).all(dim=-1).all()
