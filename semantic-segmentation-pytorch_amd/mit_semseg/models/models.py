@@ -38,7 +38,8 @@ def _repeatable(module, keep_statistics=False):
         if isinstance(m, (Dropout2d, nn.modules.dropout._DropoutNd)):
             dropped.append(m)
         elif keep_statistics and m._buffers.get('running_mean') is not None:
-            kept.append((m._buffers, {k: m._buffers[k] for k in ('running_mean', 'running_var', 'num_batches_tracked')}))
+            names = ('running_mean', 'running_var', 'num_batches_tracked')
+            kept.append((m._buffers, {k: m._buffers[k] for k in names if m._buffers.get(k) is not None}))
     try:
         for m in dropped:
             m.training = False

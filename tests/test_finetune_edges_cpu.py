@@ -184,6 +184,11 @@ def test_log_probabilities_leave_the_module_as_it_was(stub, monkeypatch):  # noq
             assert t is own[k][0] and torch.equal(t, own[k][1]), k
         assert all(m.training for m in sm.modules())
     back()
+    sm.encoder.other = torch.nn.BatchNorm2d(4)                        # a module of the user's with fewer statistics
+    del sm.encoder.other.num_batches_tracked
+    with torch.no_grad():
+        sm.label_log_prob(_feed())
+    del sm.encoder.other
     monkeypatch.setattr(sm.decoder, 'forward', lambda *a, **k: 1 // 0)
     with pytest.raises(ZeroDivisionError):
         sm.label_log_prob(_feed())
