@@ -2372,7 +2372,8 @@ def label_log_prob(z, label, ignore_index=-1):
     """Log probability of the chosen label under softmax over the classes: z [N, C, H, W] (NHWC memory is read in place, with any
     pixel stride) or [P, C], float32 / bfloat16 / float16; label [N, H, W] or [P], integers.  Returns float32 of the label's shape;
     rows whose label is `ignore_index` or outside [0, C) give 0 and a zero gradient.  Log probabilities are logits too, so the
-    output of log_softmax can be handed in.  Differentiable in z."""
+    output of log_softmax can be handed in.  Differentiable in z, once; a backward pass is recorded into a graph only together with its
+    forward pass."""
     ignore_index = int(ignore_index)
     rows = _row_shape('label_log_prob', z)
     _native.host().no_tangents('label_log_prob', z)
