@@ -640,9 +640,10 @@ int semseg_policy_loss_fwd(const void* z, int type, int64_t ld, const int64_t* l
                            float clip_low, float clip_high, float kl_weight, float* stats, float* coef, float* loss, float* kl, float* clipped,
                            float* inv_count, void* dz, void* workspace, size_t workspace_bytes, void* stream);
 /* dz (may be NULL): the gradient of the logits for an upstream gradient of 1, written by the forward call where policy_loss_one_pass says
- * so (float32 rows of 8 to 320 classes that lie close together); scale_by multiplies n floats (16-byte aligned) by a device scalar. */
+ * so (float32 rows of 8 to 320 classes that lie close together); scale_by: out = x g[0], n floats,
+ * both 16-byte aligned; out may be x. */
 int semseg_policy_loss_one_pass(const void* z, int type, int64_t ld, int64_t P, int C);
-int semseg_scale_by(float* x, int64_t n, const float* g, void* stream);
+int semseg_scale_by(float* out, const float* x, int64_t n, const float* g, void* stream);
 int semseg_label_logp_bwd(const void* z, int type, int64_t ld, const int64_t* label, int64_t ignore_index, const float* stats,
                           const float* g, const float* gloss, const float* inv_count, int64_t P, int C, void* dz, void* stream);
 

@@ -269,7 +269,7 @@ PyObject* grad_table(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // ---------------------------------------------------------------- backward of the per-row losses -------------------------------
 typedef int (*LogpBackward)(const void*, int, int64_t, const int64_t*, int64_t, const float*, const float*, const float*, const float*, int64_t,
                             int, void*, void*);
-typedef int (*ScaleBy)(float*, int64_t, const float*, void*);
+typedef int (*ScaleBy)(float*, const float*, int64_t, const float*, void*);
 
 void* stream_of(const at::Tensor& t) {
     return t.is_cuda() ? (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream() : nullptr;
@@ -291,9 +291,9 @@ void check(int rc, const char* what) {
 
 // d logits of label_log_prob (kept: {maximum, log sum} per row) and of policy_loss (kept: scratch, the same, gradient per row, 1 / rows
 // that count; `written`: the gradient for an upstream gradient of 1, where the forward pass has written it).
-// `written` is scaled in place and handed out, so it is taken only where the forward pass runs once for every backward pass: both eager, or
-// both in one recording.  A recorded forward pass would write over a gradient that an eager backward pass has handed out.  A backward pass
-// that is recorded while its forward pass was eager is refused: every replay would scale `written` once more, and what is kept for it is the
+// `written` is scaled in place and handed out where the forward pass runs once for every backward pass: both eager, or both in one recording.
+// Where the forward pass was recorded apart (its replays write `written` again), the product goes to memory of its own.  A backward pass that is
+// recorded while its forward pass was eager is refused: every replay would scale `written` once more, and what is kept for it is the
 // eager pass's memory, free for other tensors once the node is gone.
 struct RowsBackward : public torch::autograd::Node {
     torch::autograd::SavedVariable z, label, kept;
@@ -315,7 +315,7 @@ struct RowsBackward : public torch::autograd::Node {
     }
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         if (!grads[0].defined()) return {at::Tensor()};
-        at::Tensor zt, lab, keep, dz;
+        at::Tensor zt, lab, keep, dz, again;
         {
             std::lock_guard<std::mutex> lock(mutex_);
             zt = z.unpack(shared_from_this());
@@ -324,6 +324,7 @@ struct RowsBackward : public torch::autograd::Node {
             const auto now = recording_of(zt);
             TORCH_CHECK(!now || recording, name(), ": a backward pass cannot be recorded apart from its forward pass: record both");
             if (now == recording) std::swap(dz, written);
+            else again = written;
         }
         {
             at::AutoDispatchBelowADInplaceOrView below;
@@ -339,8 +340,10 @@ struct RowsBackward : public torch::autograd::Node {
             const float* kp = (const float*)keep.const_data_ptr();
             const float* inv = loss && P ? kp + keep.numel() - 1 : nullptr;
             const float* coef = loss ? inv - P : nullptr;
-            if (dz.defined()) {                       // handed out once: a second backward pass computes its own
-                check(scale_by((float*)dz.mutable_data_ptr(), dz.numel(), (const float*)g.const_data_ptr(), stream_of(zt)), "scale_by");
+            if (again.defined()) dz = at::empty_strided(again.sizes(), again.strides(), again.options());
+            if (dz.defined()) {                       // handed out once: a second eager backward pass computes its own
+                const void* from = again.defined() ? again.const_data_ptr() : dz.const_data_ptr();
+                check(scale_by((float*)dz.mutable_data_ptr(), (const float*)from, dz.numel(), (const float*)g.const_data_ptr(), stream_of(zt)), "scale_by");
             } else {
                 dz = shape.size() == 2 ? at::empty(shape, zt.options())
                                        : at::empty({shape[0], shape[2], shape[3], shape[1]}, zt.options()).permute({0, 3, 1, 2});

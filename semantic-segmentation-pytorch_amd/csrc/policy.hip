@@ -475,22 +475,23 @@ __global__ __launch_bounds__(256) void count_rows_kernel(const Rows r, int* __re
     if (threadIdx.x == 0) counts[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// x *= g[0]; nothing to do, and nothing read, where it is 1 (a loss that backward() is called on).  A zero stays one under a factor that is not
+// out = x g[0]; in place there is nothing to do, and nothing read, where it is 1 (a loss that backward() is called on).  A zero stays one under a factor that is not
 // finite (an overflowed loss scale): most are the gradients of rows that do not count
-__global__ __launch_bounds__(256) void scale_by_kernel(float* __restrict__ x, int64_t n, const float* __restrict__ g) {
+__global__ __launch_bounds__(256) void scale_by_kernel(float* out, const float* x, int64_t n, const float* __restrict__ g) {
     const float s = g[0];
-    if (s == 1.f) return;
+    if (s == 1.f && out == x) return;
     const bool plain = fabsf(s) < INFINITY;
-    f32x4* x4 = reinterpret_cast<f32x4*>(x);
+    const f32x4* x4 = reinterpret_cast<const f32x4*>(x);
+    f32x4* o4 = reinterpret_cast<f32x4*>(out);
     const int64_t stride = (int64_t)gridDim.x * 256, quads = n >> 2;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += stride) {
         f32x4 v = x4[i];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = plain || v[j] != 0.f ? v[j] * s : v[j];
-        x4[i] = v;
+        o4[i] = v;
     }
     const int64_t i = quads * 4 + (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n && (plain || x[i] != 0.f)) x[i] *= s;
+    if (i < n) out[i] = plain || x[i] != 0.f ? x[i] * s : x[i];
 }
 
 struct PolicyOut {
@@ -707,10 +708,10 @@ extern "C" int semseg_policy_loss_one_pass(const void* z, int type, int64_t ld, 
     return one_pass_able(z, type, ld, P, C) && C >= ONE_PASS_CLASSES;
 }
 
-extern "C" int semseg_scale_by(float* x, int64_t n, const float* g, void* stream) {
-    if (!x || !g || n <= 0 || !aligned16(x)) return SEMSEG_EINVAL;
+extern "C" int semseg_scale_by(float* out, const float* x, int64_t n, const float* g, void* stream) {
+    if (!out || !x || !g || n <= 0 || !aligned16(out) || !aligned16(x)) return SEMSEG_EINVAL;
     const int64_t b = (n / 4 + 1023) / 1024;
-    hipLaunchKernelGGL(scale_by_kernel, dim3((unsigned)(b < 1 ? 1 : b > 2048 ? 2048 : b)), dim3(256), 0, (hipStream_t)stream, x, n, g);
+    hipLaunchKernelGGL(scale_by_kernel, dim3((unsigned)(b < 1 ? 1 : b > 2048 ? 2048 : b)), dim3(256), 0, (hipStream_t)stream, out, x, n, g);
     SEMSEG_LAUNCH_CHECK();
     return 0;
 }

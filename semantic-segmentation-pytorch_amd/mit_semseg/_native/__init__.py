@@ -175,7 +175,7 @@ SIGNATURES = {
     'semseg_policy_loss_workspace_bytes': (c_sz, [c_int, c_l, c_l, c_int]),
     'semseg_policy_loss_fwd': (c_int, [vp, c_int, c_l, vp, c_l, c_l, c_int, vp, c_l, vp, vp, c_f, c_f, c_f] + [vp] * 8 + [c_sz, vp]),
     'semseg_policy_loss_one_pass': (c_int, [vp, c_int, c_l, c_l, c_int]),
-    'semseg_scale_by': (c_int, [vp, c_l, vp, vp]),
+    'semseg_scale_by': (c_int, [vp, vp, c_l, vp, vp]),
     'semseg_label_logp_bwd': (c_int, [vp, c_int, c_l, vp, c_l, vp, vp, vp, vp, c_l, c_int, vp, vp]),
     'semseg_weights_absmax_slots': (vp, [vp, c_int, c_int, c_int]),
     'semseg_weights_prepare_h2_after_sgd': (c_int, [ctypes.POINTER(WPrepTensor), c_int, c_int, vp]),

@@ -337,3 +337,35 @@ def test_rows_that_do_not_count_have_no_gradient_under_an_overflowed_scale(shape
         out = label < 0
         assert torch.all(dz[out] == 0)
         assert not torch.isfinite(dz[~out]).all(dim=-1).all()
+
+
+def test_policy_step_in_segments_equals_eager():
+    """a step recorded as a chain of graphs (collectives between them, forced on one rank) has its loss and its backward pass in recordings
+    of their own: losses and weights are the eager ones to the bit, at every replay"""
+    from mit_semseg import ops
+    from mit_semseg.engine import TrainStep
+    from mit_semseg.models import ModelBuilder, PolicyLoss, SegmentationModule, resnet
+    from mit_semseg.models.models import ResnetDilated
+    prev, out = ops._SYNC_GROUP['force'], []
+    ops._SYNC_GROUP['force'] = True
+    try:
+        for graph in (False, True):
+            torch.manual_seed(11)
+            enc = ResnetDilated(resnet.resnet18(pretrained=False), 8)
+            sm = SegmentationModule(enc, ModelBuilder.build_decoder('c1', fc_dim=512, num_class=150), PolicyLoss(kl_weight=0.05)).to(dev()).train()
+            ts = TrainStep(sm, lr_encoder=1e-5, lr_decoder=1e-4, max_iters=100, optim='AdamW', clip_grad_norm=0.5, graph=graph)
+            g = torch.Generator().manual_seed(12)
+            feed = {'img_data': torch.randn(2, 3, 64, 96, generator=g).to(dev()), 'seg_label': torch.randint(-1, 150, (2, 8, 12), generator=g).to(dev()),
+                    'advantage': torch.randn(2, generator=g).to(dev()), 'old_logp': (-5 + 0.5 * torch.randn(2, 8, 12, generator=g)).to(dev()),
+                    'ref_logp': (-5 + 0.5 * torch.randn(2, 8, 12, generator=g)).to(dev())}
+            losses = []
+            for _ in range(6):
+                loss, _ = ts.step(feed)
+                losses.append(loss.clone())
+                torch.cuda.synchronize()
+            out.append(losses + [p.detach().clone() for p in sm.parameters()])
+    finally:
+        ops._SYNC_GROUP['force'] = prev
+    assert ts.stats['replayed'] >= 3 and ts.launch_mode() != 'eager'
+    assert ts._graph.counts().get('allreduce', 0) > 0                 # really a chain
+    assert all(torch.equal(a, b) for a, b in zip(*out))
